@@ -276,6 +276,134 @@ BLAZE_API int blazeQuantizeFp8RowGroups(const void* x, int64_t ldx, int32_t rows
 BLAZE_API int blazeQuantizeFp8Blocks(const void* w, int64_t ldw, int32_t N, int32_t K, void* codes, int64_t ld_codes,
                                      void* scales, void* stream);
 
+/* ------------------------------------------------------------------------------------------------------------
+ * Paged key / value cache in 8 bits, and the three operators a serving step needs around it: the block tables and slot
+ * maps of the step (blazeCacheAssign), the quantising store of its keys and values (blazeCacheStore) and the attention
+ * over the cache (blazeCacheAttention).  They sit between the GEMM that makes Q, K and V and the one that takes the
+ * attention's output.  No counterpart in the reference.
+ *
+ * A cache holds `num_blocks` blocks of `block_size` tokens; a request owns the blocks that its row of the block table
+ * names, token p of the request being row p % block_size of block table[p / block_size].  Codes are E4M3, with one
+ * float32 scale per (block, kv head) for K and one for V: value = code * scale.
+ * Constraints: block_size 16, 32, 64 or 128; head_dim 64 or 128; base pointers 16-byte aligned and strides multiples
+ * of 16 bytes, so both [block][head][token][dim] and [block][token][head][dim] orders work (in the first one a (block,
+ * head) page is one contiguous run).
+ * ------------------------------------------------------------------------------------------------------------ */
+typedef struct {
+    size_t struct_size;    /* sizeof(blazeKvCache) */
+    int32_t elem;          /* BLAZE_ELEM_E4M3 */
+    int32_t num_blocks, block_size, kv_heads, head_dim;
+    int32_t reserved;
+    void* k;               /* device codes: (block, head, token) starts block * block_stride + head * head_stride + */
+    void* v;               /* token * token_stride bytes behind the base, head_dim bytes long */
+    int64_t block_stride, head_stride, token_stride;
+    void* k_scale;         /* device float32, (block, head) at block * scale_stride + head; positive and finite */
+    void* v_scale;
+    int64_t scale_stride;  /* elements */
+} blazeKvCache;
+
+/* The step's bookkeeping on the GPU.  Request r has cached_len[r] tokens in the cache; new_len[r] > 0 appends that many,
+ * new_len[r] < 0 ends the request (its blocks go back to the stack of free blocks), 0 leaves it as it is.
+ *   - free stack: free_blocks[0 .. free_count); the blocks of ended requests are pushed in request order, table order,
+ *     then the blocks that growing requests need are popped from the top, in request order;
+ *   - a request is denied when the blocks that it and the requests before it need are not there, when its row of the
+ *     table is too short, or when its rows end behind max_tokens: it gets no blocks, its kv_len stays cached_len and its
+ *     slots are -1.  Later requests that need no block are still served;
+ *   - row_offsets[requests + 1]: first row of each request in the packed batch of new tokens (row_offsets[0] = 0), as if
+ *     none were denied; capped at max_tokens;
+ *   - slots[max_tokens]: block * block_size + row of each packed row, -1 for rows of denied requests and behind the last
+ *     request's; positions[max_tokens] (optional): the token's position in its request, -1 behind the last row;
+ *   - block_table entries behind a request's last block, and of ended requests, are left as they were.
+ * Nothing is read back to the host.  kv_len may be cached_len and free_count_out may be free_count (in place); without
+ * that, repeating a call with the same inputs repeats its outputs.  Lengths are clamped to what the table can hold and
+ * pushes to free_capacity, so no value of the length arrays makes the call leave its buffers.
+ * Constraints: requests <= 8192; max_blocks * block_size and requests * max_blocks below 2^31. */
+typedef struct {
+    size_t struct_size;        /* sizeof(blazeCacheAssignArgs) */
+    int32_t requests;
+    int32_t block_size;        /* 16, 32, 64 or 128 */
+    int32_t max_blocks;        /* columns of the block table that a request may use */
+    int32_t max_tokens;        /* entries of slots and positions */
+    const void* cached_len;    /* device int32[requests] */
+    const void* new_len;       /* device int32[requests] */
+    void* block_table;         /* device int32 [requests][table_stride] */
+    int64_t table_stride;      /* elements, >= max_blocks */
+    void* free_blocks;         /* device int32[free_capacity] */
+    int32_t free_capacity;
+    int32_t reserved;
+    const void* free_count;    /* device int32[1] */
+    void* free_count_out;      /* device int32[1] */
+    void* row_offsets;         /* device int32[requests + 1] */
+    void* kv_len;              /* device int32[requests] */
+    void* slots;               /* device int64[max_tokens] */
+    void* positions;           /* device int32[max_tokens] or NULL */
+    void* denied;              /* device int32[1], the number of denied requests, or NULL */
+} blazeCacheAssignArgs;
+BLAZE_API int blazeCacheAssign(const blazeCacheAssignArgs* args, void* stream);
+
+/* Quantising store: row t of k and v goes to slot slots[t] of the cache; rows whose slot is outside the cache (such as
+ * -1) are skipped.  Per (block, head) and for K and V on their own: with amax the largest finite magnitude among the
+ * rows that go to the block, need = the smallest power of two with amax <= 448 * need, its exponent kept within
+ * [-64, 120]; a block whose first row is among them gets scale = need, any other block
+ * scale = max(old scale, need).  Codes are E4M3(x / scale), to nearest even, saturating, NaN as NaN.  Where the scale of
+ * a block rises, the codes of the rows below the first new one become E4M3(code * (old / new)); since scales are powers
+ * of two that is exact down to E4M3's subnormals.
+ * The rows of one block are neighbours in the call (as blazeCacheAssign lays them out) and, the call's lowest row apart,
+ * nothing is assumed about their order; a slot that is named twice among them keeps the last row.  A block that is named
+ * again further on in the call, with another block between, would be written by two warps at once: don't. */
+typedef struct {
+    size_t struct_size;        /* sizeof(blazeCacheStoreArgs) */
+    int32_t tokens;
+    int32_t in_type;           /* BLAZE_OUT_BF16 or BLAZE_OUT_F16: type of k and v */
+    const void* k;             /* device [tokens][kv_heads][head_dim], 16-byte aligned */
+    const void* v;
+    int64_t k_token_stride, k_head_stride;   /* elements, multiples of 8 */
+    int64_t v_token_stride, v_head_stride;
+    const void* slots;         /* device int64[tokens] */
+} blazeCacheStoreArgs;
+BLAZE_API int blazeCacheStore(const blazeKvCache* cache, const blazeCacheStoreArgs* args, void* stream);
+
+/* Attention of a packed batch of queries over the cache: request r's query rows are row_offsets[r] .. row_offsets[r+1],
+ * its keys and values the first kv_len[r] tokens of its blocks (the step's own tokens among them, stored before).  Query i
+ * of a request's n stands at position p = kv_len - n + i; it sees token j < kv_len when (not causal or j <= p) and
+ * (window == 0 or j > p - window).  Query head h reads kv head h / (heads / kv_heads).
+ *   out[row][h] = sum_j softmax_j(scale * q . K_j) V_j,   lse[row][h] = ln sum_j exp(scale * q . K_j)
+ * A row that sees nothing gives zeros and lse = -inf.  Nothing that a row does not see reaches its result, NaN codes
+ * there and in the blocks' unused rows included.  Rows outside every request are left as they were.
+ * A token whose block number is outside the cache counts as not seen and the device status word reports code 8.
+ * Scores, softmax and sums are float32; probabilities are rounded to half (11 bits) for the product with V.
+ * max_q and max_kv bound the requests' rows and kv_len (lengths above are cut to them; max_kv may not pass max_blocks *
+ * block_size); min_q is a hint: a bound from below on the rows of every request that has any, 0 if unknown.  The result
+ * does not depend on how the work is split over the SMs beyond float32 rounding, and is the same from run to run.
+ * The workspace needs no initialisation and keeps nothing between calls; calls that may overlap on the GPU need one
+ * each. */
+typedef struct {
+    size_t struct_size;        /* sizeof(blazeCacheAttentionArgs) */
+    int32_t requests;          /* <= 8192 */
+    int32_t tokens;            /* rows of q and out */
+    int32_t heads;             /* query heads, a multiple of the cache's kv_heads */
+    int32_t q_type;            /* BLAZE_OUT_BF16 or BLAZE_OUT_F16: type of q and out */
+    const void* q;             /* device [tokens][heads][head_dim], 16-byte aligned */
+    int64_t q_token_stride, q_head_stride;       /* elements, multiples of 8 */
+    void* out;                 /* device [tokens][heads][head_dim], 16-byte aligned */
+    int64_t out_token_stride, out_head_stride;   /* elements, multiples of 8 */
+    void* lse;                 /* device float32 [tokens][heads] or NULL */
+    const void* row_offsets;   /* device int32[requests + 1], not falling */
+    const void* kv_len;        /* device int32[requests] */
+    const void* block_table;   /* device int32 [requests][table_stride] */
+    int64_t table_stride;      /* elements, >= max_blocks */
+    int32_t max_blocks;
+    int32_t max_q, min_q, max_kv;
+    float scale;               /* finite */
+    int32_t causal;            /* 0 or 1 */
+    int32_t window;            /* 0 = none */
+    int32_t sm_limit;          /* 0 = all SMs */
+    void* workspace;           /* device, 256-byte aligned */
+    size_t workspace_bytes;
+} blazeCacheAttentionArgs;
+BLAZE_API int blazeCacheAttentionWorkspaceSize(const blazeKvCache* cache, const blazeCacheAttentionArgs* args, size_t* bytes);
+BLAZE_API int blazeCacheAttention(const blazeKvCache* cache, const blazeCacheAttentionArgs* args, void* stream);
+
 /* D = A + C on n floats: the CUDA stand-in for the reference's only shipped operator
  * (src/add/add_kernel.cpp:173-189). */
 BLAZE_API int blazeAddF32(const void* A, const void* C, void* D, int64_t n, void* stream);

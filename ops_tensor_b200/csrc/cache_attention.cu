@@ -1,0 +1,741 @@
+// Attention over the paged 8-bit cache.
+//
+//   t_j = (q . k8_j) * c_b + L_b      c_b = scale * log2(e) * k_scale_b,  L_b = log2(v_scale_b)
+//   m = max t_j - 15,  p_j = 2^(t_j - m),  O = sum p_j v8_j,  l = sum p_j / v_scale_b
+//   out = O / l,  lse = (m + log2 l) * ln 2
+//
+// for the codes k8, v8 of block b's tokens: with the V scale in the exponent neither K nor V is ever multiplied by its
+// scale, the codes enter the matrix products as they are (E4M3 is a subset of half), and what is rounded to half is
+// p_j relative to the largest p_j * v_scale of its row.
+//
+// The few-rows kernel (decode steps and short runs of tokens) is bound by the bytes of the cache.  A block has one
+// warp that fetches tiles of 64 tokens into a ring in shared memory by TMA (one box per page and operand, 128-byte
+// swizzle: 64-byte for 64-wide heads) and four warps that each take 16 of a tile's tokens through both products with
+// m16n8k16 instructions, with a running maximum, sum and output of their own, joined once per piece.  The order of the k
+// index of a product is free, so a lane reads 16 consecutive code bytes and converts them in registers; the swizzle
+// makes these reads free of bank conflicts for both operands.
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+#include <cuda_runtime.h>
+#include <cmath>
+
+#include "cache.h"
+#include "cache_schedule.cuh"
+#include "cann_ops_tensor_types.h"
+#include "launch.h"
+#include "ptx.cuh"
+
+namespace blaze {
+
+constexpr int kFewRows = 16;          // packed rows of a row tile
+constexpr int kFewTokens = 64;        // tokens of a tile
+constexpr int kFewWarps = 4;          // computing warps, 16 tokens of a tile each
+constexpr int kFewThreads = 32 * (kFewWarps + 1);
+constexpr int kFewStages = 4;
+
+template <int kDim>
+struct FewSmem {
+    static constexpr int kTileBytes = kFewTokens * kDim;             // of K, and of V
+    static constexpr int kStageBytes = 2 * kTileBytes;
+    static constexpr int kPitch = kDim + 4;                          // floats of a row of a warp's output
+    static constexpr int kJoinOffset = kFewStages * kStageBytes;
+    static constexpr int kMlOffset = kJoinOffset + kFewWarps * kFewRows * kPitch * 4;
+    static constexpr int kMetaOffset = kMlOffset + kFewWarps * kFewRows * 2 * 4;    // float4 per stage and warp
+    static constexpr int kBarOffset = kMetaOffset + kFewStages * kFewWarps * 16;
+    static constexpr int kMiscOffset = kBarOffset + 2 * kFewStages * 8;
+    static constexpr int kPrefixOffset = kMiscOffset + 64;
+    static int bytes(int requests) { return 1024 + kPrefixOffset + (requests + 1) * 4; }
+};
+
+__device__ __forceinline__ void mma_f16(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+    asm volatile(
+        "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
+        : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+        : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+
+// Two E4M3 codes (the low or the high half of w) as two halves.
+__device__ __forceinline__ uint32_t codes_lo(uint32_t w) {
+    const __half2_raw r = __nv_cvt_fp8x2_to_halfraw2((__nv_fp8x2_storage_t)(w & 0xFFFFu), __NV_E4M3);
+    return *reinterpret_cast<const uint32_t*>(&r);
+}
+__device__ __forceinline__ uint32_t codes_hi(uint32_t w) {
+    const __half2_raw r = __nv_cvt_fp8x2_to_halfraw2((__nv_fp8x2_storage_t)(w >> 16), __NV_E4M3);
+    return *reinterpret_cast<const uint32_t*>(&r);
+}
+// 0xFF in every byte that is an E4M3 NaN.
+__device__ __forceinline__ uint32_t nan_bytes(uint32_t w) { return __vcmpeq4(w & 0x7F7F7F7Fu, 0x7F7F7F7Fu); }
+
+__device__ __forceinline__ void tma_load_page(uint32_t dst, const CUtensorMap* map, uint32_t bar, int row, int head, int block) {
+    asm volatile(
+        "cp.async.bulk.tensor.4d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5, %6}], [%2];" ::"r"(dst),
+        "l"(reinterpret_cast<uint64_t>(map)), "r"(bar), "r"(0), "r"(row), "r"(head), "r"(block)
+        : "memory");
+}
+
+// A named barrier of the computing warps.
+__device__ __forceinline__ void compute_sync() { asm volatile("bar.sync 1, %0;" ::"n"(32 * kFewWarps) : "memory"); }
+
+// Power of two that brings the largest magnitude of a row of bf16 queries to [2^14, 2^15), so that the row fits half
+// with all its bits; 1 for half queries, which are taken as they are.
+__device__ __forceinline__ int query_shift(float amax) {
+    const int e = (int)(__float_as_uint(amax) >> 23) - 127;
+    return amax > 0.0f ? min(max(14 - e, -120), 120) : 0;
+}
+__device__ __forceinline__ float pow2i(int e) { return __uint_as_float((uint32_t)(e + 127) << 23); }
+
+template <int kDim, bool kBf16>
+__global__ void __launch_bounds__(kFewThreads, 2)
+cache_attention_few_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v,
+                           const CacheAttentionParams p) {
+    using L = FewSmem<kDim>;
+    constexpr int kSteps = kDim / 16;          // k16 steps of Q K^T
+    constexpr int kTiles = kDim / 8;           // n8 tiles of P V
+    extern __shared__ uint8_t few_smem_raw[];
+    uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(few_smem_raw) + 1023) & ~uintptr_t(1023));
+    float* join = reinterpret_cast<float*>(smem + L::kJoinOffset);
+    float* ml = reinterpret_cast<float*>(smem + L::kMlOffset);
+    float4* meta = reinterpret_cast<float4*>(smem + L::kMetaOffset);
+    uint64_t* full = reinterpret_cast<uint64_t*>(smem + L::kBarOffset);
+    uint64_t* empty = full + kFewStages;
+    int* misc = reinterpret_cast<int*>(smem + L::kMiscOffset);
+    volatile int* abort_flag = misc + 8;
+    int* prefix = reinterpret_cast<int*>(smem + L::kPrefixOffset);
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+
+    if (threadIdx.x == 0) {
+        for (int s = 0; s < kFewStages; ++s) {
+            mbar_init(&full[s], 1);
+            mbar_init(&empty[s], kFewWarps);
+        }
+        *abort_flag = 0;
+        fence_mbar_init();
+        tma_prefetch_desc(&map_k);
+        tma_prefetch_desc(&map_v);
+    }
+    grid_dependency_wait();
+    attn_prefix<kFewRows, kFewTokens>(p, prefix, misc);
+    const int total = prefix[p.requests];
+    const int chunk = attn_chunk(p, total, gridDim.x);
+    const long long begin64 = (long long)blockIdx.x * chunk;
+    const int begin = (int)min(begin64, (long long)total);
+    const int end = (int)min(begin64 + chunk, (long long)total);
+
+    if (warp == kFewWarps) {
+        // ------------------------------------------------------------------ fetching warp
+        const int bs = 1 << p.block_shift;
+        const int box_rows = min(bs, kFewTokens);
+        const uint32_t box_bytes = (uint32_t)box_rows * kDim;
+        const int boxes = kFewTokens / box_rows;
+        int stage = 0;
+        uint32_t phase = 0;
+        bool ok = true;
+        for (int u = begin; u < end && ok;) {
+            const AttnPiece s = attn_piece<kFewRows, kFewTokens>(p, prefix, u, end);
+            u += max(1, s.tile1 - s.tile0);
+            const int* table = p.table + (long long)s.r * p.table_stride;
+            // Lane i holds page `base + i` of the request: block number and scales, fetched 32 pages at a time and one
+            // batch ahead of their use.  A batch starts at the page of a tile's first token, so no tile crosses one.
+            auto fetch = [&](int base, int& block, float& ks, float& vs) {
+                const int page = base + lane;
+                const bool in = page < p.max_blocks && ((page + 1) << p.block_shift) > s.lo && (page << p.block_shift) < s.hi;
+                block = in ? table[page] : -1;
+                if (in && (block < 0 || block >= p.num_blocks)) {
+                    atomicCAS(p.status, 0, DEV_BAD_CACHE_BLOCK);
+                    block = -1;
+                }
+                ks = vs = 0.0f;
+                if (block >= 0) {
+                    ks = p.k_scale[(long long)block * p.scale_stride + s.head];
+                    vs = p.v_scale[(long long)block * p.scale_stride + s.head];
+                }
+            };
+            int base = (s.tile0 * kFewTokens) >> p.block_shift;
+            int blk, blk2;
+            float ks, vs, ks2, vs2;
+            fetch(base, blk, ks, vs);
+            fetch(base + 32, blk2, ks2, vs2);
+            for (int t = s.tile0; t < s.tile1; ++t) {
+                const int page0 = (t * kFewTokens) >> p.block_shift;
+                if (page0 >= base + 32) {
+                    base += 32;
+                    blk = blk2; ks = ks2; vs = vs2;
+                    fetch(base + 32, blk2, ks2, vs2);
+                }
+                // lanes 0..3: the tile's groups of 16 tokens
+                const int tok = t * kFewTokens + (lane & 3) * 16;
+                const int src = (tok >> p.block_shift) - base;
+                const int block = __shfl_sync(0xffffffffu, blk, src);
+                const float k_s = __shfl_sync(0xffffffffu, ks, src), v_s = __shfl_sync(0xffffffffu, vs, src);
+                ok = mbar_wait(&empty[stage], phase ^ 1, abort_flag, p.status, DEV_TIMEOUT_SMEM_EMPTY);
+                ok = __all_sync(0xffffffffu, ok);
+                if (!ok) break;
+                // a box (a page, or 64 tokens of one) is loaded when any of its tokens is seen and its block exists
+                const bool leader = lane < 4 && (lane * 16) % box_rows == 0;
+                const bool load = leader && block >= 0 && tok < s.hi && tok + box_rows > s.lo;
+                const uint32_t loads = __ballot_sync(0xffffffffu, load);
+                if (lane < 4) {
+                    const bool seen = block >= 0 && tok < s.hi && tok + 16 > s.lo;
+                    const float lv = fmaxf(lg2(v_s), kMinLogScale);
+                    meta[stage * kFewWarps + lane] =
+                        make_float4(k_s * p.scale_log2, seen ? lv : -INFINITY, ex2(-lv), 0.0f);
+                }
+                __syncwarp();
+                if (lane == 0) mbar_arrive_expect_tx(&full[stage], (uint32_t)__popc(loads) * 2u * box_bytes);
+                __syncwarp();
+                if (load) {
+                    const uint32_t dst = smem_u32(smem + stage * L::kStageBytes) + (uint32_t)lane * 16u * kDim;
+                    const uint32_t bar = smem_u32(&full[stage]);
+                    const int row = tok & (bs - 1);
+                    tma_load_page(dst, &map_k, bar, row, s.head, block);
+                    tma_load_page(dst + L::kTileBytes, &map_v, bar, row, s.head, block);
+                }
+                __syncwarp();
+                if (++stage == kFewStages) { stage = 0; phase ^= 1; }
+            }
+        }
+        (void)boxes;
+        grid_launch_dependents();
+    } else {
+        // ------------------------------------------------------------------ computing warps
+        const int g = lane >> 2, c = lane & 3;         // row g and g + 8 of the tile; column pair of an instruction
+        int stage = 0;
+        uint32_t phase = 0;
+        bool ok = true;
+        for (int u = begin; u < end && ok;) {
+            const AttnPiece s = attn_piece<kFewRows, kFewTokens>(p, prefix, u, end);
+            const int u_next = u + max(1, s.tile1 - s.tile0);
+            // ---- queries of this lane's two rows, as half
+            uint32_t qf[kSteps][4];
+            float c_row[2];
+            int see_lo[2], see_hi[2];                  // tokens that the row sees
+            const int off = s.req.kv - s.req.qlen;
+#pragma unroll
+            for (int e = 0; e < 2; ++e) {
+                const int row = s.row0 + g + 8 * e;
+                const bool there = row < s.rows;
+                const int i = there ? row / p.group : 0;
+                const int head = s.head * p.group + (there ? row - i * p.group : 0);
+                const int pos = off + i;
+                see_hi[e] = there ? (p.causal ? min(s.req.kv, pos + 1) : s.req.kv) : 0;
+                see_lo[e] = p.window > 0 ? max(0, pos - p.window + 1) : 0;
+                const uint16_t* src = static_cast<const uint16_t*>(p.q) + (long long)(s.req.q0 + i) * p.q_token_stride +
+                                      (long long)head * p.q_head_stride;
+                uint4 w[kSteps / 2];                   // 16 dims (two loads) for every four steps
+#pragma unroll
+                for (int k = 0; k < kSteps / 2; ++k) {
+                    const int dim = kDim == 128 ? (2 * c + (k >> 1)) * 16 + (k & 1) * 8 : c * 16 + k * 8;
+                    w[k] = there ? *reinterpret_cast<const uint4*>(src + dim) : make_uint4(0, 0, 0, 0);
+                }
+                float mul = 1.0f;
+                int shift = 0;
+                if constexpr (kBf16) {
+                    float amax = 0.0f;
+#pragma unroll
+                    for (int k = 0; k < kSteps / 2; ++k) {
+                        const uint32_t* x = &w[k].x;
+#pragma unroll
+                        for (int h = 0; h < 4; ++h) {
+                            const uint32_t a = x[h] & 0x7FFFu, b = (x[h] >> 16) & 0x7FFFu;
+                            amax = fmaxf(amax, __uint_as_float((a < 0x7F80u ? a : 0u) << 16));
+                            amax = fmaxf(amax, __uint_as_float((b < 0x7F80u ? b : 0u) << 16));
+                        }
+                    }
+                    amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, 1));
+                    amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, 2));
+                    shift = query_shift(amax);
+                    mul = pow2i(shift);
+                }
+                c_row[e] = pow2i(-shift);
+#pragma unroll
+                for (int k = 0; k < kSteps / 2; ++k) {
+                    const uint32_t* x = &w[k].x;
+#pragma unroll
+                    for (int h = 0; h < 4; ++h) {
+                        uint32_t v = x[h];
+                        if constexpr (kBf16)
+                            v = pack_f16(__uint_as_float(v << 16) * mul, __uint_as_float(v & 0xFFFF0000u) * mul);
+                        qf[2 * k + (h >> 1)][(h & 1) * 2 + e] = v;    // words 0, 1: step 2k; words 2, 3: step 2k + 1
+                    }
+                }
+            }
+            // every row of the tile sees the tokens [all_lo, all_hi)
+            const int i_first = s.row0 / p.group, i_last = (min(s.rows, s.row0 + kFewRows) - 1) / p.group;
+            const int all_hi = p.causal ? min(s.req.kv, off + i_first + 1) : s.req.kv;
+            const int all_lo = p.window > 0 ? max(0, off + i_last - p.window + 1) : 0;
+
+            float o[kTiles][4];
+#pragma unroll
+            for (int j = 0; j < kTiles; ++j) o[j][0] = o[j][1] = o[j][2] = o[j][3] = 0.0f;
+            float m[2] = {-INFINITY, -INFINITY}, l[2] = {0.0f, 0.0f};
+
+            for (int t = s.tile0; t < s.tile1; ++t) {
+                ok = mbar_wait(&full[stage], phase, abort_flag, p.status, DEV_TIMEOUT_SMEM_FULL);
+                ok = __all_sync(0xffffffffu, ok);
+                if (!ok) break;
+                const float4 mt = meta[stage * kFewWarps + warp];
+                const int tok0 = t * kFewTokens + warp * 16;
+                const uint8_t* kt = smem + stage * L::kStageBytes;
+                const uint8_t* vt = kt + L::kTileBytes;
+                if (mt.y != -INFINITY) {               // same for the whole warp
+                    // ---- scores: two n8 tiles of eight tokens
+                    float sc[2][4];
+#pragma unroll
+                    for (int n = 0; n < 2; ++n) {
+                        sc[n][0] = sc[n][1] = sc[n][2] = sc[n][3] = 0.0f;
+                        const int row = warp * 16 + n * 8 + g;
+                        if constexpr (kDim == 128) {
+#pragma unroll
+                            for (int i = 0; i < 2; ++i) {
+                                const uint4 w = *reinterpret_cast<const uint4*>(kt + row * 128 + (((2 * c + i) ^ (row & 7)) << 4));
+                                mma_f16(sc[n], qf[4 * i + 0], codes_lo(w.x), codes_hi(w.x));
+                                mma_f16(sc[n], qf[4 * i + 1], codes_lo(w.y), codes_hi(w.y));
+                                mma_f16(sc[n], qf[4 * i + 2], codes_lo(w.z), codes_hi(w.z));
+                                mma_f16(sc[n], qf[4 * i + 3], codes_lo(w.w), codes_hi(w.w));
+                            }
+                        } else {
+                            const uint4 w = *reinterpret_cast<const uint4*>(kt + row * 64 + ((c ^ ((row >> 1) & 3)) << 4));
+                            mma_f16(sc[n], qf[0], codes_lo(w.x), codes_hi(w.x));
+                            mma_f16(sc[n], qf[1], codes_lo(w.y), codes_hi(w.y));
+                            mma_f16(sc[n], qf[2], codes_lo(w.z), codes_hi(w.z));
+                            mma_f16(sc[n], qf[3], codes_lo(w.w), codes_hi(w.w));
+                        }
+                    }
+                    // ---- V codes of the tokens 2c, 2c + 1, 2c + 8, 2c + 9, dims [g * kDim / 8, (g + 1) * kDim / 8)
+                    uint32_t wv[4][kDim / 32];
+#pragma unroll
+                    for (int k = 0; k < 4; ++k) {
+                        const int row = warp * 16 + 2 * c + (k & 1) + (k >> 1) * 8;
+                        if constexpr (kDim == 128) {
+                            const uint4 w = *reinterpret_cast<const uint4*>(vt + row * 128 + ((g ^ (row & 7)) << 4));
+                            wv[k][0] = w.x; wv[k][1] = w.y; wv[k][2] = w.z; wv[k][3] = w.w;
+                        } else {
+                            const uint2 w = *reinterpret_cast<const uint2*>(vt + row * 64 + (((g >> 1) ^ ((row >> 1) & 3)) << 4) + (g & 1) * 8);
+                            wv[k][0] = w.x; wv[k][1] = w.y;
+                        }
+                    }
+                    // ---- softmax
+                    const float c0 = c_row[0] * mt.x, c1 = c_row[1] * mt.x;
+                    const bool masked = tok0 < all_lo || tok0 + 16 > all_hi;
+                    float tt[2][4];
+#pragma unroll
+                    for (int n = 0; n < 2; ++n) {
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) tt[n][e] = fmaf(sc[n][e], e < 2 ? c0 : c1, mt.y);
+                    }
+                    if (masked) {
+                        uint32_t pm[4];                // 1 where the row sees the token, in the layout of P
+#pragma unroll
+                        for (int n = 0; n < 2; ++n) {
+#pragma unroll
+                            for (int e = 0; e < 2; ++e) {
+                                const int tok = tok0 + n * 8 + 2 * c;
+                                const bool s0 = tok >= see_lo[e] && tok < see_hi[e];
+                                const bool s1 = tok + 1 >= see_lo[e] && tok + 1 < see_hi[e];
+                                if (!s0) tt[n][2 * e] = -INFINITY;
+                                if (!s1) tt[n][2 * e + 1] = -INFINITY;
+                                pm[2 * n + e] = (s0 ? 0x3C00u : 0u) | (s1 ? 0x3C000000u : 0u);
+                            }
+                        }
+                        // codes of tokens outside the item do not count; NaN codes of tokens that some rows see and
+                        // others do not are taken out of the product, and the rows that see them are given their NaN
+                        // by a product of ones: seen x is-NaN
+                        bool any = false;
+#pragma unroll
+                        for (int k = 0; k < 4; ++k) {
+                            const int tok = tok0 + 2 * c + (k & 1) + (k >> 1) * 8;
+#pragma unroll
+                            for (int i = 0; i < kDim / 32; ++i) {
+                                if (tok < s.lo || tok >= s.hi) wv[k][i] = 0;
+                                any |= nan_bytes(wv[k][i]) != 0;
+                            }
+                        }
+                        if (__any_sync(0xffffffffu, any)) {
+                            uint32_t wn[4][kDim / 32];
+#pragma unroll
+                            for (int k = 0; k < 4; ++k) {
+#pragma unroll
+                                for (int i = 0; i < kDim / 32; ++i) {
+                                    const uint32_t nb = nan_bytes(wv[k][i]);
+                                    wn[k][i] = nb & 0x38383838u;      // E4M3 one
+                                    wv[k][i] &= ~nb;
+                                }
+                            }
+#pragma unroll
+                            for (int j = 0; j < kTiles; j += 2) {
+                                const int i = j >> 2, sel = (j & 2) ? 0x7362 : 0x5140;
+                                const uint32_t x = __byte_perm(wn[0][i], wn[1][i], sel), y = __byte_perm(wn[2][i], wn[3][i], sel);
+                                float d0[4] = {0.f, 0.f, 0.f, 0.f}, d1[4] = {0.f, 0.f, 0.f, 0.f};
+                                mma_f16(d0, pm, codes_lo(x), codes_lo(y));
+                                mma_f16(d1, pm, codes_hi(x), codes_hi(y));
+#pragma unroll
+                                for (int e = 0; e < 4; ++e) {
+                                    if (d0[e] > 0.0f) o[j][e] = NAN;
+                                    if (d1[e] > 0.0f) o[j + 1][e] = NAN;
+                                }
+                            }
+                        }
+                    }
+                    float mx[2];
+#pragma unroll
+                    for (int e = 0; e < 2; ++e) {
+                        mx[e] = fmaxf(fmaxf(tt[0][2 * e], tt[0][2 * e + 1]), fmaxf(tt[1][2 * e], tt[1][2 * e + 1]));
+                        mx[e] = fmaxf(mx[e], __shfl_xor_sync(0xffffffffu, mx[e], 1));
+                        mx[e] = fmaxf(mx[e], __shfl_xor_sync(0xffffffffu, mx[e], 2));
+                        mx[e] = fmaxf(m[e], mx[e] - kProbShift);
+                    }
+                    if (__any_sync(0xffffffffu, mx[0] > m[0] || mx[1] > m[1])) {
+                        float al[2];
+#pragma unroll
+                        for (int e = 0; e < 2; ++e) {
+                            al[e] = m[e] == -INFINITY ? 0.0f : ex2(m[e] - mx[e]);
+                            if (m[e] == mx[e]) al[e] = 1.0f;
+                            m[e] = mx[e];
+                            l[e] *= al[e];
+                        }
+#pragma unroll
+                        for (int j = 0; j < kTiles; ++j) {
+                            o[j][0] *= al[0]; o[j][1] *= al[0];
+                            o[j][2] *= al[1]; o[j][3] *= al[1];
+                        }
+                    }
+                    const float ms0 = m[0] == -INFINITY ? 0.0f : m[0], ms1 = m[1] == -INFINITY ? 0.0f : m[1];
+                    uint32_t pf[4];
+                    float sum0 = 0.0f, sum1 = 0.0f;
+#pragma unroll
+                    for (int n = 0; n < 2; ++n) {
+                        const float p0 = ex2(tt[n][0] - ms0), p1 = ex2(tt[n][1] - ms0);
+                        const float p2 = ex2(tt[n][2] - ms1), p3 = ex2(tt[n][3] - ms1);
+                        sum0 += p0 + p1;
+                        sum1 += p2 + p3;
+                        pf[2 * n] = pack_f16(p0, p1);
+                        pf[2 * n + 1] = pack_f16(p2, p3);
+                    }
+                    l[0] = fmaf(sum0, mt.z, l[0]);
+                    l[1] = fmaf(sum1, mt.z, l[1]);
+                    // ---- P V: tile j holds dims 16g + j (64-wide heads: 8g + j) in column g
+#pragma unroll
+                    for (int j = 0; j < kTiles; j += 2) {
+                        const int i = j >> 2, sel = (j & 2) ? 0x7362 : 0x5140;
+                        const uint32_t x = __byte_perm(wv[0][i], wv[1][i], sel), y = __byte_perm(wv[2][i], wv[3][i], sel);
+                        mma_f16(o[j], pf, codes_lo(x), codes_lo(y));
+                        mma_f16(o[j + 1], pf, codes_hi(x), codes_hi(y));
+                    }
+                }
+                __syncwarp();
+                if (lane == 0) mbar_arrive(&empty[stage]);
+                if (++stage == kFewStages) { stage = 0; phase ^= 1; }
+            }
+            if (!ok) break;
+            // ---- join the four warps
+#pragma unroll
+            for (int e = 0; e < 2; ++e) {
+                l[e] += __shfl_xor_sync(0xffffffffu, l[e], 1);
+                l[e] += __shfl_xor_sync(0xffffffffu, l[e], 2);
+                const int row = g + 8 * e;
+                if (c == 0) {
+                    ml[(warp * kFewRows + row) * 2] = m[e];
+                    ml[(warp * kFewRows + row) * 2 + 1] = l[e];
+                }
+                // column n of tile j is dim n * kTiles + j: this lane has the kDim / 4 consecutive dims behind 2c * kTiles
+                float* dst = join + (warp * kFewRows + row) * L::kPitch + 2 * c * kTiles;
+#pragma unroll
+                for (int k = 0; k < kDim / 16; ++k) {
+                    const int j = 4 * (k % (kTiles / 4)), hi = k / (kTiles / 4);
+                    *reinterpret_cast<float4*>(dst + hi * kTiles + j) =
+                        make_float4(o[j][2 * e + hi], o[j + 1][2 * e + hi], o[j + 2][2 * e + hi], o[j + 3][2 * e + hi]);
+                }
+            }
+            compute_sync();
+            {
+                constexpr int kPer = kDim / 8;         // dims of this thread, eight threads a row
+                const int tid = threadIdx.x;           // the computing warps are the block's first
+                const int row = tid >> 3, d0 = (tid & 7) * kPer;
+                float mm = -INFINITY;
+#pragma unroll
+                for (int w = 0; w < kFewWarps; ++w) mm = fmaxf(mm, ml[(w * kFewRows + row) * 2]);
+                float acc[kPer];
+#pragma unroll
+                for (int k = 0; k < kPer; ++k) acc[k] = 0.0f;
+                float ll = 0.0f;
+#pragma unroll
+                for (int w = 0; w < kFewWarps; ++w) {
+                    const float mw = ml[(w * kFewRows + row) * 2];
+                    if (mw == -INFINITY) {
+                        // saw nothing: no part in the sum, but a NaN (a score that is one leaves the maximum alone)
+                        const float lw = ml[(w * kFewRows + row) * 2 + 1];
+                        if (lw != lw) ll = lw;
+                        continue;
+                    }
+                    const float wt = ex2(mw - mm);
+                    ll = fmaf(wt, ml[(w * kFewRows + row) * 2 + 1], ll);
+                    const float* src = join + (w * kFewRows + row) * L::kPitch + d0;
+#pragma unroll
+                    for (int k = 0; k < kPer; k += 4) {
+                        const float4 v = *reinterpret_cast<const float4*>(src + k);
+                        acc[k] = fmaf(wt, v.x, acc[k]);
+                        acc[k + 1] = fmaf(wt, v.y, acc[k + 1]);
+                        acc[k + 2] = fmaf(wt, v.z, acc[k + 2]);
+                        acc[k + 3] = fmaf(wt, v.w, acc[k + 3]);
+                    }
+                }
+                const int prow = s.row0 + row;
+                if (prow < s.rows) {
+                    const bool whole = s.item0 >= begin && s.item1 <= end;
+                    if (whole) {
+                        const int i = prow / p.group;
+                        const int head = s.head * p.group + (prow - i * p.group);
+                        const float inv = ll != 0.0f ? 1.0f / ll : 0.0f;
+                        uint16_t* dst = static_cast<uint16_t*>(p.out) + (long long)(s.req.q0 + i) * p.out_token_stride +
+                                        (long long)head * p.out_head_stride + d0;
+#pragma unroll
+                        for (int k = 0; k < kPer; k += 8) {
+                            uint4 w;
+                            w.x = pack_out<kBf16>(acc[k] * inv, acc[k + 1] * inv);
+                            w.y = pack_out<kBf16>(acc[k + 2] * inv, acc[k + 3] * inv);
+                            w.z = pack_out<kBf16>(acc[k + 4] * inv, acc[k + 5] * inv);
+                            w.w = pack_out<kBf16>(acc[k + 6] * inv, acc[k + 7] * inv);
+                            *reinterpret_cast<uint4*>(dst + k) = w;
+                        }
+                        if (p.lse && (tid & 7) == 0)
+                            p.lse[(long long)(s.req.q0 + i) * p.heads + head] =
+                                ll != 0.0f ? (mm + lg2(ll)) * 0.6931471805599453f : -INFINITY;
+                    } else {
+                        const long long slot = (long long)blockIdx.x * 2 + (u == begin ? 0 : 1);
+                        float* dst = p.part_out + (slot * kFewRows + row) * kDim + d0;
+#pragma unroll
+                        for (int k = 0; k < kPer; k += 4)
+                            *reinterpret_cast<float4*>(dst + k) = make_float4(acc[k], acc[k + 1], acc[k + 2], acc[k + 3]);
+                        if ((tid & 7) == 0)
+                            *reinterpret_cast<float2*>(p.part_ml + (slot * kFewRows + row) * 2) = make_float2(mm, ll);
+                    }
+                }
+            }
+            compute_sync();
+            u = u_next;
+        }
+        grid_launch_dependents();
+    }
+    // (a block whose wait ran out leaves with copies in flight: give them time to land before its memory is reused)
+    __syncthreads();
+    if (*abort_flag != 0) {
+        for (int i = 0; i < 64; ++i) __nanosleep(2000);
+    }
+}
+
+// Joins the pieces of the items that are cut by a chunk's border.  Block b takes the item that holds border (b + 1) *
+// chunk, unless an earlier border is in it too; warps take rows.
+template <int kRows, int kTokens, int kDim, bool kBf16>
+__global__ void __launch_bounds__(256) cache_attention_join_kernel(const CacheAttentionParams p, int blocks) {
+    extern __shared__ int join_prefix[];
+    __shared__ int warp_sums[8];
+    grid_launch_dependents();
+    grid_dependency_wait();
+    attn_prefix<kRows, kTokens>(p, join_prefix, warp_sums);
+    const int total = join_prefix[p.requests];
+    const int chunk = attn_chunk(p, total, blocks);
+    const long long border = (long long)(blockIdx.x + 1) * chunk;
+    if (border >= total) return;
+    const AttnPiece s = attn_piece<kRows, kTokens>(p, join_prefix, (int)border, total);
+    if (s.item0 == (int)border) return;                            // nothing is cut here
+    const int first = s.item0 / chunk, last = (s.item1 - 1) / chunk;
+    if (first != (int)blockIdx.x) return;                          // the item's first border belongs to another block
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    constexpr int kPer = kDim / 32;
+    const int rows = min(kRows, s.rows - s.row0);
+    for (int row = warp; row < rows; row += 8) {
+        float mm = -INFINITY, ll = 0.0f, acc[kPer];
+#pragma unroll
+        for (int k = 0; k < kPer; ++k) acc[k] = 0.0f;
+        for (int b = first; b <= last; ++b) {
+            // the piece that starts its block's chunk is in slot 0, one that starts inside it in slot 1
+            const long long slot = (long long)b * 2 + (b == first && s.item0 != b * chunk ? 1 : 0);
+            const float2 v = *reinterpret_cast<const float2*>(p.part_ml + (slot * kRows + row) * 2);
+            if (v.x == -INFINITY) {
+                if (v.y != v.y) ll = v.y;
+                continue;
+            }
+            const float m_new = fmaxf(mm, v.x);
+            const float keep = mm == -INFINITY ? (ll != ll ? 1.0f : 0.0f) : ex2(mm - m_new), add = ex2(v.x - m_new);
+            mm = m_new;
+            ll = ll * keep + v.y * add;
+            const float* src = p.part_out + (slot * kRows + row) * kDim + lane * kPer;
+#pragma unroll
+            for (int k = 0; k < kPer; ++k) acc[k] = acc[k] * keep + src[k] * add;
+        }
+        const int prow = s.row0 + row;
+        const int i = prow / p.group;
+        const int head = s.head * p.group + (prow - i * p.group);
+        const float inv = ll != 0.0f ? 1.0f / ll : 0.0f;
+        uint16_t* dst = static_cast<uint16_t*>(p.out) + (long long)(s.req.q0 + i) * p.out_token_stride +
+                        (long long)head * p.out_head_stride + lane * kPer;
+#pragma unroll
+        for (int k = 0; k < kPer; k += 2)
+            *reinterpret_cast<uint32_t*>(dst + k) = pack_out<kBf16>(acc[k] * inv, acc[k + 1] * inv);
+        if (p.lse && lane == 0)
+            p.lse[(long long)(s.req.q0 + i) * p.heads + head] =
+                ll != 0.0f ? (mm + lg2(ll)) * 0.6931471805599453f : -INFINITY;
+    }
+}
+
+// ---------------------------------------------------------------------------------------------------- launch
+
+// One page, or `box_rows` tokens of one, per box; the coordinates are (dim, token in block, head, block).
+static bool make_tmap_pages(CUtensorMap* map, const void* base, const blazeKvCache* c, int box_rows) {
+    EncodeTiledFn fn = encode_tiled_fn();
+    if (!fn) return false;
+    const cuuint64_t dims[4] = {(cuuint64_t)c->head_dim, (cuuint64_t)c->block_size, (cuuint64_t)c->kv_heads,
+                                (cuuint64_t)c->num_blocks};
+    // (the stride of a dimension of one is never used, but has to be a legal one)
+    const cuuint64_t token = (cuuint64_t)c->token_stride;
+    const cuuint64_t strides[3] = {token, c->kv_heads > 1 ? (cuuint64_t)c->head_stride : token,
+                                   c->num_blocks > 1 ? (cuuint64_t)c->block_stride : token};
+    const cuuint32_t box[4] = {(cuuint32_t)c->head_dim, (cuuint32_t)box_rows, 1, 1};
+    const cuuint32_t elem_strides[4] = {1, 1, 1, 1};
+    return fn(map, CU_TENSOR_MAP_DATA_TYPE_UINT8, 4, const_cast<void*>(base), dims, strides, box, elem_strides,
+              CU_TENSOR_MAP_INTERLEAVE_NONE, c->head_dim == 128 ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_64B,
+              CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
+static int status_of(cudaError_t e) {
+    if (e == cudaSuccess) return ACLTENSOR_STATUS_SUCCESS;
+    cudaGetLastError();
+    return ACLTENSOR_STATUS_EXECUTION_FAILED;
+}
+
+struct AttnPlan {
+    int few_grid;
+    size_t few_out, few_ml, total;
+};
+
+static size_t round256(size_t x) { return (x + 255) & ~size_t(255); }
+
+static int plan_attention(const blazeKvCache* c, const blazeCacheAttentionArgs* a, int sms, AttnPlan* pl) {
+    const int st = check_kv_cache(c);
+    if (st != ACLTENSOR_STATUS_SUCCESS) return st;
+    if (!a || a->struct_size < sizeof(blazeCacheAttentionArgs)) return ACLTENSOR_STATUS_INVALID_VALUE;
+    if (a->requests < 0 || a->tokens < 0 || a->heads < 1 || (a->heads % c->kv_heads) || a->max_q < 0 || a->min_q < 0 ||
+        a->max_kv < 0 || a->max_blocks < 0 || a->window < 0 || a->sm_limit < 0 || (a->causal != 0 && a->causal != 1) ||
+        a->table_stride < a->max_blocks || (int64_t)a->max_kv > (int64_t)a->max_blocks * c->block_size ||
+        !std::isfinite(a->scale))
+        return ACLTENSOR_STATUS_INVALID_VALUE;
+    if (a->requests > kAttnMaxRequests || (a->q_type != BLAZE_OUT_BF16 && a->q_type != BLAZE_OUT_F16))
+        return ACLTENSOR_STATUS_NOT_SUPPORTED;
+    // units are counted in 32 bits
+    const int64_t group = a->heads / c->kv_heads;
+    const int64_t tiles = ((int64_t)a->max_q * group + kFewRows - 1) / kFewRows;
+    const int64_t per_tile = (int64_t)a->max_kv / kFewTokens + 2;
+    if (a->max_kv > (1 << 30) || (int64_t)a->max_q * group > (1 << 24)) return ACLTENSOR_STATUS_NOT_SUPPORTED;
+    if ((double)a->requests * c->kv_heads * (double)tiles * (double)per_tile > 2.0e9) return ACLTENSOR_STATUS_NOT_SUPPORTED;
+    if (a->sm_limit > 0 && a->sm_limit < sms) sms = a->sm_limit;
+    pl->few_grid = 2 * sms;
+    pl->few_out = 0;
+    pl->few_ml = round256((size_t)pl->few_grid * 2 * kFewRows * c->head_dim * 4);
+    pl->total = pl->few_ml + round256((size_t)pl->few_grid * 2 * kFewRows * 2 * 4);
+    return ACLTENSOR_STATUS_SUCCESS;
+}
+
+template <int kDim, bool kBf16>
+static cudaError_t launch_few(const CUtensorMap& mk, const CUtensorMap& mv, const CacheAttentionParams& p, int grid,
+                              cudaStream_t stream) {
+    auto kernel = cache_attention_few_kernel<kDim, kBf16>;
+    auto join = cache_attention_join_kernel<kFewRows, kFewTokens, kDim, kBf16>;
+    static bool done[64] = {};
+    int dev = 0;
+    cudaGetDevice(&dev);
+    if (!done[dev & 63]) {
+        static_assert(FewSmem<kDim>::kPrefixOffset + 1024 + (kAttnMaxRequests + 1) * 4 <= 227 * 1024, "shared memory");
+        cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                             FewSmem<kDim>::bytes(kAttnMaxRequests));
+        if (e != cudaSuccess) return e;
+        done[dev & 63] = true;
+    }
+    cudaError_t e = launch_after_prepass(kernel, grid, kFewThreads, (size_t)FewSmem<kDim>::bytes(p.requests), stream, mk, mv, p);
+    if (e != cudaSuccess) return e;
+    return launch_after_prepass(join, grid - 1, 256, (size_t)(p.requests + 1) * 4, stream, p, grid);
+}
+
+}  // namespace blaze
+
+using namespace blaze;
+
+extern "C" int blazeCacheAttentionWorkspaceSize(const blazeKvCache* cache, const blazeCacheAttentionArgs* args, size_t* bytes) {
+    if (!bytes) return ACLTENSOR_STATUS_INVALID_VALUE;
+    DeviceContext* ctx = current_context();
+    AttnPlan pl;
+    const int st = plan_attention(cache, args, ctx ? ctx->sm_count : 148, &pl);
+    if (st != ACLTENSOR_STATUS_SUCCESS) return st;
+    *bytes = pl.total;
+    return ACLTENSOR_STATUS_SUCCESS;
+}
+
+extern "C" int blazeCacheAttention(const blazeKvCache* cache, const blazeCacheAttentionArgs* a, void* stream_v) {
+    DeviceContext* ctx = current_context();
+    AttnPlan pl;
+    const int st = plan_attention(cache, a, ctx ? ctx->sm_count : 148, &pl);
+    if (st != ACLTENSOR_STATUS_SUCCESS) return st;
+    if (a->requests == 0 || a->tokens == 0 || a->max_q == 0) return ACLTENSOR_STATUS_SUCCESS;
+    auto aligned = [](const void* x, uintptr_t n) { return (reinterpret_cast<uintptr_t>(x) & (n - 1)) == 0; };
+    if (!a->q || !a->out || !a->row_offsets || !a->kv_len || (a->max_blocks > 0 && !a->block_table))
+        return ACLTENSOR_STATUS_INVALID_VALUE;
+    if (!aligned(a->q, 16) || !aligned(a->out, 16) || !aligned(a->lse, 4) || !aligned(a->row_offsets, 4) ||
+        !aligned(a->kv_len, 4) || !aligned(a->block_table, 4) || (a->q_token_stride % 8) || (a->q_head_stride % 8) ||
+        (a->out_token_stride % 8) || (a->out_head_stride % 8))
+        return ACLTENSOR_STATUS_NOT_SUPPORTED;
+    if (!a->workspace || a->workspace_bytes < pl.total) return ACLTENSOR_STATUS_INSUFFICIENT_WORKSPACE;
+    if (!aligned(a->workspace, 256)) return ACLTENSOR_STATUS_INVALID_VALUE;
+    if (!ctx) return ACLTENSOR_STATUS_NOT_INITIALIZED;
+    if (ctx->cc_major != 10) return ACLTENSOR_STATUS_ARCH_MISMATCH;
+    cudaStream_t stream = static_cast<cudaStream_t>(stream_v);
+
+    CUtensorMap mk, mv;
+    const int box_rows = cache->block_size < kFewTokens ? cache->block_size : kFewTokens;
+    if (!make_tmap_pages(&mk, cache->k, cache, box_rows) || !make_tmap_pages(&mv, cache->v, cache, box_rows))
+        return ACLTENSOR_STATUS_INTERNAL_ERROR;
+
+    const CacheView cv = cache_view(cache);
+    CacheAttentionParams p;
+    p.requests = a->requests;
+    p.tokens = a->tokens;
+    p.heads = a->heads;
+    p.kv_heads = cache->kv_heads;
+    p.group = a->heads / cache->kv_heads;
+    p.head_dim = cache->head_dim;
+    p.block_shift = cv.block_shift;
+    p.num_blocks = cache->num_blocks;
+    p.max_blocks = a->max_blocks;
+    p.max_q = a->max_q;
+    p.max_kv = a->max_kv;
+    p.causal = a->causal;
+    p.window = a->window;
+    p.scale_log2 = a->scale * 1.4426950408889634f;
+    p.q = a->q;
+    p.q_token_stride = a->q_token_stride;
+    p.q_head_stride = a->q_head_stride;
+    p.out = a->out;
+    p.out_token_stride = a->out_token_stride;
+    p.out_head_stride = a->out_head_stride;
+    p.lse = static_cast<float*>(a->lse);
+    p.row_offsets = static_cast<const int*>(a->row_offsets);
+    p.kv_len = static_cast<const int*>(a->kv_len);
+    p.table = static_cast<const int*>(a->block_table);
+    p.table_stride = a->table_stride;
+    p.k_scale = cv.k_scale;
+    p.v_scale = cv.v_scale;
+    p.scale_stride = cv.scale_stride;
+    p.few_rows = 0x7FFFFFFF;
+    p.take_few = 1;
+    p.take_many = 0;
+    p.min_chunk = 2;
+    uint8_t* ws = static_cast<uint8_t*>(a->workspace);
+    p.part_out = reinterpret_cast<float*>(ws + pl.few_out);
+    p.part_ml = reinterpret_cast<float*>(ws + pl.few_ml);
+    p.status = ctx->status_word;
+    const bool bf16 = a->q_type == BLAZE_OUT_BF16;
+    cudaError_t e;
+    if (cache->head_dim == 128)
+        e = bf16 ? launch_few<128, true>(mk, mv, p, pl.few_grid, stream) : launch_few<128, false>(mk, mv, p, pl.few_grid, stream);
+    else
+        e = bf16 ? launch_few<64, true>(mk, mv, p, pl.few_grid, stream) : launch_few<64, false>(mk, mv, p, pl.few_grid, stream);
+    return status_of(e);
+}

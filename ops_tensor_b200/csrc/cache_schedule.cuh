@@ -1,0 +1,197 @@
+// How the attention over the paged cache is cut into work: shared by its kernels and by the kernel that joins their
+// partial results.
+//
+// A request's query rows, heads of a kv head's group packed beside one another (row = token * group + head in group),
+// are cut into row tiles; an item is one row tile of one kv head, and its work is the tiles of `kTokens` cached tokens
+// that any of its rows sees (one unit for an item that sees nothing: its zeros have to be written).  The units of all
+// items, request by request, head by head, row tile by row tile, are numbered through and dealt to the blocks in equal
+// contiguous chunks, so lengths need not be known on the host and a long request costs no more than the same tokens in
+// short ones.  An item inside one chunk is finished there; the pieces of any other leave float32 partial results
+// (unnormalised output, running maximum and sum), which the joining kernel adds in the order of the chunks: the result
+// is the same from run to run.
+#pragma once
+
+#include <cstdint>
+
+#include "cache.h"
+#include "ptx.cuh"
+
+namespace blaze {
+
+constexpr int kAttnMaxRequests = 8192;
+
+struct CacheAttentionParams {
+    int requests, tokens, heads, kv_heads, group, head_dim;
+    int block_shift, num_blocks, max_blocks;
+    int max_q, max_kv;
+    int causal, window;
+    float scale_log2;                 // scale * log2(e)
+    const void* q;
+    long long q_token_stride, q_head_stride;
+    void* out;
+    long long out_token_stride, out_head_stride;
+    float* lse;
+    const int* row_offsets;
+    const int* kv_len;
+    const int* table;
+    long long table_stride;
+    const float* k_scale;
+    const float* v_scale;
+    long long scale_stride;
+    int few_rows;                     // requests of at most so many packed rows go to the few-rows kernel, others not
+    int take_few, take_many;          // which of the two this launch takes
+    int min_chunk;                    // units per block, at least
+    float* part_out;                  // [block][2][row tile][head_dim]
+    float* part_ml;                   // [block][2][row tile][2]
+    int* status;
+};
+
+struct AttnRequest {
+    int q0, qlen, kv;
+};
+
+__device__ __forceinline__ AttnRequest attn_request(const CacheAttentionParams& p, int r) {
+    AttnRequest q;
+    const int a = min(max(p.row_offsets[r], 0), p.tokens);
+    const int b = min(max(p.row_offsets[r + 1], a), p.tokens);
+    q.q0 = a;
+    q.qlen = min(b - a, p.max_q);
+    q.kv = min(max(p.kv_len[r], 0), p.max_kv);
+    const bool few = (long long)q.qlen * p.group <= p.few_rows;
+    if (few ? !p.take_few : !p.take_many) q.qlen = 0;
+    return q;
+}
+
+// Tokens [lo, hi) that the rows of row tile `qt` see between them.
+template <int kRows>
+__device__ __forceinline__ void attn_span(const CacheAttentionParams& p, const AttnRequest& q, int qt, int& lo, int& hi) {
+    const int rows = q.qlen * p.group;
+    const int i0 = (qt * kRows) / p.group;
+    const int i1 = (min(rows, (qt + 1) * kRows) - 1) / p.group;
+    const int off = q.kv - q.qlen;
+    hi = p.causal ? min(q.kv, off + i1 + 1) : q.kv;
+    lo = p.window > 0 ? max(0, off + i0 - p.window + 1) : 0;
+    if (hi <= lo) { lo = 0; hi = 0; }
+}
+
+template <int kTokens>
+__device__ __forceinline__ int attn_units(int lo, int hi) {
+    return hi <= lo ? 1 : (hi + kTokens - 1) / kTokens - lo / kTokens;
+}
+
+// Units of one kv head of request q.
+template <int kRows, int kTokens>
+__device__ __forceinline__ int attn_units_of_head(const CacheAttentionParams& p, const AttnRequest& q) {
+    const int tiles = (q.qlen * p.group + kRows - 1) / kRows;
+    int n = 0;
+    for (int t = 0; t < tiles; ++t) {
+        int lo, hi;
+        attn_span<kRows>(p, q, t, lo, hi);
+        n += attn_units<kTokens>(lo, hi);
+    }
+    return n;
+}
+
+// prefix[r] = units before request r, prefix[requests] = all of them.  Called by the whole block.
+template <int kRows, int kTokens>
+__device__ __forceinline__ void attn_prefix(const CacheAttentionParams& p, int* prefix, int* warp_sums) {
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, warps = blockDim.x >> 5;
+    int carry = 0;
+    for (int base = 0; base < p.requests; base += blockDim.x) {
+        const int r = base + threadIdx.x;
+        int u = 0;
+        if (r < p.requests) {
+            const AttnRequest q = attn_request(p, r);
+            if (q.qlen > 0) u = p.kv_heads * attn_units_of_head<kRows, kTokens>(p, q);
+        }
+        int inc = u;
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+            const int y = __shfl_up_sync(0xffffffffu, inc, o);
+            if (lane >= o) inc += y;
+        }
+        if (lane == 31) warp_sums[warp] = inc;
+        __syncthreads();
+        int before = carry, total = carry;
+        for (int w = 0; w < warps; ++w) {
+            const int s = warp_sums[w];
+            if (w < warp) before += s;
+            total += s;
+        }
+        if (r < p.requests) prefix[r] = before + inc - u;
+        carry = total;
+        __syncthreads();
+    }
+    if (threadIdx.x == 0) prefix[p.requests] = carry;
+    __syncthreads();
+}
+
+// Units of a block's chunk: equal for all blocks but the last that has any.
+__device__ __forceinline__ int attn_chunk(const CacheAttentionParams& p, int total, int blocks) {
+    return max((total + blocks - 1) / blocks, p.min_chunk);
+}
+
+// The piece of an item that starts at unit u and ends at the item's end or at unit `end`.
+struct AttnPiece {
+    AttnRequest req;
+    int r, head, row0, rows;          // first packed row of the tile, packed rows of the request
+    int lo, hi;                       // tokens that the whole item's rows see between them
+    int tile0, tile1;                 // tiles of this piece
+    int item0, item1;                 // units of the item
+};
+
+template <int kRows, int kTokens>
+__device__ __forceinline__ AttnPiece attn_piece(const CacheAttentionParams& p, const int* prefix, int u, int end) {
+    AttnPiece s;
+    int a = 0, b = p.requests;
+    while (b - a > 1) {
+        const int mid = (a + b) >> 1;
+        if (prefix[mid] <= u) a = mid; else b = mid;
+    }
+    s.r = a;
+    s.req = attn_request(p, a);
+    s.rows = s.req.qlen * p.group;
+    const int per_head = (prefix[a + 1] - prefix[a]) / p.kv_heads;
+    const int local = u - prefix[a];
+    s.head = local / per_head;
+    int rem = local - s.head * per_head;
+    int qt = 0, n;
+    for (;;) {
+        attn_span<kRows>(p, s.req, qt, s.lo, s.hi);
+        n = attn_units<kTokens>(s.lo, s.hi);
+        if (rem < n) break;
+        rem -= n;
+        ++qt;
+    }
+    s.row0 = qt * kRows;
+    s.item0 = u - rem;
+    s.item1 = s.item0 + n;
+    const int take = min(s.item1, end) - u;
+    s.tile0 = s.lo / kTokens + rem;
+    s.tile1 = s.hi <= s.lo ? s.tile0 : s.tile0 + take;
+    return s;
+}
+
+__device__ __forceinline__ float ex2(float x) {
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+__device__ __forceinline__ float lg2(float x) {
+    float y;
+    asm("lg2.approx.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+
+// Probabilities are kept up to 2^15 (the running maximum less 15), so that in half the values down to 2^-29 of a row's
+// largest have all their bits and nothing above 2^-40 of it vanishes, however long the row.
+constexpr float kProbShift = 15.0f;
+// A V scale enters the exponent; below 2^-64 (which the store never writes) it counts as that.
+constexpr float kMinLogScale = -64.0f;
+
+template <bool kBf16>
+__device__ __forceinline__ uint32_t pack_out(float lo, float hi) {
+    return kBf16 ? pack_bf16(lo, hi) : pack_f16(lo, hi);
+}
+
+}  // namespace blaze

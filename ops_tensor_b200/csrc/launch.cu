@@ -57,11 +57,7 @@ DeviceContext* current_context() {
 
 // ------------------------------------------------------------------------------------------------ tensor maps
 
-using EncodeTiledFn = CUresult (*)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*,
-                                   const cuuint64_t*, const cuuint32_t*, const cuuint32_t*, CUtensorMapInterleave,
-                                   CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
-
-static EncodeTiledFn encode_tiled_fn() {
+EncodeTiledFn encode_tiled_fn() {
     static EncodeTiledFn fn = []() -> EncodeTiledFn {
         void* sym = nullptr;
         cudaDriverEntryPointQueryResult q;
@@ -299,25 +295,6 @@ static int plan_mx(const blazeMxGemmArgs* a, int sms, MxPlan* pl, bool wide_scal
         pl->total += 1024;
     }
     return ACLTENSOR_STATUS_SUCCESS;
-}
-
-// Launch of a GEMM kernel that follows its scale re-tile pre-pass in the stream: programmatic stream serialisation
-// lets the GEMM's blocks set themselves up while the pre-pass is still running; the kernel's producer thread waits for
-// the pre-pass (griddepcontrol.wait) before its first load.
-template <class... KArgs, class... Args>
-static cudaError_t launch_after_prepass(void (*kernel)(KArgs...), int grid, int block, size_t smem, cudaStream_t stream,
-                                        const Args&... args) {
-    cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3((unsigned)grid, 1, 1);
-    cfg.blockDim = dim3((unsigned)block, 1, 1);
-    cfg.dynamicSmemBytes = smem;
-    cfg.stream = stream;
-    cudaLaunchAttribute attr[1];
-    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-    attr[0].val.programmaticStreamSerializationAllowed = 1;
-    cfg.attrs = attr;
-    cfg.numAttrs = 1;
-    return cudaLaunchKernelEx(&cfg, kernel, args...);
 }
 
 template <int kBN, int kAct>

@@ -1,6 +1,7 @@
 // Internal C++ declarations shared by the kernel translation units and the C-ABI layer.
 #pragma once
 
+#include <cuda.h>
 #include <cuda_runtime.h>
 #include <cstddef>
 #include <cstdint>
@@ -16,6 +17,32 @@ struct DeviceContext {
 
 // Per-device context of the current device (created on first use; thread-safe).  nullptr if no usable device.
 DeviceContext* current_context();
+
+// cuTensorMapEncodeTiled, looked up through the runtime (the library does not link the driver); nullptr if missing.
+using EncodeTiledFn = CUresult (*)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*,
+                                   const cuuint64_t*, const cuuint32_t*, const cuuint32_t*, CUtensorMapInterleave,
+                                   CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
+EncodeTiledFn encode_tiled_fn();
+
+// Launch of a kernel behind another one in its stream with programmatic stream serialisation: its blocks may set
+// themselves up while the kernel before is still running, and wait for it (griddepcontrol.wait) before they touch
+// memory.  Every block of such a kernel executes that wait before it ends, so that the kernel behind this one, which
+// waits for this one alone, comes after the kernel before it as well.
+template <class... KArgs, class... Args>
+inline cudaError_t launch_after_prepass(void (*kernel)(KArgs...), int grid, int block, size_t smem, cudaStream_t stream,
+                                        const Args&... args) {
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3((unsigned)grid, 1, 1);
+    cfg.blockDim = dim3((unsigned)block, 1, 1);
+    cfg.dynamicSmemBytes = smem;
+    cfg.stream = stream;
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = 1;
+    return cudaLaunchKernelEx(&cfg, kernel, args...);
+}
 
 // Bytes of the re-tiled scale-factor array for `rows` x K with tiles of `tile_rows` rows, every 512-byte block
 // stored `replicas` times in a row.

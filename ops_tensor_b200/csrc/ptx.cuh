@@ -25,6 +25,7 @@ enum DeviceStatus : int {
     DEV_TIMEOUT_FIXUP_FLAG = 5,   // stream-K owner waited for a partial tile that was never published
     DEV_TIMEOUT_PEER = 6,         // 2-CTA pair: waited for the partner CTA
     DEV_TIMEOUT_SELFTEST = 7,     // the diagnostic kernel's wait on a barrier nobody signals (expected to expire)
+    DEV_BAD_CACHE_BLOCK = 8,      // a block table names a block that the cache does not have (no wait: bad input)
 };
 
 #ifndef BLAZE_WAIT_LIMIT_CYCLES

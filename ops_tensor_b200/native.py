@@ -110,6 +110,60 @@ DENSE_SCALE_NONE, DENSE_SCALE_PER_TENSOR, DENSE_SCALE_PER_CHANNEL = 0, 1, 2
 OUT_S32 = 5
 
 
+class KvCacheDesc(C.Structure):
+    """blazeKvCache: the paged 8-bit key / value cache."""
+    _fields_ = [
+        ("struct_size", C.c_size_t),
+        ("elem", C.c_int32),
+        ("num_blocks", C.c_int32), ("block_size", C.c_int32), ("kv_heads", C.c_int32), ("head_dim", C.c_int32),
+        ("reserved", C.c_int32),
+        ("k", C.c_void_p), ("v", C.c_void_p),
+        ("block_stride", C.c_int64), ("head_stride", C.c_int64), ("token_stride", C.c_int64),
+        ("k_scale", C.c_void_p), ("v_scale", C.c_void_p),
+        ("scale_stride", C.c_int64),
+    ]
+
+
+class CacheAssignArgs(C.Structure):
+    _fields_ = [
+        ("struct_size", C.c_size_t),
+        ("requests", C.c_int32), ("block_size", C.c_int32), ("max_blocks", C.c_int32), ("max_tokens", C.c_int32),
+        ("cached_len", C.c_void_p), ("new_len", C.c_void_p),
+        ("block_table", C.c_void_p), ("table_stride", C.c_int64),
+        ("free_blocks", C.c_void_p), ("free_capacity", C.c_int32), ("reserved", C.c_int32),
+        ("free_count", C.c_void_p), ("free_count_out", C.c_void_p),
+        ("row_offsets", C.c_void_p), ("kv_len", C.c_void_p),
+        ("slots", C.c_void_p), ("positions", C.c_void_p), ("denied", C.c_void_p),
+    ]
+
+
+class CacheStoreArgs(C.Structure):
+    _fields_ = [
+        ("struct_size", C.c_size_t),
+        ("tokens", C.c_int32), ("in_type", C.c_int32),
+        ("k", C.c_void_p), ("v", C.c_void_p),
+        ("k_token_stride", C.c_int64), ("k_head_stride", C.c_int64),
+        ("v_token_stride", C.c_int64), ("v_head_stride", C.c_int64),
+        ("slots", C.c_void_p),
+    ]
+
+
+class CacheAttentionArgs(C.Structure):
+    _fields_ = [
+        ("struct_size", C.c_size_t),
+        ("requests", C.c_int32), ("tokens", C.c_int32), ("heads", C.c_int32), ("q_type", C.c_int32),
+        ("q", C.c_void_p), ("q_token_stride", C.c_int64), ("q_head_stride", C.c_int64),
+        ("out", C.c_void_p), ("out_token_stride", C.c_int64), ("out_head_stride", C.c_int64),
+        ("lse", C.c_void_p),
+        ("row_offsets", C.c_void_p), ("kv_len", C.c_void_p),
+        ("block_table", C.c_void_p), ("table_stride", C.c_int64),
+        ("max_blocks", C.c_int32),
+        ("max_q", C.c_int32), ("min_q", C.c_int32), ("max_kv", C.c_int32),
+        ("scale", C.c_float), ("causal", C.c_int32), ("window", C.c_int32), ("sm_limit", C.c_int32),
+        ("workspace", C.c_void_p), ("workspace_bytes", C.c_size_t),
+    ]
+
+
 class BlazeError(RuntimeError):
     def __init__(self, status: int, where: str):
         self.status = status
@@ -151,6 +205,11 @@ def _declare(l: C.CDLL) -> None:
                                             C.c_void_p, C.c_void_p]
     l.blazeQuantizeFp8Blocks.argtypes = [C.c_void_p, C.c_int64, C.c_int32, C.c_int32, C.c_void_p, C.c_int64,
                                          C.c_void_p, C.c_void_p]
+    l.blazeCacheAssign.argtypes = [C.POINTER(CacheAssignArgs), C.c_void_p]
+    l.blazeCacheStore.argtypes = [C.POINTER(KvCacheDesc), C.POINTER(CacheStoreArgs), C.c_void_p]
+    l.blazeCacheAttentionWorkspaceSize.argtypes = [C.POINTER(KvCacheDesc), C.POINTER(CacheAttentionArgs),
+                                                   C.POINTER(C.c_size_t)]
+    l.blazeCacheAttention.argtypes = [C.POINTER(KvCacheDesc), C.POINTER(CacheAttentionArgs), C.c_void_p]
     l.blazeAddF32.argtypes = [C.c_void_p, C.c_void_p, C.c_void_p, C.c_int64, C.c_void_p]
     l.blazeSelfTestWaitTimeout.argtypes = [C.c_int64, C.c_void_p]
     l.blazeSelfTestWaitTimeout.restype = C.c_int
@@ -158,7 +217,8 @@ def _declare(l: C.CDLL) -> None:
     l.blazeDeviceInfo.argtypes = [C.POINTER(C.c_int32), C.POINTER(C.c_int32), C.POINTER(C.c_int32)]
     for name in ("blazeMxGemmWorkspaceSize", "blazeMxGemm", "blazeFp8GemmWorkspaceSize", "blazeFp8Gemm",
                  "blazeQuantizeMx", "blazeQuantizeFp8RowGroups", "blazeQuantizeFp8Blocks", "blazeAddF32",
-                 "blazeDeviceStatus", "blazeDeviceInfo"):
+                 "blazeDeviceStatus", "blazeDeviceInfo", "blazeCacheAssign", "blazeCacheStore",
+                 "blazeCacheAttentionWorkspaceSize", "blazeCacheAttention"):
         getattr(l, name).restype = C.c_int
 
 
@@ -422,6 +482,223 @@ def peer_signal(local_flags, peer_flags, my_rank: int, peer_ranks, value: int, l
     l = lib()
     l.blazePeerSignal.restype = C.c_int
     check(l.blazePeerSignal(C.byref(args), _stream()), "blazePeerSignal")
+
+
+# ------------------------------------------------------------------------------------------------ paged 8-bit cache
+
+def _on(t):
+    """The device of a CUDA tensor made current, and its current stream: what a call on `t` is launched with."""
+    import torch
+    return torch.cuda.device(t.device), lambda: C.c_void_p(torch.cuda.current_stream(t.device).cuda_stream)
+
+
+def _same_device(first, **others):
+    if not first.is_cuda:
+        raise ValueError("the cache operators take CUDA tensors")
+    for name, t in others.items():
+        if t is not None and t.device != first.device:
+            raise ValueError(f"{name} is on {t.device}, not on {first.device}")
+
+
+def _vector(t, name, dtype, at_least):
+    if t.dtype != dtype or t.dim() != 1 or t.numel() < at_least or (t.numel() > 1 and t.stride(0) != 1):
+        raise ValueError(f"{name}: a contiguous {dtype} vector of at least {at_least} elements is wanted")
+
+
+def _table(t):
+    """(rows, columns, pitch) of a block table."""
+    import torch
+    if t.dtype != torch.int32 or t.dim() != 2 or (t.numel() and t.shape[1] > 1 and t.stride(1) != 1):
+        raise ValueError("block_table: an int32 [requests, blocks] tensor with contiguous rows is wanted")
+    pitch = t.stride(0) if t.numel() and t.shape[0] > 1 else t.shape[1]
+    return t.shape[0], t.shape[1], pitch
+
+
+class PagedCache:
+    """A paged key / value cache in E4M3 with one float32 scale per (block, kv head): `k`, `v` [blocks, kv heads, block
+    size, head size] of uint8 or float8_e4m3fn with equal strides (any order of the first three dimensions in memory;
+    `k.permute(0, 2, 1, 3)` of a [blocks, tokens, heads, size] tensor is one), `k_scale`, `v_scale` float32
+    [blocks, kv heads].  Keeps the tensors; `desc` is the C ABI's view of them."""
+
+    def __init__(self, k, v, k_scale, v_scale):
+        import torch
+        _same_device(k, v=v, k_scale=k_scale, v_scale=v_scale)
+        if k.dim() != 4 or k.shape != v.shape or k.dtype != v.dtype or k.dtype not in (torch.uint8, torch.float8_e4m3fn):
+            raise ValueError("k and v: two [blocks, heads, block size, head size] tensors of uint8 or float8_e4m3fn")
+        n, h, bs, d = k.shape
+        strides = [s for s, size in zip(k.stride(), k.shape) if size > 1]
+        if strides != [s for s, size in zip(v.stride(), v.shape) if size > 1] or k.stride(3) != 1 or v.stride(3) != 1:
+            raise ValueError("k and v must have the same strides, the last dimension contiguous")
+        for name, t in (("k_scale", k_scale), ("v_scale", v_scale)):
+            if t.dtype != torch.float32 or tuple(t.shape) != (n, h) or (h > 1 and t.stride(1) != 1):
+                raise ValueError(f"{name}: a float32 [blocks, heads] tensor with contiguous rows is wanted")
+        if n > 1 and k_scale.stride(0) != v_scale.stride(0):
+            raise ValueError("k_scale and v_scale must have the same row stride")
+        self.k, self.v, self.k_scale, self.v_scale = k, v, k_scale, v_scale
+        self.device = k.device
+        self.num_blocks, self.kv_heads, self.block_size, self.head_dim = n, h, bs, d
+        c = self.desc = KvCacheDesc()
+        c.struct_size = C.sizeof(KvCacheDesc)
+        c.elem = ELEM_E4M3
+        c.num_blocks, c.kv_heads, c.block_size, c.head_dim = n, h, bs, d
+        c.k, c.v = k.data_ptr(), v.data_ptr()
+        c.block_stride, c.head_stride, c.token_stride = k.stride()[:3]
+        c.k_scale, c.v_scale = k_scale.data_ptr(), v_scale.data_ptr()
+        c.scale_stride = k_scale.stride(0) if n > 1 else h
+
+    @classmethod
+    def empty(cls, num_blocks, kv_heads, block_size, head_dim, device="cuda"):
+        """A new cache: codes of zero, scales of one."""
+        import torch
+        shape = (num_blocks, kv_heads, block_size, head_dim)
+        k, v = (torch.zeros(shape, dtype=torch.uint8, device=device) for _ in range(2))
+        ks, vs = (torch.ones((num_blocks, kv_heads), dtype=torch.float32, device=device) for _ in range(2))
+        return cls(k, v, ks, vs)
+
+
+def cache_assign(cached_len, new_len, block_table, free_blocks, free_count, *, block_size, row_offsets, kv_len, slots,
+                 positions=None, free_count_out=None, denied=None):
+    """The bookkeeping of a serving step on the GPU (blazeCacheAssign): blocks for the requests that grow, the blocks of
+    the ended ones (`new_len` < 0) back on the stack, and the packed batch's `row_offsets`, `slots` and `positions`.
+    `kv_len` may be `cached_len`; `free_count_out` defaults to `free_count` (in place)."""
+    import torch
+    if free_count_out is None:
+        free_count_out = free_count
+    _same_device(cached_len, new_len=new_len, block_table=block_table, free_blocks=free_blocks, free_count=free_count,
+                 row_offsets=row_offsets, kv_len=kv_len, slots=slots, positions=positions,
+                 free_count_out=free_count_out, denied=denied)
+    n = cached_len.numel()
+    for name, t, size in (("cached_len", cached_len, n), ("new_len", new_len, n), ("kv_len", kv_len, n),
+                          ("row_offsets", row_offsets, n + 1), ("free_blocks", free_blocks, 0),
+                          ("free_count", free_count, 1), ("free_count_out", free_count_out, 1)):
+        _vector(t, name, torch.int32, size)
+    _vector(slots, "slots", torch.int64, 0)
+    if positions is not None:
+        _vector(positions, "positions", torch.int32, slots.numel())
+    if denied is not None:
+        _vector(denied, "denied", torch.int32, 1)
+    rows, columns, pitch = _table(block_table)
+    if rows < n:
+        raise ValueError("block_table has fewer rows than there are requests")
+    a = CacheAssignArgs()
+    a.struct_size = C.sizeof(CacheAssignArgs)
+    a.requests, a.block_size, a.max_blocks, a.max_tokens = n, block_size, columns, slots.numel()
+    a.cached_len, a.new_len = cached_len.data_ptr(), new_len.data_ptr()
+    a.block_table, a.table_stride = block_table.data_ptr(), pitch
+    a.free_blocks, a.free_capacity = free_blocks.data_ptr(), free_blocks.numel()
+    a.free_count, a.free_count_out = free_count.data_ptr(), free_count_out.data_ptr()
+    a.row_offsets, a.kv_len, a.slots = row_offsets.data_ptr(), kv_len.data_ptr(), slots.data_ptr()
+    a.positions = positions.data_ptr() if positions is not None else None
+    a.denied = denied.data_ptr() if denied is not None else None
+    on, stream = _on(cached_len)
+    with on:
+        check(lib().blazeCacheAssign(C.byref(a), stream()), "blazeCacheAssign")
+
+
+def _rows_type(t, name):
+    import torch
+    if t.dtype not in (torch.bfloat16, torch.float16) or t.dim() != 3 or (t.shape[2] > 1 and t.stride(2) != 1):
+        raise ValueError(f"{name}: a bf16 or half [tokens, heads, head size] tensor with contiguous rows is wanted")
+    return out_type_of(t)
+
+
+def cache_store(cache: PagedCache, k, v, slots):
+    """Quantises the rows of `k` and `v` [tokens, kv heads, head size] into the cache's slots (blazeCacheStore)."""
+    import torch
+    _same_device(cache.k, k=k, v=v, slots=slots)
+    _vector(slots, "slots", torch.int64, 0)
+    n = slots.numel()
+    for name, t in (("k", k), ("v", v)):
+        _rows_type(t, name)
+        if t.dtype != k.dtype or t.shape[0] < n or tuple(t.shape[1:]) != (cache.kv_heads, cache.head_dim):
+            raise ValueError(f"{name}: [at least {n}, {cache.kv_heads}, {cache.head_dim}] is wanted, of one type")
+    a = CacheStoreArgs()
+    a.struct_size = C.sizeof(CacheStoreArgs)
+    a.tokens, a.in_type = n, out_type_of(k)
+    a.k, a.v = k.data_ptr(), v.data_ptr()
+    a.k_token_stride, a.k_head_stride = _row_strides(k)
+    a.v_token_stride, a.v_head_stride = _row_strides(v)
+    a.slots = slots.data_ptr()
+    on, stream = _on(cache.k)
+    with on:
+        check(lib().blazeCacheStore(C.byref(cache.desc), C.byref(a), stream()), "blazeCacheStore")
+
+
+def _row_strides(t):
+    """Token and head strides; a dimension of one has none that counts."""
+    return t.stride(0) if t.shape[0] > 1 else 0, t.stride(1) if t.shape[1] > 1 else 0
+
+
+def _attention_args(cache, q, *, requests, max_q, max_kv, max_blocks, min_q=0, scale=1.0, causal=True, window=0,
+                    sm_limit=0) -> CacheAttentionArgs:
+    a = CacheAttentionArgs()
+    a.struct_size = C.sizeof(CacheAttentionArgs)
+    a.requests, a.tokens, a.heads, a.q_type = requests, q.shape[0], q.shape[1], _rows_type(q, "q")
+    a.max_blocks = a.table_stride = max_blocks
+    a.max_q, a.min_q, a.max_kv = max_q, min_q, max_kv
+    a.scale, a.causal, a.window, a.sm_limit = scale, 1 if causal else 0, window, sm_limit
+    return a
+
+
+def cache_attention_workspace_bytes(cache: PagedCache, q, *, requests, max_q, max_kv, sm_limit=0) -> int:
+    a = _attention_args(cache, q, requests=requests, max_q=max_q, max_kv=max_kv,
+                        max_blocks=-(-max_kv // cache.block_size), sm_limit=sm_limit)
+    n = C.c_size_t(0)
+    check(lib().blazeCacheAttentionWorkspaceSize(C.byref(cache.desc), C.byref(a), C.byref(n)),
+          "blazeCacheAttentionWorkspaceSize")
+    return n.value
+
+
+def cache_attention_workspace(cache: PagedCache, q, *, requests, max_q, max_kv, sm_limit=0):
+    """A workspace for cache_attention calls of these bounds; needs no initialisation, keeps nothing between calls."""
+    import torch
+    need = cache_attention_workspace_bytes(cache, q, requests=requests, max_q=max_q, max_kv=max_kv, sm_limit=sm_limit)
+    return torch.empty(max(need, 256), dtype=torch.uint8, device=cache.device)
+
+
+def cache_attention(cache: PagedCache, q, row_offsets, kv_len, block_table, *, scale=None, max_q, max_kv, min_q=0,
+                    causal=True, window=0, out=None, lse=None, workspace=None, sm_limit=0):
+    """Attention of the packed queries `q` [tokens, heads, head size] over the cache (blazeCacheAttention); `scale`
+    defaults to head size ** -0.5.  `max_q`, `max_kv` bound the requests' rows and lengths, `min_q` is a hint.
+    Allocates `out` (zeros: rows outside every request are not written) and `workspace` when not given; fills `lse`
+    [tokens, heads] float32 when given."""
+    import torch
+    _same_device(cache.k, q=q, row_offsets=row_offsets, kv_len=kv_len, block_table=block_table, out=out, lse=lse,
+                 workspace=workspace)
+    n = kv_len.numel()
+    _vector(kv_len, "kv_len", torch.int32, 0)
+    _vector(row_offsets, "row_offsets", torch.int32, n + 1)
+    rows, columns, pitch = _table(block_table)
+    if rows < n:
+        raise ValueError("block_table has fewer rows than there are requests")
+    _rows_type(q, "q")
+    if q.shape[2] != cache.head_dim:
+        raise ValueError(f"q has heads of {q.shape[2]}, the cache of {cache.head_dim}")
+    if out is None:
+        out = torch.zeros(q.shape, dtype=q.dtype, device=q.device)
+    _rows_type(out, "out")
+    if out.shape != q.shape or out.dtype != q.dtype:
+        raise ValueError("out must have q's shape and type")
+    if lse is not None and (lse.dtype != torch.float32 or lse.shape != q.shape[:2] or not lse.is_contiguous()):
+        raise ValueError("lse: a contiguous float32 [tokens, heads] tensor is wanted")
+    a = _attention_args(cache, q, requests=n, max_q=max_q, max_kv=max_kv, max_blocks=columns, min_q=min_q,
+                        scale=cache.head_dim ** -0.5 if scale is None else scale, causal=causal, window=window,
+                        sm_limit=sm_limit)
+    a.q, (a.q_token_stride, a.q_head_stride) = q.data_ptr(), _row_strides(q)
+    a.out, (a.out_token_stride, a.out_head_stride) = out.data_ptr(), _row_strides(out)
+    a.lse = lse.data_ptr() if lse is not None else None
+    a.row_offsets, a.kv_len = row_offsets.data_ptr(), kv_len.data_ptr()
+    a.block_table, a.table_stride = block_table.data_ptr(), pitch
+    on, stream = _on(cache.k)
+    with on:
+        if workspace is None:
+            need = C.c_size_t(0)
+            check(lib().blazeCacheAttentionWorkspaceSize(C.byref(cache.desc), C.byref(a), C.byref(need)),
+                  "blazeCacheAttentionWorkspaceSize")
+            workspace = torch.empty(max(need.value, 256), dtype=torch.uint8, device=cache.device)
+        a.workspace, a.workspace_bytes = workspace.data_ptr(), workspace.numel() * workspace.element_size()
+        check(lib().blazeCacheAttention(C.byref(cache.desc), C.byref(a), stream()), "blazeCacheAttention")
+    return out
 
 
 def add_f32(a, c, out=None):

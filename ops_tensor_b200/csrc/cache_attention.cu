@@ -20,6 +20,7 @@
 #include <cmath>
 
 #include "cache.h"
+#include "cache_attention_many.cuh"
 #include "cache_schedule.cuh"
 #include "cann_ops_tensor_types.h"
 #include "launch.h"
@@ -32,6 +33,10 @@ constexpr int kFewTokens = 64;        // tokens of a tile
 constexpr int kFewWarps = 4;          // computing warps, 16 tokens of a tile each
 constexpr int kFewThreads = 32 * (kFewWarps + 1);
 constexpr int kFewStages = 4;
+constexpr int kFewMinChunk = 2;       // tiles of a block's chunk, at least
+constexpr int kManyMinChunk = 2;
+// Requests of more packed rows go to the many-rows kernel.
+constexpr int kFewLimit = kFewRows;
 
 template <int kDim>
 struct FewSmem {
@@ -75,14 +80,6 @@ __device__ __forceinline__ void tma_load_page(uint32_t dst, const CUtensorMap* m
 
 // A named barrier of the computing warps.
 __device__ __forceinline__ void compute_sync() { asm volatile("bar.sync 1, %0;" ::"n"(32 * kFewWarps) : "memory"); }
-
-// Power of two that brings the largest magnitude of a row of bf16 queries to [2^14, 2^15), so that the row fits half
-// with all its bits; 1 for half queries, which are taken as they are.
-__device__ __forceinline__ int query_shift(float amax) {
-    const int e = (int)(__float_as_uint(amax) >> 23) - 127;
-    return amax > 0.0f ? min(max(14 - e, -120), 120) : 0;
-}
-__device__ __forceinline__ float pow2i(int e) { return __uint_as_float((uint32_t)(e + 127) << 23); }
 
 template <int kDim, bool kBf16>
 __global__ void __launch_bounds__(kFewThreads, 2)
@@ -524,9 +521,10 @@ cache_attention_few_kernel(const __grid_constant__ CUtensorMap map_k, const __gr
 }
 
 // Joins the pieces of the items that are cut by a chunk's border.  Block b takes the item that holds border (b + 1) *
-// chunk, unless an earlier border is in it too; warps take rows.
+// chunk, unless an earlier border is in it too; a row tile is shared by kGroups blocks, whose warps take rows.
 template <int kRows, int kTokens, int kDim, bool kBf16>
 __global__ void __launch_bounds__(256) cache_attention_join_kernel(const CacheAttentionParams p, int blocks) {
+    constexpr int kGroups = kRows / 16;
     extern __shared__ int join_prefix[];
     __shared__ int warp_sums[8];
     grid_launch_dependents();
@@ -534,16 +532,17 @@ __global__ void __launch_bounds__(256) cache_attention_join_kernel(const CacheAt
     attn_prefix<kRows, kTokens>(p, join_prefix, warp_sums);
     const int total = join_prefix[p.requests];
     const int chunk = attn_chunk(p, total, blocks);
-    const long long border = (long long)(blockIdx.x + 1) * chunk;
+    const int which = blockIdx.x / kGroups, group = blockIdx.x % kGroups;
+    const long long border = (long long)(which + 1) * chunk;
     if (border >= total) return;
     const AttnPiece s = attn_piece<kRows, kTokens>(p, join_prefix, (int)border, total);
     if (s.item0 == (int)border) return;                            // nothing is cut here
     const int first = s.item0 / chunk, last = (s.item1 - 1) / chunk;
-    if (first != (int)blockIdx.x) return;                          // the item's first border belongs to another block
+    if (first != which) return;                                     // the item's first border belongs to another block
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     constexpr int kPer = kDim / 32;
-    const int rows = min(kRows, s.rows - s.row0);
-    for (int row = warp; row < rows; row += 8) {
+    const int rows = min((group + 1) * 16, s.rows - s.row0);
+    for (int row = group * 16 + warp; row < rows; row += 8) {
         float mm = -INFINITY, ll = 0.0f, acc[kPer];
 #pragma unroll
         for (int k = 0; k < kPer; ++k) acc[k] = 0.0f;
@@ -603,9 +602,11 @@ static int status_of(cudaError_t e) {
     return ACLTENSOR_STATUS_EXECUTION_FAILED;
 }
 
+// Which kernels a call needs, by the bounds of its requests' rows, and where their partial results lie.
 struct AttnPlan {
-    int few_grid;
-    size_t few_out, few_ml, total;
+    bool few, many;
+    int few_grid, many_grid;
+    size_t few_ml, many_out, many_ml, total;           // offsets in the workspace (few_out is 0)
 };
 
 static size_t round256(size_t x) { return (x + 255) & ~size_t(255); }
@@ -621,38 +622,78 @@ static int plan_attention(const blazeKvCache* c, const blazeCacheAttentionArgs* 
         return ACLTENSOR_STATUS_INVALID_VALUE;
     if (a->requests > kAttnMaxRequests || (a->q_type != BLAZE_OUT_BF16 && a->q_type != BLAZE_OUT_F16))
         return ACLTENSOR_STATUS_NOT_SUPPORTED;
+    const int64_t group = a->heads / c->kv_heads, rows = (int64_t)a->max_q * group;
+    if (a->max_kv > (1 << 30) || rows > (1 << 24)) return ACLTENSOR_STATUS_NOT_SUPPORTED;
+    pl->many = rows > kFewLimit;
+    pl->few = !pl->many || (int64_t)a->min_q * group <= kFewLimit;
     // units are counted in 32 bits
-    const int64_t group = a->heads / c->kv_heads;
-    const int64_t tiles = ((int64_t)a->max_q * group + kFewRows - 1) / kFewRows;
-    const int64_t per_tile = (int64_t)a->max_kv / kFewTokens + 2;
-    if (a->max_kv > (1 << 30) || (int64_t)a->max_q * group > (1 << 24)) return ACLTENSOR_STATUS_NOT_SUPPORTED;
-    if ((double)a->requests * c->kv_heads * (double)tiles * (double)per_tile > 2.0e9) return ACLTENSOR_STATUS_NOT_SUPPORTED;
+    const double heads = (double)a->requests * c->kv_heads;
+    if (heads * (double)(a->max_kv / kFewTokens + 2) > 2.0e9 ||
+        (pl->many && heads * (double)((rows + kManyRows - 1) / kManyRows) * (double)(a->max_kv / kManyTokens + 2) > 2.0e9))
+        return ACLTENSOR_STATUS_NOT_SUPPORTED;
     if (a->sm_limit > 0 && a->sm_limit < sms) sms = a->sm_limit;
     pl->few_grid = 2 * sms;
-    pl->few_out = 0;
-    pl->few_ml = round256((size_t)pl->few_grid * 2 * kFewRows * c->head_dim * 4);
-    pl->total = pl->few_ml + round256((size_t)pl->few_grid * 2 * kFewRows * 2 * 4);
+    pl->many_grid = sms;
+    size_t at = 0;
+    auto room = [&](int grid, int tile_rows, size_t* ml) {
+        at += round256((size_t)grid * 2 * tile_rows * c->head_dim * 4);
+        *ml = at;
+        at += round256((size_t)grid * 2 * tile_rows * 2 * 4);
+    };
+    pl->few_ml = pl->many_out = pl->many_ml = 0;
+    if (pl->few) room(pl->few_grid, kFewRows, &pl->few_ml);
+    pl->many_out = at;
+    if (pl->many) room(pl->many_grid, kManyRows, &pl->many_ml);
+    pl->total = at;
     return ACLTENSOR_STATUS_SUCCESS;
 }
 
 template <int kDim, bool kBf16>
-static cudaError_t launch_few(const CUtensorMap& mk, const CUtensorMap& mv, const CacheAttentionParams& p, int grid,
-                              cudaStream_t stream) {
-    auto kernel = cache_attention_few_kernel<kDim, kBf16>;
-    auto join = cache_attention_join_kernel<kFewRows, kFewTokens, kDim, kBf16>;
+static cudaError_t launch_attention(const CUtensorMap& mk, const CUtensorMap& mv, CacheAttentionParams p, const CacheView& cv,
+                                    const AttnPlan& pl, uint8_t* ws, cudaStream_t stream) {
+    auto few = cache_attention_few_kernel<kDim, kBf16>;
+    auto many = cache_attention_many_kernel<kDim, kBf16>;
     static bool done[64] = {};
     int dev = 0;
     cudaGetDevice(&dev);
     if (!done[dev & 63]) {
-        static_assert(FewSmem<kDim>::kPrefixOffset + 1024 + (kAttnMaxRequests + 1) * 4 <= 227 * 1024, "shared memory");
-        cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
+        static_assert(1024 + FewSmem<kDim>::kPrefixOffset + (kAttnMaxRequests + 1) * 4 <= 227 * 1024 &&
+                      1024 + ManySmem<kDim>::kPrefixOffset + (kAttnMaxRequests + 1) * 4 <= 227 * 1024, "shared memory");
+        cudaError_t e = cudaFuncSetAttribute(few, cudaFuncAttributeMaxDynamicSharedMemorySize,
                                              FewSmem<kDim>::bytes(kAttnMaxRequests));
+        if (e == cudaSuccess)
+            e = cudaFuncSetAttribute(many, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                     ManySmem<kDim>::bytes(kAttnMaxRequests));
         if (e != cudaSuccess) return e;
         done[dev & 63] = true;
     }
-    cudaError_t e = launch_after_prepass(kernel, grid, kFewThreads, (size_t)FewSmem<kDim>::bytes(p.requests), stream, mk, mv, p);
-    if (e != cudaSuccess) return e;
-    return launch_after_prepass(join, grid - 1, 256, (size_t)(p.requests + 1) * 4, stream, p, grid);
+    const size_t join_smem = (size_t)(p.requests + 1) * 4;
+    cudaError_t e = cudaSuccess;
+    p.few_rows = kFewLimit;
+    if (pl.few) {
+        p.take_few = 1;
+        p.take_many = 0;
+        p.min_chunk = kFewMinChunk;
+        p.part_out = reinterpret_cast<float*>(ws);
+        p.part_ml = reinterpret_cast<float*>(ws + pl.few_ml);
+        e = launch_after_prepass(few, pl.few_grid, kFewThreads, (size_t)FewSmem<kDim>::bytes(p.requests), stream, mk, mv, p);
+        if (e == cudaSuccess && pl.few_grid > 1)
+            e = launch_after_prepass(cache_attention_join_kernel<kFewRows, kFewTokens, kDim, kBf16>, pl.few_grid - 1, 256,
+                                     join_smem, stream, p, pl.few_grid);
+        if (e != cudaSuccess) return e;
+    }
+    if (pl.many) {
+        p.take_few = pl.few ? 0 : 1;                   // (without the few-rows launch every request is this one's)
+        p.take_many = 1;
+        p.min_chunk = kManyMinChunk;
+        p.part_out = reinterpret_cast<float*>(ws + pl.many_out);
+        p.part_ml = reinterpret_cast<float*>(ws + pl.many_ml);
+        e = launch_after_prepass(many, pl.many_grid, kManyThreads, (size_t)ManySmem<kDim>::bytes(p.requests), stream, p, cv);
+        if (e == cudaSuccess && pl.many_grid > 1)
+            e = launch_after_prepass(cache_attention_join_kernel<kManyRows, kManyTokens, kDim, kBf16>,
+                                     (pl.many_grid - 1) * (kManyRows / 16), 256, join_smem, stream, p, pl.many_grid);
+    }
+    return e;
 }
 
 }  // namespace blaze
@@ -723,19 +764,10 @@ extern "C" int blazeCacheAttention(const blazeKvCache* cache, const blazeCacheAt
     p.k_scale = cv.k_scale;
     p.v_scale = cv.v_scale;
     p.scale_stride = cv.scale_stride;
-    p.few_rows = 0x7FFFFFFF;
-    p.take_few = 1;
-    p.take_many = 0;
-    p.min_chunk = 2;
-    uint8_t* ws = static_cast<uint8_t*>(a->workspace);
-    p.part_out = reinterpret_cast<float*>(ws + pl.few_out);
-    p.part_ml = reinterpret_cast<float*>(ws + pl.few_ml);
     p.status = ctx->status_word;
+    uint8_t* ws = static_cast<uint8_t*>(a->workspace);
     const bool bf16 = a->q_type == BLAZE_OUT_BF16;
-    cudaError_t e;
-    if (cache->head_dim == 128)
-        e = bf16 ? launch_few<128, true>(mk, mv, p, pl.few_grid, stream) : launch_few<128, false>(mk, mv, p, pl.few_grid, stream);
-    else
-        e = bf16 ? launch_few<64, true>(mk, mv, p, pl.few_grid, stream) : launch_few<64, false>(mk, mv, p, pl.few_grid, stream);
-    return status_of(e);
+    auto launch = cache->head_dim == 128 ? (bf16 ? launch_attention<128, true> : launch_attention<128, false>)
+                                         : (bf16 ? launch_attention<64, true> : launch_attention<64, false>);
+    return status_of(launch(mk, mv, p, cv, pl, ws, stream));
 }

@@ -1,0 +1,655 @@
+// The many-rows kernel of the attention over the paged cache (prompts and chunks of prompts): both products on the
+// tensor cores with tcgen05 (kind::f16, float32 accumulation).  The formulas are at the top of cache_attention.cu.
+//
+// A row tile is 256 packed query rows, two sub-tiles A and B of 128, one accumulator row per thread of a warpgroup each;
+// a tile of the cache is 128 tokens.  Roles:
+//   warps 0-3, 4-7   softmax of sub-tile A / B: scores from TMEM, probabilities back into the same TMEM columns as half
+//                    (the A operand of P V), O re-scaled in TMEM when a row's maximum has grown by more than 2^8
+//                    since it was last taken, the piece's epilogue
+//   warps 8-11       codes -> half: 16-byte loads of the pages straight from global memory, one tile ahead in registers,
+//                    converted (exactly) and stored into the 128-byte-swizzled operand tiles; block numbers and scales of the
+//                    tiles; the queries of a row tile
+//   warp 12          issues the MMAs: P_A V(t), Q_A K(t+1), P_B V(t), Q_B K(t+1), so each warpgroup's softmax runs while the
+//                    tensor cores work for the other one
+// Q K^T takes K as the K-major operand; P V takes V as it lies, dims contiguous (MN-major), no transposition anywhere.
+#pragma once
+
+#include "cache_schedule.cuh"
+
+namespace blaze {
+
+constexpr int kManyRows = 256;
+constexpr int kManyTokens = 128;
+constexpr int kManyThreads = 32 * 13;
+constexpr int kManyMeta = 4;              // tiles whose scales are held
+
+// Largest of the exponents by which p may pass its reference: p <= 2^15.
+constexpr float kManyShift = 7.0f;
+constexpr float kManyGrow = 15.0f;
+
+template <int kDim>
+struct ManySmem {
+    static constexpr int kHalves = kDim / 64;                        // 64-wide (128-byte) column halves
+    static constexpr int kOperandBytes = 128 * kDim * 2;             // 128 rows of Q, K or V as half
+    static constexpr int kQOffset = 0;                               // A, B
+    static constexpr int kKOffset = 2 * kOperandBytes;               // two stages
+    static constexpr int kVOffset = kKOffset + 2 * kOperandBytes;    // two stages
+    static constexpr int kMetaOffset = kVOffset + 2 * kOperandBytes; // float4 [kManyMeta][8]
+    static constexpr int kRowOffset = kMetaOffset + kManyMeta * 8 * 16;    // float [256]: score factor of each row
+    static constexpr int kBarOffset = kRowOffset + kManyRows * 4;
+    static constexpr int kNumBars = 2 + 4 + 4 + kManyMeta + 6;
+    static constexpr int kMiscOffset = kBarOffset + kNumBars * 8;
+    static constexpr int kPrefixOffset = kMiscOffset + 128;
+    static int bytes(int requests) { return 1024 + kPrefixOffset + (requests + 1) * 4; }
+};
+
+// Operand of kDim or 128 columns stored [k row][64 columns] per half with the 128-byte swizzle, the contiguous
+// direction being the instruction's N: halves `half_bytes` apart, groups of 8 k rows 1024 bytes apart.
+__device__ __forceinline__ uint64_t umma_desc_sw128_mn(uint32_t smem_addr, uint32_t half_bytes) {
+    uint64_t d = 0;
+    d |= static_cast<uint64_t>((smem_addr & 0x3FFFFu) >> 4);
+    d |= static_cast<uint64_t>(half_bytes >> 4) << 16;               // leading byte offset: next 64 columns
+    d |= static_cast<uint64_t>(1024 >> 4) << 32;                     // stride byte offset: next 8 k rows
+    d |= static_cast<uint64_t>(1) << 46;
+    d |= static_cast<uint64_t>(2) << 61;
+    return d;
+}
+
+__host__ __device__ constexpr uint32_t umma_idesc_half(uint32_t n, bool b_mn) {          // M = 128, half x half -> float32
+    return (1u << 4) | (b_mn ? 1u << 16 : 0u) | ((n >> 3) << 17) | ((128u >> 4) << 24);
+}
+
+__device__ __forceinline__ void umma_f16_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t acc) {
+    asm volatile(
+        "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
+        "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}\n" ::"r"(d),
+        "l"(a), "l"(b), "r"(idesc), "r"(acc)
+        : "memory");
+}
+__device__ __forceinline__ void umma_f16_ts(uint32_t d, uint32_t a_tmem, uint64_t b, uint32_t idesc, uint32_t acc) {
+    asm volatile(
+        "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
+        "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}\n" ::"r"(d),
+        "r"(a_tmem), "l"(b), "r"(idesc), "r"(acc)
+        : "memory");
+}
+__device__ __forceinline__ void tmem_st_32x16(uint32_t taddr, const uint32_t (&r)[16]) {
+    asm volatile(
+        "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16};" ::"r"(taddr),
+        "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]),
+        "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15])
+        : "memory");
+}
+__device__ __forceinline__ void tmem_st_32x32(uint32_t taddr, const uint32_t (&r)[32]) {
+    asm volatile(
+        "tcgen05.st.sync.aligned.32x32b.x32.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16, "
+        "%17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31, %32};" ::"r"(taddr),
+        "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]),
+        "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15]), "r"(r[16]), "r"(r[17]), "r"(r[18]),
+        "r"(r[19]), "r"(r[20]), "r"(r[21]), "r"(r[22]), "r"(r[23]), "r"(r[24]), "r"(r[25]), "r"(r[26]), "r"(r[27]),
+        "r"(r[28]), "r"(r[29]), "r"(r[30]), "r"(r[31])
+        : "memory");
+}
+__device__ __forceinline__ void tmem_st_wait() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
+
+// Tokens [lo, hi) that any row of the sub-tile of 128 rows at `row0` sees, and [all_lo, all_hi) that every row sees.
+struct SubTile {
+    int lo, hi, all_lo, all_hi;
+    __device__ __forceinline__ bool active(int t) const {
+        return t * kManyTokens < hi && (t + 1) * kManyTokens > lo;
+    }
+    __device__ __forceinline__ bool masked(int t) const {
+        return t * kManyTokens < all_lo || (t + 1) * kManyTokens > all_hi;
+    }
+};
+__device__ __forceinline__ SubTile sub_tile(const CacheAttentionParams& p, const AttnPiece& s, int row0, int row1) {
+    SubTile x;
+    const int end = min(s.rows, row1);
+    if (row0 >= end) {
+        x.lo = x.hi = x.all_lo = x.all_hi = 0;
+        return x;
+    }
+    const int i0 = row0 / p.group, i1 = (end - 1) / p.group, off = s.req.kv - s.req.qlen;
+    x.hi = p.causal ? min(s.req.kv, off + i1 + 1) : s.req.kv;
+    x.lo = p.window > 0 ? max(0, off + i0 - p.window + 1) : 0;
+    x.all_hi = p.causal ? min(s.req.kv, off + i0 + 1) : s.req.kv;
+    x.all_lo = p.window > 0 ? max(0, off + i1 - p.window + 1) : 0;
+    if (x.hi <= x.lo) x.lo = x.hi = 0;
+    return x;
+}
+
+// 16 E4M3 codes -> 16 halves.
+__device__ __forceinline__ void codes_to_half(const uint4& w, uint4& a, uint4& b) {
+    auto lo = [](uint32_t x) {
+        const __half2_raw r = __nv_cvt_fp8x2_to_halfraw2((__nv_fp8x2_storage_t)(x & 0xFFFFu), __NV_E4M3);
+        return *reinterpret_cast<const uint32_t*>(&r);
+    };
+    auto hi = [](uint32_t x) {
+        const __half2_raw r = __nv_cvt_fp8x2_to_halfraw2((__nv_fp8x2_storage_t)(x >> 16), __NV_E4M3);
+        return *reinterpret_cast<const uint32_t*>(&r);
+    };
+    a = make_uint4(lo(w.x), hi(w.x), lo(w.y), hi(w.y));
+    b = make_uint4(lo(w.z), hi(w.z), lo(w.w), hi(w.w));
+}
+
+template <int kDim, bool kBf16>
+__global__ void __launch_bounds__(kManyThreads, 1)
+cache_attention_many_kernel(const CacheAttentionParams p, const CacheView cache) {
+    using L = ManySmem<kDim>;
+    extern __shared__ uint8_t many_smem_raw[];
+    uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(many_smem_raw) + 1023) & ~uintptr_t(1023));
+    float4* meta = reinterpret_cast<float4*>(smem + L::kMetaOffset);
+    float* row_factor = reinterpret_cast<float*>(smem + L::kRowOffset);
+    uint64_t* bars = reinterpret_cast<uint64_t*>(smem + L::kBarOffset);
+    uint64_t* q_full = bars;                  // the converting warps
+    uint64_t* q_free = bars + 1;              // the last Q K^T of the piece, and the eight softmax warps that took the factors
+    uint64_t* k_full = bars + 2;              // [2]
+    uint64_t* k_free = bars + 4;              // [2]
+    uint64_t* v_full = bars + 6;              // [2]
+    uint64_t* v_free = bars + 8;              // [2]
+    uint64_t* meta_full = bars + 10;          // [kManyMeta]
+    uint64_t* s_full = bars + 10 + kManyMeta;     // [2] sub-tiles
+    uint64_t* p_full = s_full + 2;            // [2]
+    uint64_t* pv_done = s_full + 4;           // [2]
+    int* misc = reinterpret_cast<int*>(smem + L::kMiscOffset);           // [0, 16): sums; 16: TMEM; 17: abort; 18, 19: last piece (+ 1) with NaN codes taken out
+    uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(misc + 16);
+    volatile int* abort_flag = misc + 17;
+    volatile int* nan_piece = misc + 18;       // by the parity of the piece
+    int* prefix = reinterpret_cast<int*>(smem + L::kPrefixOffset);
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+
+    if (threadIdx.x == 0) {
+        mbar_init(q_full, 4);
+        mbar_init(q_free, 9);
+        for (int i = 0; i < 2; ++i) {
+            mbar_init(&k_full[i], 4);
+            mbar_init(&k_free[i], 1);
+            mbar_init(&v_full[i], 4);
+            mbar_init(&v_free[i], 1);
+            mbar_init(&s_full[i], 1);
+            mbar_init(&p_full[i], 4);
+            mbar_init(&pv_done[i], 1);
+        }
+        for (int i = 0; i < kManyMeta; ++i) mbar_init(&meta_full[i], 1);
+        *abort_flag = 0;
+        nan_piece[0] = nan_piece[1] = 0;
+        fence_mbar_init();
+    }
+    if (warp == 12) tmem_alloc<1>(tmem_slot, 512);
+    grid_dependency_wait();
+    tcgen05_fence_before();
+    attn_prefix<kManyRows, kManyTokens>(p, prefix, misc);
+    tcgen05_fence_after();
+    const uint32_t tmem = *tmem_slot;
+    const uint32_t tmem_s[2] = {tmem, tmem + 128};
+    const uint32_t tmem_o[2] = {tmem + 256, tmem + 256 + kDim};
+    const int total = prefix[p.requests];
+    const int chunk = attn_chunk(p, total, gridDim.x);
+    const long long begin64 = (long long)blockIdx.x * chunk;
+    const int begin = (int)min(begin64, (long long)total);
+    const int end = (int)min(begin64 + chunk, (long long)total);
+    bool ok = true;
+
+    if (warp < 8) {
+        // ------------------------------------------------------------------ softmax
+        const int x = warp >> 2;                              // sub-tile
+        const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16;
+        const uint32_t ts = tmem_s[x] + lanes, to = tmem_o[x] + lanes;
+        const int row_in_tile = x * 128 + (warp & 3) * 32 + lane;
+        int n_piece = 0, n_tile = 0, n_mine = 0;              // pieces, tiles of the block, tiles of this sub-tile so far
+        for (int u = begin; u < end && ok; ++n_piece) {
+            const AttnPiece s = attn_piece<kManyRows, kManyTokens>(p, prefix, u, end);
+            const int u_next = u + max(1, s.tile1 - s.tile0);
+            const SubTile sub = sub_tile(p, s, s.row0 + x * 128, s.row0 + x * 128 + 128);
+            const int row = s.row0 + row_in_tile;
+            const bool there = row < s.rows;
+            const int i = there ? row / p.group : 0;
+            const int head = s.head * p.group + (there ? row - i * p.group : 0);
+            const int pos = s.req.kv - s.req.qlen + i;
+            const int see_hi = there ? (p.causal ? min(s.req.kv, pos + 1) : s.req.kv) : 0;
+            const int see_lo = p.window > 0 ? max(0, pos - p.window + 1) : 0;
+            ok = mbar_wait(q_full, n_piece & 1, abort_flag, p.status, DEV_TIMEOUT_SMEM_FULL);
+            ok = __all_sync(0xffffffffu, ok);
+            if (!ok) break;
+            const float factor = row_factor[row_in_tile];
+            __syncwarp();
+            if (lane == 0) mbar_arrive(q_free);
+
+            float m = -INFINITY, l = 0.0f;
+            int done = 0;                                     // tiles of this piece whose P V has been asked for
+            for (int t = s.tile0; t < s.tile1; ++t, ++n_tile) {
+                if (!sub.active(t)) continue;
+                ok = mbar_wait(&meta_full[n_tile % kManyMeta], (n_tile / kManyMeta) & 1, abort_flag, p.status, DEV_TIMEOUT_SMEM_FULL) &&
+                     mbar_wait(&s_full[x], n_mine & 1, abort_flag, p.status, DEV_TIMEOUT_TMEM_FULL);
+                ok = __all_sync(0xffffffffu, ok);
+                if (!ok) break;
+                tcgen05_fence_after();
+                const float4* mt = meta + (n_tile % kManyMeta) * 8;
+                const bool masked = sub.masked(t);
+                const int tok0 = t * kManyTokens;
+                // bits of the tokens [tok0 + 16 g, + 16) that this row sees
+                auto seen = [&](int g) -> uint32_t {
+                    const int a = max(see_lo - (tok0 + 16 * g), 0), b = min(see_hi - (tok0 + 16 * g), 16);
+                    return b > a ? ((1u << b) - 1u) & ~((1u << a) - 1u) : 0u;
+                };
+                // ---- largest score of the row
+                float mx = -INFINITY;
+#pragma unroll
+                for (int c = 0; c < 4; ++c) {
+                    uint32_t v[32];
+                    __syncwarp();
+                    tmem_ld_32x32(ts + c * 32, v);
+                    tmem_ld_wait();
+#pragma unroll
+                    for (int h = 0; h < 2; ++h) {
+                        const float4 q = mt[2 * c + h];
+                        if (q.y == -INFINITY) continue;
+                        float g = -INFINITY;
+                        if (masked) {
+                            const uint32_t bits = seen(2 * c + h);
+                            if (bits == 0) continue;
+#pragma unroll
+                            for (int k = 0; k < 16; ++k)
+                                if (bits >> k & 1) g = fmaxf(g, __uint_as_float(v[16 * h + k]));
+                        } else {
+#pragma unroll
+                            for (int k = 0; k < 16; ++k) g = fmaxf(g, __uint_as_float(v[16 * h + k]));
+                        }
+                        mx = fmaxf(mx, fmaf(g, factor * q.x, q.y));
+                    }
+                }
+                // ---- a new reference, where the row has outgrown the old one
+                const bool grow = mx > m + kManyGrow;
+                if (__any_sync(0xffffffffu, grow)) {
+                    const float m_new = grow ? mx - kManyShift : m;
+                    const float al = grow ? (m == -INFINITY ? 0.0f : ex2(m - m_new)) : 1.0f;
+                    m = m_new;
+                    l *= al;
+                    if (done > 0) {
+                        ok = mbar_wait(&pv_done[x], (n_mine - 1) & 1, abort_flag, p.status, DEV_TIMEOUT_TMEM_FULL);
+                        ok = __all_sync(0xffffffffu, ok);
+                        if (!ok) break;
+                        tcgen05_fence_after();
+#pragma unroll
+                        for (int c = 0; c < kDim / 32; ++c) {
+                            uint32_t v[32];
+                            tmem_ld_32x32(to + c * 32, v);
+                            tmem_ld_wait();
+#pragma unroll
+                            for (int k = 0; k < 32; ++k) v[k] = __float_as_uint(__uint_as_float(v[k]) * al);
+                            tmem_st_32x32(to + c * 32, v);
+                        }
+                    }
+                }
+                const float ms = m == -INFINITY ? 0.0f : m;
+                // ---- probabilities
+#pragma unroll
+                for (int c = 0; c < 4; ++c) {
+                    uint32_t v[32], w[16];
+                    __syncwarp();
+                    tmem_ld_32x32(ts + c * 32, v);
+                    tmem_ld_wait();
+#pragma unroll
+                    for (int h = 0; h < 2; ++h) {
+                        const float4 q = mt[2 * c + h];
+                        const float k1 = factor * q.x, k0 = q.y - ms;
+                        float sum = 0.0f;
+                        if (q.y == -INFINITY) {
+#pragma unroll
+                            for (int k = 0; k < 8; ++k) w[8 * h + k] = 0;
+                        } else {
+                            const uint32_t bits = masked ? seen(2 * c + h) : 0xFFFFu;
+#pragma unroll
+                            for (int k = 0; k < 16; k += 2) {
+                                float a = ex2(fmaf(__uint_as_float(v[16 * h + k]), k1, k0));
+                                float b = ex2(fmaf(__uint_as_float(v[16 * h + k + 1]), k1, k0));
+                                if (masked) {
+                                    if (!(bits >> k & 1)) a = 0.0f;
+                                    if (!(bits >> k & 2)) b = 0.0f;
+                                }
+                                sum += a + b;
+                                w[8 * h + (k >> 1)] = pack_f16(a, b);
+                            }
+                            l = fmaf(sum, q.z, l);
+                        }
+                    }
+                    __syncwarp();
+                    tmem_st_32x16(ts + c * 16, w);
+                }
+                tmem_st_wait();
+                tcgen05_fence_before();
+                __syncwarp();
+                if (lane == 0) mbar_arrive(&p_full[x]);
+                ++done;
+                ++n_mine;
+            }
+            if (!ok) break;
+            // ---- epilogue
+            if (done > 0) {
+                ok = mbar_wait(&pv_done[x], (n_mine - 1) & 1, abort_flag, p.status, DEV_TIMEOUT_TMEM_FULL);
+                ok = __all_sync(0xffffffffu, ok);
+                if (!ok) break;
+                tcgen05_fence_after();
+            }
+            const bool whole = s.item0 >= begin && s.item1 <= end;
+            const bool nans = nan_piece[n_piece & 1] == n_piece + 1;
+            const float inv = l != 0.0f ? 1.0f / l : 0.0f;
+            const long long slot = (long long)blockIdx.x * 2 + (u == begin ? 0 : 1);
+            uint16_t* out = static_cast<uint16_t*>(p.out) + (long long)(s.req.q0 + i) * p.out_token_stride +
+                            (long long)head * p.out_head_stride;
+            float* part = p.part_out + (slot * kManyRows + row_in_tile) * kDim;
+#pragma unroll 1
+            for (int c = 0; c < kDim / 32; ++c) {
+                uint32_t v[32];
+                __syncwarp();
+                if (done > 0) {
+                    tmem_ld_32x32(to + c * 32, v);
+                    tmem_ld_wait();
+                } else {
+#pragma unroll
+                    for (int k = 0; k < 32; ++k) v[k] = 0;
+                }
+                if (nans && there) {
+                    // NaN codes of V in tiles that not every row sees were taken out of the product: the rows that do see
+                    // them get their NaN here, from the codes themselves
+                    const SubTile all = sub_tile(p, s, s.row0, s.row0 + kManyRows);
+                    for (int t = s.tile0; t < s.tile1; ++t) {
+                        if (!all.masked(t)) continue;
+                        const int a = max(see_lo, t * kManyTokens), b = min(see_hi, (t + 1) * kManyTokens);
+                        for (int tok = a; tok < b; ++tok) {
+                            const int block = p.table[(long long)s.r * p.table_stride + (tok >> p.block_shift)];
+                            if (block < 0 || block >= p.num_blocks) continue;
+                            const uint8_t* code = cache.v + block * cache.block_stride + s.head * cache.head_stride +
+                                                  (long long)(tok & (cache.block_size - 1)) * cache.token_stride + c * 32;
+#pragma unroll
+                            for (int k = 0; k < 32; ++k)
+                                if ((code[k] & 0x7F) == 0x7F) v[k] = 0x7FC00000u;
+                        }
+                    }
+                }
+                if (!there) {
+                } else if (whole) {
+#pragma unroll
+                    for (int k = 0; k < 32; k += 8) {
+                        uint4 w;
+                        w.x = pack_out<kBf16>(__uint_as_float(v[k]) * inv, __uint_as_float(v[k + 1]) * inv);
+                        w.y = pack_out<kBf16>(__uint_as_float(v[k + 2]) * inv, __uint_as_float(v[k + 3]) * inv);
+                        w.z = pack_out<kBf16>(__uint_as_float(v[k + 4]) * inv, __uint_as_float(v[k + 5]) * inv);
+                        w.w = pack_out<kBf16>(__uint_as_float(v[k + 6]) * inv, __uint_as_float(v[k + 7]) * inv);
+                        *reinterpret_cast<uint4*>(out + c * 32 + k) = w;
+                    }
+                } else {
+#pragma unroll
+                    for (int k = 0; k < 32; k += 4)
+                        *reinterpret_cast<uint4*>(part + c * 32 + k) = make_uint4(v[k], v[k + 1], v[k + 2], v[k + 3]);
+                }
+            }
+            if (there) {
+                if (whole) {
+                    if (p.lse) p.lse[(long long)(s.req.q0 + i) * p.heads + head] = l != 0.0f ? (m + lg2(l)) * 0.6931471805599453f : -INFINITY;
+                } else {
+                    *reinterpret_cast<float2*>(p.part_ml + (slot * kManyRows + row_in_tile) * 2) = make_float2(m, l);
+                }
+            }
+            tcgen05_fence_before();                           // O has been read: the next piece may overwrite it
+            __syncwarp();
+            u = u_next;
+        }
+    } else if (warp < 12) {
+        // ------------------------------------------------------------------ queries, codes -> half, scales
+        const int tid = threadIdx.x - 256;
+        constexpr int kChunks = kDim / 16;                    // 16-code chunks of a row
+        constexpr int kPasses = kDim / 16;                    // rows of a tile that a thread has a chunk of
+        constexpr int kPassRows = 128 / kPasses;
+        const int ch = tid % kChunks, r0 = tid / kChunks;
+        int n_piece = 0, n_tile = 0;
+        for (int u = begin; u < end && ok; ++n_piece) {
+            const AttnPiece s = attn_piece<kManyRows, kManyTokens>(p, prefix, u, end);
+            u += max(1, s.tile1 - s.tile0);
+            const int* table = p.table + (long long)s.r * p.table_stride;
+            const SubTile all = sub_tile(p, s, s.row0, s.row0 + kManyRows);
+            const uint8_t* kc = cache.k + s.head * cache.head_stride + ch * 16;
+            const uint8_t* vc = cache.v + s.head * cache.head_stride + ch * 16;
+            // lanes 0..7 hold the blocks of a tile's groups of 16 tokens
+            auto block_of = [&](int t) -> int {
+                const int tok = t * kManyTokens + (lane & 7) * 16;
+                if (t >= s.tile1 || tok >= s.hi || tok + 16 <= s.lo) return -1;
+                const int block = table[tok >> p.block_shift];
+                if (block < 0 || block >= p.num_blocks) {
+                    atomicCAS(p.status, 0, DEV_BAD_CACHE_BLOCK);
+                    return -1;
+                }
+                return block;
+            };
+            auto scale_of = [&](const float* scales, int block) -> float {
+                return block >= 0 ? scales[(long long)block * p.scale_stride + s.head] : 0.0f;
+            };
+            auto load = [&](const uint8_t* base, int t, int blocks, uint4 (&w)[kPasses]) {
+#pragma unroll
+                for (int j = 0; j < kPasses; ++j) {
+                    const int row = j * kPassRows + r0, tok = t * kManyTokens + row;
+                    const int block = __shfl_sync(0xffffffffu, blocks, row >> 4);
+                    w[j] = make_uint4(0, 0, 0, 0);
+                    if (block >= 0 && tok >= s.lo && tok < s.hi)
+                        w[j] = *reinterpret_cast<const uint4*>(base + block * cache.block_stride +
+                                                               (long long)(tok & (cache.block_size - 1)) * cache.token_stride);
+                }
+            };
+            auto store = [&](uint8_t* tile, const uint4 (&w)[kPasses]) {
+#pragma unroll
+                for (int j = 0; j < kPasses; ++j) {
+                    const int row = j * kPassRows + r0;
+                    uint8_t* at = tile + (ch >> 2) * 16384 + row * 128;
+                    uint4 a, b;
+                    codes_to_half(w[j], a, b);
+                    // the two 16-byte halves in an order that keeps the eight lanes of a row on different banks
+                    const int c0 = (ch & 3) * 2, flip = (ch >> 2) & 1;
+                    const uint4 first = flip ? b : a, second = flip ? a : b;
+                    *reinterpret_cast<uint4*>(at + (((c0 + flip) ^ (row & 7)) << 4)) = first;
+                    *reinterpret_cast<uint4*>(at + (((c0 + 1 - flip) ^ (row & 7)) << 4)) = second;
+                }
+            };
+            int blk = block_of(s.tile0), blk2 = block_of(s.tile0 + 1);
+            float ks = scale_of(p.k_scale, blk), vs = scale_of(p.v_scale, blk);
+            uint4 kw[kPasses], vw[kPasses];
+            load(kc, s.tile0, blk, kw);
+
+            // ---- queries of the 256 rows: as half, bf16 rows scaled by a power of two
+            if (n_piece > 0) {
+                ok = mbar_wait(q_free, (n_piece - 1) & 1, abort_flag, p.status, DEV_TIMEOUT_SMEM_EMPTY);
+                ok = __all_sync(0xffffffffu, ok);
+                if (!ok) break;
+            }
+            {
+                constexpr int kLanes = kDim / 8;              // lanes of a row, 16 bytes each
+                constexpr int kRowsPer = 32 / kLanes;
+                constexpr int kBatch = 8;
+                const int sub = lane / kLanes, col = (lane % kLanes) * 8;
+                const float sign = p.scale_log2 < 0.0f ? -1.0f : 1.0f;
+                for (int base = (warp - 8) * 64; base < (warp - 8) * 64 + 64; base += kRowsPer * kBatch) {
+                    uint4 w[kBatch];
+#pragma unroll
+                    for (int j = 0; j < kBatch; ++j) {
+                        const int row = s.row0 + base + j * kRowsPer + sub;
+                        w[j] = make_uint4(0, 0, 0, 0);
+                        if (row < s.rows) {
+                            const int i = row / p.group;
+                            const int head = s.head * p.group + row - i * p.group;
+                            w[j] = *reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(p.q) +
+                                                                   (long long)(s.req.q0 + i) * p.q_token_stride +
+                                                                   (long long)head * p.q_head_stride + col);
+                        }
+                    }
+#pragma unroll
+                    for (int j = 0; j < kBatch; ++j) {
+                        const int rit = base + j * kRowsPer + sub;
+                        uint32_t* e = &w[j].x;
+                        int shift = 0;
+                        if constexpr (kBf16) {
+                            uint32_t mag = 0;
+#pragma unroll
+                            for (int h = 0; h < 4; ++h) {
+                                const uint32_t a = e[h] & 0x7FFFu, b = (e[h] >> 16) & 0x7FFFu;
+                                mag = max(mag, max(a < 0x7F80u ? a : 0u, b < 0x7F80u ? b : 0u));
+                            }
+#pragma unroll
+                            for (int o = 1; o < kLanes; o <<= 1) mag = max(mag, __shfl_xor_sync(0xffffffffu, mag, o));
+                            shift = query_shift(__uint_as_float(mag << 16));
+                            const float mul = pow2i(shift) * sign;
+#pragma unroll
+                            for (int h = 0; h < 4; ++h)
+                                e[h] = pack_f16(__uint_as_float(e[h] << 16) * mul, __uint_as_float(e[h] & 0xFFFF0000u) * mul);
+                        } else if (sign < 0.0f) {
+#pragma unroll
+                            for (int h = 0; h < 4; ++h) e[h] ^= 0x80008000u;
+                        }
+                        uint8_t* at = smem + L::kQOffset + (rit >> 7) * L::kOperandBytes + (col >> 6) * 16384 + (rit & 127) * 128;
+                        *reinterpret_cast<uint4*>(at + ((((col & 63) >> 3) ^ (rit & 7)) << 4)) = w[j];
+                        if (lane % kLanes == 0) row_factor[rit] = pow2i(-shift);
+                    }
+                }
+            }
+            fence_proxy_async();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(q_full);
+
+            load(vc, s.tile0, blk, vw);
+            for (int t = s.tile0; t < s.tile1; ++t, ++n_tile) {
+                const int st = n_tile & 1;
+                const uint32_t ph = (n_tile >> 1) & 1;
+                const bool partial = all.masked(t);
+                // the scales of this tile (read before: block numbers two tiles ahead, scales and codes one)
+                if (warp == 8 && lane < 8) {
+                    const float lv = fmaxf(lg2(vs), kMinLogScale);
+                    // (the scores' factor is not negative: the sign of `scale` went into the queries)
+                    meta[(n_tile % kManyMeta) * 8 + lane] =
+                        make_float4(ks * fabsf(p.scale_log2), blk >= 0 ? lv : -INFINITY, ex2(-lv), 0.0f);
+                }
+                if (warp == 8) {
+                    __syncwarp();
+                    if (lane == 0) mbar_arrive(&meta_full[n_tile % kManyMeta]);
+                }
+                blk = blk2;
+                blk2 = block_of(t + 2);
+                ks = scale_of(p.k_scale, blk);
+                vs = scale_of(p.v_scale, blk);
+                ok = mbar_wait(&k_free[st], ph ^ 1, abort_flag, p.status, DEV_TIMEOUT_SMEM_EMPTY);
+                ok = __all_sync(0xffffffffu, ok);
+                if (!ok) break;
+                store(smem + L::kKOffset + st * L::kOperandBytes, kw);
+                fence_proxy_async();
+                __syncwarp();
+                if (lane == 0) mbar_arrive(&k_full[st]);
+                if (t + 1 < s.tile1) load(kc, t + 1, blk, kw);
+                if (partial) {
+                    bool any = false;
+#pragma unroll
+                    for (int j = 0; j < kPasses; ++j) {
+                        uint32_t* w = &vw[j].x;
+#pragma unroll
+                        for (int h = 0; h < 4; ++h) {
+                            const uint32_t nb = __vcmpeq4(w[h] & 0x7F7F7F7Fu, 0x7F7F7F7Fu);
+                            any |= nb != 0;
+                            w[h] &= ~nb;
+                        }
+                    }
+                    if (any) nan_piece[n_piece & 1] = n_piece + 1;
+                }
+                ok = mbar_wait(&v_free[st], ph ^ 1, abort_flag, p.status, DEV_TIMEOUT_SMEM_EMPTY);
+                ok = __all_sync(0xffffffffu, ok);
+                if (!ok) break;
+                store(smem + L::kVOffset + st * L::kOperandBytes, vw);
+                fence_proxy_async();
+                __syncwarp();
+                if (lane == 0) mbar_arrive(&v_full[st]);
+                if (t + 1 < s.tile1) load(vc, t + 1, blk, vw);
+            }
+        }
+    } else {
+        // ------------------------------------------------------------------ MMA issue
+        constexpr uint32_t idesc_qk = umma_idesc_half(128, false);
+        constexpr uint32_t idesc_pv = umma_idesc_half(kDim, true);
+        const uint32_t q_addr = smem_u32(smem + L::kQOffset), k_addr = smem_u32(smem + L::kKOffset), v_addr = smem_u32(smem + L::kVOffset);
+        int n_piece = 0, n_tile = 0, n_mine[2] = {0, 0};
+        for (int u = begin; u < end && ok; ++n_piece) {
+            const AttnPiece s = attn_piece<kManyRows, kManyTokens>(p, prefix, u, end);
+            u += max(1, s.tile1 - s.tile0);
+            const SubTile sub[2] = {sub_tile(p, s, s.row0, s.row0 + 128), sub_tile(p, s, s.row0 + 128, s.row0 + 256)};
+            ok = mbar_wait(q_full, n_piece & 1, abort_flag, p.status, DEV_TIMEOUT_SMEM_FULL);
+            ok = __all_sync(0xffffffffu, ok);
+            if (!ok) break;
+            bool first[2] = {true, true}, pending[2] = {false, false};
+            for (int t = s.tile0; t <= s.tile1 && ok; ++t) {
+                const bool more = t < s.tile1;
+                const int st = n_tile & 1, pst = st ^ 1;       // stage of this tile, of the one before
+                if (more) {
+                    ok = mbar_wait(&k_full[st], (n_tile >> 1) & 1, abort_flag, p.status, DEV_TIMEOUT_SMEM_FULL);
+                    ok = __all_sync(0xffffffffu, ok);
+                    if (!ok) break;
+                }
+                if (t > s.tile0) {
+                    ok = mbar_wait(&v_full[pst], ((n_tile - 1) >> 1) & 1, abort_flag, p.status, DEV_TIMEOUT_SMEM_FULL);
+                    ok = __all_sync(0xffffffffu, ok);
+                    if (!ok) break;
+                }
+#pragma unroll
+                for (int x = 0; x < 2; ++x) {
+                    if (pending[x]) {
+                        ok = mbar_wait(&p_full[x], (n_mine[x] - 1) & 1, abort_flag, p.status, DEV_TIMEOUT_TMEM_EMPTY);
+                        ok = __all_sync(0xffffffffu, ok);
+                        if (!ok) break;
+                        tcgen05_fence_after();
+                        if (elect_one()) {
+                            const uint64_t b = umma_desc_sw128_mn(v_addr + pst * L::kOperandBytes, 16384);
+#pragma unroll
+                            for (int k = 0; k < 8; ++k)        // 16 tokens a step: 2048 bytes of V, 8 columns of P
+                                umma_f16_ts(tmem_o[x], tmem_s[x] + 8 * k, b + 128 * k, idesc_pv, (k > 0 || !first[x]) ? 1u : 0u);
+                            umma_commit(&pv_done[x]);
+                        }
+                        __syncwarp();
+                        first[x] = false;
+                        pending[x] = false;
+                    }
+                    if (more && sub[x].active(t)) {
+                        tcgen05_fence_after();
+                        if (elect_one()) {
+                            const uint64_t a = umma_desc_sw128(q_addr + x * L::kOperandBytes);
+                            const uint64_t b = umma_desc_sw128(k_addr + st * L::kOperandBytes);
+#pragma unroll
+                            for (int k = 0; k < kDim / 16; ++k) {   // 16 dims a step: 32 bytes, 64 dims a half
+                                const uint64_t at = (uint64_t)((k >> 2) * (16384 >> 4) + (k & 3) * 2);
+                                umma_f16_ss(tmem_s[x], a + at, b + at, idesc_qk, k > 0 ? 1u : 0u);
+                            }
+                            umma_commit(&s_full[x]);
+                        }
+                        __syncwarp();
+                        pending[x] = true;
+                        ++n_mine[x];
+                    }
+                }
+                if (!ok) break;
+                if (elect_one()) {
+                    if (more) umma_commit(&k_free[st]);
+                    if (t > s.tile0) umma_commit(&v_free[pst]);
+                    if (t == s.tile1 - 1 || s.tile0 == s.tile1) umma_commit(q_free);
+                }
+                __syncwarp();
+                if (more) ++n_tile;
+            }
+        }
+    }
+    grid_launch_dependents();
+    __syncthreads();
+    if (*abort_flag != 0) {
+        for (int i = 0; i < 64; ++i) __nanosleep(2000);       // MMAs in flight finish before their memory goes
+    }
+    tcgen05_fence_before();
+    __syncthreads();
+    if (warp == 12) {
+        __syncwarp();
+        tcgen05_fence_after();
+        tmem_dealloc<1>(tmem, 512);
+    }
+}
+
+}  // namespace blaze

@@ -189,6 +189,14 @@ constexpr float kProbShift = 15.0f;
 // A V scale enters the exponent; below 2^-64 (which the store never writes) it counts as that.
 constexpr float kMinLogScale = -64.0f;
 
+// Power of two that brings the largest magnitude of a row of bf16 queries to [2^14, 2^15), so that the row fits half
+// with all its bits; 1 for half queries, which are taken as they are.
+__device__ __forceinline__ int query_shift(float amax) {
+    const int e = (int)(__float_as_uint(amax) >> 23) - 127;
+    return amax > 0.0f ? min(max(14 - e, -120), 120) : 0;
+}
+__device__ __forceinline__ float pow2i(int e) { return __uint_as_float((uint32_t)(e + 127) << 23); }
+
 template <bool kBf16>
 __device__ __forceinline__ uint32_t pack_out(float lo, float hi) {
     return kBf16 ? pack_bf16(lo, hi) : pack_f16(lo, hi);

@@ -486,32 +486,47 @@ def peer_signal(local_flags, peer_flags, my_rank: int, peer_ranks, value: int, l
 
 # ------------------------------------------------------------------------------------------------ paged 8-bit cache
 
-def _on(t):
-    """The device of a CUDA tensor made current, and its current stream: what a call on `t` is launched with."""
+def _launch(fn, name, device: int, *args) -> None:
+    """Calls a C entry point on the current stream of the GPU that its tensors live on, with that GPU current."""
     import torch
-    return torch.cuda.device(t.device), lambda: C.c_void_p(torch.cuda.current_stream(t.device).cuda_stream)
+    if device == torch.cuda.current_device():
+        status = fn(*args, torch._C._cuda_getCurrentRawStream(device))
+    else:
+        with torch.cuda.device(device):
+            status = fn(*args, torch._C._cuda_getCurrentRawStream(device))
+    if status != STATUS_SUCCESS:
+        raise BlazeError(status, name)
 
 
-def _same_device(first, **others):
-    if not first.is_cuda:
+def _same_device(first, *others) -> int:
+    """The GPU of all these tensors (None among them is left out)."""
+    device = first.get_device()
+    if device < 0:
         raise ValueError("the cache operators take CUDA tensors")
-    for name, t in others.items():
-        if t is not None and t.device != first.device:
-            raise ValueError(f"{name} is on {t.device}, not on {first.device}")
+    for t in others:
+        if t is not None and t.get_device() != device:
+            raise ValueError(f"a tensor is on {t.device}, the others on {first.device}")
+    return device
 
 
-def _vector(t, name, dtype, at_least):
-    if t.dtype != dtype or t.dim() != 1 or t.numel() < at_least or (t.numel() > 1 and t.stride(0) != 1):
+def _vector(t, name, dtype, at_least) -> int:
+    """The address of a contiguous vector."""
+    if t.dtype is not dtype or t.dim() != 1 or t.numel() < at_least or not t.is_contiguous():
         raise ValueError(f"{name}: a contiguous {dtype} vector of at least {at_least} elements is wanted")
+    return t.data_ptr()
 
 
 def _table(t):
     """(rows, columns, pitch) of a block table."""
     import torch
-    if t.dtype != torch.int32 or t.dim() != 2 or (t.numel() and t.shape[1] > 1 and t.stride(1) != 1):
-        raise ValueError("block_table: an int32 [requests, blocks] tensor with contiguous rows is wanted")
-    pitch = t.stride(0) if t.numel() and t.shape[0] > 1 else t.shape[1]
-    return t.shape[0], t.shape[1], pitch
+    if t.dtype is not torch.int32 or t.dim() != 2:
+        raise ValueError("block_table: an int32 [requests, blocks] tensor is wanted")
+    rows, columns = t.shape
+    if rows == 0 or columns == 0 or t.is_contiguous():
+        return rows, columns, columns
+    if columns > 1 and t.stride(1) != 1:
+        raise ValueError("block_table: rows of contiguous elements are wanted")
+    return rows, columns, t.stride(0) if rows > 1 else columns
 
 
 class PagedCache:
@@ -522,7 +537,7 @@ class PagedCache:
 
     def __init__(self, k, v, k_scale, v_scale):
         import torch
-        _same_device(k, v=v, k_scale=k_scale, v_scale=v_scale)
+        _same_device(k, v, k_scale, v_scale)
         if k.dim() != 4 or k.shape != v.shape or k.dtype != v.dtype or k.dtype not in (torch.uint8, torch.float8_e4m3fn):
             raise ValueError("k and v: two [blocks, heads, block size, head size] tensors of uint8 or float8_e4m3fn")
         n, h, bs, d = k.shape
@@ -564,88 +579,68 @@ def cache_assign(cached_len, new_len, block_table, free_blocks, free_count, *, b
     import torch
     if free_count_out is None:
         free_count_out = free_count
-    _same_device(cached_len, new_len=new_len, block_table=block_table, free_blocks=free_blocks, free_count=free_count,
-                 row_offsets=row_offsets, kv_len=kv_len, slots=slots, positions=positions,
-                 free_count_out=free_count_out, denied=denied)
-    n = cached_len.numel()
-    for name, t, size in (("cached_len", cached_len, n), ("new_len", new_len, n), ("kv_len", kv_len, n),
-                          ("row_offsets", row_offsets, n + 1), ("free_blocks", free_blocks, 0),
-                          ("free_count", free_count, 1), ("free_count_out", free_count_out, 1)):
-        _vector(t, name, torch.int32, size)
-    _vector(slots, "slots", torch.int64, 0)
-    if positions is not None:
-        _vector(positions, "positions", torch.int32, slots.numel())
-    if denied is not None:
-        _vector(denied, "denied", torch.int32, 1)
+    device = _same_device(cached_len, new_len, block_table, free_blocks, free_count, row_offsets, kv_len, slots,
+                          positions, free_count_out, denied)
+    n, tokens, i32 = cached_len.numel(), slots.numel(), torch.int32
     rows, columns, pitch = _table(block_table)
     if rows < n:
         raise ValueError("block_table has fewer rows than there are requests")
-    a = CacheAssignArgs()
-    a.struct_size = C.sizeof(CacheAssignArgs)
-    a.requests, a.block_size, a.max_blocks, a.max_tokens = n, block_size, columns, slots.numel()
-    a.cached_len, a.new_len = cached_len.data_ptr(), new_len.data_ptr()
-    a.block_table, a.table_stride = block_table.data_ptr(), pitch
-    a.free_blocks, a.free_capacity = free_blocks.data_ptr(), free_blocks.numel()
-    a.free_count, a.free_count_out = free_count.data_ptr(), free_count_out.data_ptr()
-    a.row_offsets, a.kv_len, a.slots = row_offsets.data_ptr(), kv_len.data_ptr(), slots.data_ptr()
-    a.positions = positions.data_ptr() if positions is not None else None
-    a.denied = denied.data_ptr() if denied is not None else None
-    on, stream = _on(cached_len)
-    with on:
-        check(lib().blazeCacheAssign(C.byref(a), stream()), "blazeCacheAssign")
+    a = CacheAssignArgs(
+        C.sizeof(CacheAssignArgs), n, block_size, columns, tokens,
+        _vector(cached_len, "cached_len", i32, n), _vector(new_len, "new_len", i32, n),
+        block_table.data_ptr(), pitch,
+        _vector(free_blocks, "free_blocks", i32, 0), free_blocks.numel(), 0,
+        _vector(free_count, "free_count", i32, 1), _vector(free_count_out, "free_count_out", i32, 1),
+        _vector(row_offsets, "row_offsets", i32, n + 1), _vector(kv_len, "kv_len", i32, n),
+        _vector(slots, "slots", torch.int64, 0),
+        None if positions is None else _vector(positions, "positions", i32, tokens),
+        None if denied is None else _vector(denied, "denied", i32, 1))
+    _launch(lib().blazeCacheAssign, "blazeCacheAssign", device, a)
 
 
-def _rows_type(t, name):
+def _rows(t, name):
+    """(address, token stride, head stride) of bf16 or half rows [tokens, heads, head size]; the stride of a dimension
+    of one, which never counts, as 0."""
     import torch
-    if t.dtype not in (torch.bfloat16, torch.float16) or t.dim() != 3 or (t.shape[2] > 1 and t.stride(2) != 1):
-        raise ValueError(f"{name}: a bf16 or half [tokens, heads, head size] tensor with contiguous rows is wanted")
-    return out_type_of(t)
+    if (t.dtype is not torch.bfloat16 and t.dtype is not torch.float16) or t.dim() != 3:
+        raise ValueError(f"{name}: a bf16 or half [tokens, heads, head size] tensor is wanted")
+    st, sh, sd = t.stride()
+    if sd != 1 and t.shape[2] > 1:
+        raise ValueError(f"{name}: the last dimension must be contiguous")
+    return t.data_ptr(), st if t.shape[0] > 1 else 0, sh if t.shape[1] > 1 else 0
 
 
 def cache_store(cache: PagedCache, k, v, slots):
     """Quantises the rows of `k` and `v` [tokens, kv heads, head size] into the cache's slots (blazeCacheStore)."""
     import torch
-    _same_device(cache.k, k=k, v=v, slots=slots)
-    _vector(slots, "slots", torch.int64, 0)
+    device = _same_device(cache.k, k, v, slots)
+    at = _vector(slots, "slots", torch.int64, 0)
     n = slots.numel()
-    for name, t in (("k", k), ("v", v)):
-        _rows_type(t, name)
-        if t.dtype != k.dtype or t.shape[0] < n or tuple(t.shape[1:]) != (cache.kv_heads, cache.head_dim):
-            raise ValueError(f"{name}: [at least {n}, {cache.kv_heads}, {cache.head_dim}] is wanted, of one type")
-    a = CacheStoreArgs()
-    a.struct_size = C.sizeof(CacheStoreArgs)
-    a.tokens, a.in_type = n, out_type_of(k)
-    a.k, a.v = k.data_ptr(), v.data_ptr()
-    a.k_token_stride, a.k_head_stride = _row_strides(k)
-    a.v_token_stride, a.v_head_stride = _row_strides(v)
-    a.slots = slots.data_ptr()
-    on, stream = _on(cache.k)
-    with on:
-        check(lib().blazeCacheStore(C.byref(cache.desc), C.byref(a), stream()), "blazeCacheStore")
+    pk, k_token, k_head = _rows(k, "k")
+    pv, v_token, v_head = _rows(v, "v")
+    rows = (cache.kv_heads, cache.head_dim)
+    if k.dtype is not v.dtype or k.shape[0] < n or v.shape[0] < n or k.shape[1:] != rows or v.shape[1:] != rows:
+        raise ValueError(f"k and v: [at least {n}, {cache.kv_heads}, {cache.head_dim}] is wanted, of one type")
+    a = CacheStoreArgs(C.sizeof(CacheStoreArgs), n, out_type_of(k), pk, pv, k_token, k_head, v_token, v_head, at)
+    _launch(lib().blazeCacheStore, "blazeCacheStore", device, cache.desc, a)
 
 
-def _row_strides(t):
-    """Token and head strides; a dimension of one has none that counts."""
-    return t.stride(0) if t.shape[0] > 1 else 0, t.stride(1) if t.shape[1] > 1 else 0
-
-
-def _attention_args(cache, q, *, requests, max_q, max_kv, max_blocks, min_q=0, scale=1.0, causal=True, window=0,
-                    sm_limit=0) -> CacheAttentionArgs:
-    a = CacheAttentionArgs()
-    a.struct_size = C.sizeof(CacheAttentionArgs)
-    a.requests, a.tokens, a.heads, a.q_type = requests, q.shape[0], q.shape[1], _rows_type(q, "q")
-    a.max_blocks = a.table_stride = max_blocks
-    a.max_q, a.min_q, a.max_kv = max_q, min_q, max_kv
-    a.scale, a.causal, a.window, a.sm_limit = scale, 1 if causal else 0, window, sm_limit
-    return a
+def _attention_bounds(cache, q, requests, max_q, max_kv, sm_limit) -> CacheAttentionArgs:
+    """Arguments as far as the workspace's size depends on them."""
+    blocks = -(-max_kv // cache.block_size)
+    return CacheAttentionArgs(struct_size=C.sizeof(CacheAttentionArgs), requests=requests, tokens=q.shape[0],
+                              heads=q.shape[1], q_type=out_type_of(q), table_stride=blocks, max_blocks=blocks,
+                              max_q=max_q, max_kv=max_kv, scale=1.0, sm_limit=sm_limit)
 
 
 def cache_attention_workspace_bytes(cache: PagedCache, q, *, requests, max_q, max_kv, sm_limit=0) -> int:
-    a = _attention_args(cache, q, requests=requests, max_q=max_q, max_kv=max_kv,
-                        max_blocks=-(-max_kv // cache.block_size), sm_limit=sm_limit)
+    import torch
     n = C.c_size_t(0)
-    check(lib().blazeCacheAttentionWorkspaceSize(C.byref(cache.desc), C.byref(a), C.byref(n)),
-          "blazeCacheAttentionWorkspaceSize")
+    _rows(q, "q")
+    with torch.cuda.device(cache.device):
+        check(lib().blazeCacheAttentionWorkspaceSize(
+            cache.desc, _attention_bounds(cache, q, requests, max_q, max_kv, sm_limit), C.byref(n)),
+            "blazeCacheAttentionWorkspaceSize")
     return n.value
 
 
@@ -663,41 +658,34 @@ def cache_attention(cache: PagedCache, q, row_offsets, kv_len, block_table, *, s
     Allocates `out` (zeros: rows outside every request are not written) and `workspace` when not given; fills `lse`
     [tokens, heads] float32 when given."""
     import torch
-    _same_device(cache.k, q=q, row_offsets=row_offsets, kv_len=kv_len, block_table=block_table, out=out, lse=lse,
-                 workspace=workspace)
-    n = kv_len.numel()
-    _vector(kv_len, "kv_len", torch.int32, 0)
-    _vector(row_offsets, "row_offsets", torch.int32, n + 1)
-    rows, columns, pitch = _table(block_table)
-    if rows < n:
-        raise ValueError("block_table has fewer rows than there are requests")
-    _rows_type(q, "q")
-    if q.shape[2] != cache.head_dim:
-        raise ValueError(f"q has heads of {q.shape[2]}, the cache of {cache.head_dim}")
     if out is None:
         out = torch.zeros(q.shape, dtype=q.dtype, device=q.device)
-    _rows_type(out, "out")
-    if out.shape != q.shape or out.dtype != q.dtype:
+    if workspace is None:
+        workspace = cache_attention_workspace(cache, q, requests=kv_len.numel(), max_q=max_q, max_kv=max_kv,
+                                              sm_limit=sm_limit)
+    device = _same_device(cache.k, q, row_offsets, kv_len, block_table, out, lse, workspace)
+    n = kv_len.numel()
+    offsets, lens = _vector(row_offsets, "row_offsets", torch.int32, n + 1), _vector(kv_len, "kv_len", torch.int32, 0)
+    table_rows, columns, pitch = _table(block_table)
+    if table_rows < n:
+        raise ValueError("block_table has fewer rows than there are requests")
+    pq, q_token, q_head = _rows(q, "q")
+    po, out_token, out_head = _rows(out, "out")
+    tokens, heads, dim = q.shape
+    if dim != cache.head_dim:
+        raise ValueError(f"q has heads of {dim}, the cache of {cache.head_dim}")
+    if out.shape != q.shape or out.dtype is not q.dtype:
         raise ValueError("out must have q's shape and type")
-    if lse is not None and (lse.dtype != torch.float32 or lse.shape != q.shape[:2] or not lse.is_contiguous()):
+    if lse is not None and (lse.dtype is not torch.float32 or lse.shape != (tokens, heads) or not lse.is_contiguous()):
         raise ValueError("lse: a contiguous float32 [tokens, heads] tensor is wanted")
-    a = _attention_args(cache, q, requests=n, max_q=max_q, max_kv=max_kv, max_blocks=columns, min_q=min_q,
-                        scale=cache.head_dim ** -0.5 if scale is None else scale, causal=causal, window=window,
-                        sm_limit=sm_limit)
-    a.q, (a.q_token_stride, a.q_head_stride) = q.data_ptr(), _row_strides(q)
-    a.out, (a.out_token_stride, a.out_head_stride) = out.data_ptr(), _row_strides(out)
-    a.lse = lse.data_ptr() if lse is not None else None
-    a.row_offsets, a.kv_len = row_offsets.data_ptr(), kv_len.data_ptr()
-    a.block_table, a.table_stride = block_table.data_ptr(), pitch
-    on, stream = _on(cache.k)
-    with on:
-        if workspace is None:
-            need = C.c_size_t(0)
-            check(lib().blazeCacheAttentionWorkspaceSize(C.byref(cache.desc), C.byref(a), C.byref(need)),
-                  "blazeCacheAttentionWorkspaceSize")
-            workspace = torch.empty(max(need.value, 256), dtype=torch.uint8, device=cache.device)
-        a.workspace, a.workspace_bytes = workspace.data_ptr(), workspace.numel() * workspace.element_size()
-        check(lib().blazeCacheAttention(C.byref(cache.desc), C.byref(a), stream()), "blazeCacheAttention")
+    if not workspace.is_contiguous():
+        raise ValueError("workspace: a contiguous tensor is wanted")
+    a = CacheAttentionArgs(
+        C.sizeof(CacheAttentionArgs), n, tokens, heads, out_type_of(q), pq, q_token, q_head, po, out_token, out_head,
+        None if lse is None else lse.data_ptr(), offsets, lens, block_table.data_ptr(), pitch, columns,
+        max_q, min_q, max_kv, dim ** -0.5 if scale is None else scale, 1 if causal else 0, window, sm_limit,
+        workspace.data_ptr(), workspace.numel() * workspace.element_size())
+    _launch(lib().blazeCacheAttention, "blazeCacheAttention", device, cache.desc, a)
     return out
 
 

@@ -6,11 +6,12 @@
 //   warps 0-3, 4-7   softmax of sub-tile A / B: scores from TMEM, probabilities back into the same TMEM columns as half
 //                    (the A operand of P V), O re-scaled in TMEM when a row's maximum has grown by more than 2^8
 //                    since it was last taken, the piece's epilogue
-//   warps 8-11       codes -> half: 16-byte loads of the pages straight from global memory, one tile ahead in registers,
-//                    converted (exactly) and stored into the 128-byte-swizzled operand tiles; block numbers and scales of the
-//                    tiles; the queries of a row tile
+//   warps 8-11       codes -> half: a thread copies its 16-byte pieces of the pages (cp.async, an operand tile and a half
+//                    ahead) into a staging slot of its own and expands them (exactly) into the 128-byte-swizzled operand
+//                    tile, a ring of three that K and V take turns in; block numbers and scales of the tiles
 //   warp 12          issues the MMAs: P_A V(t), Q_A K(t+1), P_B V(t), Q_B K(t+1), so each warpgroup's softmax runs while the
 //                    tensor cores work for the other one
+// The softmax threads also bring their own query row into shared memory at the start of a piece.
 // Q K^T takes K as the K-major operand; P V takes V as it lies, dims contiguous (MN-major), no transposition anywhere.
 #pragma once
 
@@ -32,12 +33,12 @@ struct ManySmem {
     static constexpr int kHalves = kDim / 64;                        // 64-wide (128-byte) column halves
     static constexpr int kOperandBytes = 128 * kDim * 2;             // 128 rows of Q, K or V as half
     static constexpr int kQOffset = 0;                               // A, B
-    static constexpr int kKOffset = 2 * kOperandBytes;               // two stages
-    static constexpr int kVOffset = kKOffset + 2 * kOperandBytes;    // two stages
-    static constexpr int kMetaOffset = kVOffset + 2 * kOperandBytes; // float4 [kManyMeta][8]
-    static constexpr int kRowOffset = kMetaOffset + kManyMeta * 8 * 16;    // float [256]: score factor of each row
-    static constexpr int kBarOffset = kRowOffset + kManyRows * 4;
-    static constexpr int kNumBars = 2 + 4 + 4 + kManyMeta + 6;
+    static constexpr int kRingOffset = 2 * kOperandBytes;            // three operand tiles, K and V in turn
+    static constexpr int kRawOffset = kRingOffset + 3 * kOperandBytes;     // codes of a K and of a V tile
+    static constexpr int kRawBytes = 128 * kDim;
+    static constexpr int kMetaOffset = kRawOffset + 2 * kRawBytes;   // float4 [kManyMeta][8]
+    static constexpr int kBarOffset = kMetaOffset + kManyMeta * 8 * 16;
+    static constexpr int kNumBars = 2 + 6 + kManyMeta + 6;
     static constexpr int kMiscOffset = kBarOffset + kNumBars * 8;
     static constexpr int kPrefixOffset = kMiscOffset + 128;
     static int bytes(int requests) { return 1024 + kPrefixOffset + (requests + 1) * 4; }
@@ -90,6 +91,11 @@ __device__ __forceinline__ void tmem_st_32x32(uint32_t taddr, const uint32_t (&r
         "r"(r[28]), "r"(r[29]), "r"(r[30]), "r"(r[31])
         : "memory");
 }
+__device__ __forceinline__ float max3(float a, float b, float c) {
+    float d;
+    asm("max.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
+    return d;
+}
 __device__ __forceinline__ void tmem_st_wait() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
 
 // Tokens [lo, hi) that any row of the sub-tile of 128 rows at `row0` sees, and [all_lo, all_hi) that every row sees.
@@ -102,7 +108,7 @@ struct SubTile {
         return t * kManyTokens < all_lo || (t + 1) * kManyTokens > all_hi;
     }
 };
-__device__ __forceinline__ SubTile sub_tile(const CacheAttentionParams& p, const AttnPiece& s, int row0, int row1) {
+__device__ __noinline__ SubTile sub_tile(const CacheAttentionParams& p, const AttnPiece& s, int row0, int row1) {
     SubTile x;
     const int end = min(s.rows, row1);
     if (row0 >= end) {
@@ -117,6 +123,14 @@ __device__ __forceinline__ SubTile sub_tile(const CacheAttentionParams& p, const
     if (x.hi <= x.lo) x.lo = x.hi = 0;
     return x;
 }
+
+// 16 bytes global -> shared, or zeros where `bytes` is 0 (nothing is read then).
+__device__ __forceinline__ void cp_async16(void* dst, const void* src, int bytes) {
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(smem_u32(dst)), "l"(src), "r"(bytes) : "memory");
+}
+__device__ __forceinline__ void cp_async_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int kPending>
+__device__ __forceinline__ void cp_async_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(kPending) : "memory"); }
 
 // 16 E4M3 codes -> 16 halves.
 __device__ __forceinline__ void codes_to_half(const uint4& w, uint4& a, uint4& b) {
@@ -139,40 +153,37 @@ cache_attention_many_kernel(const CacheAttentionParams p, const CacheView cache)
     extern __shared__ uint8_t many_smem_raw[];
     uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(many_smem_raw) + 1023) & ~uintptr_t(1023));
     float4* meta = reinterpret_cast<float4*>(smem + L::kMetaOffset);
-    float* row_factor = reinterpret_cast<float*>(smem + L::kRowOffset);
     uint64_t* bars = reinterpret_cast<uint64_t*>(smem + L::kBarOffset);
-    uint64_t* q_full = bars;                  // the converting warps
-    uint64_t* q_free = bars + 1;              // the last Q K^T of the piece, and the eight softmax warps that took the factors
-    uint64_t* k_full = bars + 2;              // [2]
-    uint64_t* k_free = bars + 4;              // [2]
-    uint64_t* v_full = bars + 6;              // [2]
-    uint64_t* v_free = bars + 8;              // [2]
-    uint64_t* meta_full = bars + 10;          // [kManyMeta]
-    uint64_t* s_full = bars + 10 + kManyMeta;     // [2] sub-tiles
+    uint64_t* q_full = bars;                  // the softmax warps
+    uint64_t* q_free = bars + 1;              // the last Q K^T of the piece
+    uint64_t* full = bars + 2;                // [3] operand tile expanded (the converting warps)
+    uint64_t* free_ = bars + 5;               // [3] its last product done
+    uint64_t* meta_full = bars + 8;           // [kManyMeta]
+    uint64_t* s_full = meta_full + kManyMeta; // [2] sub-tiles
     uint64_t* p_full = s_full + 2;            // [2]
     uint64_t* pv_done = s_full + 4;           // [2]
-    int* misc = reinterpret_cast<int*>(smem + L::kMiscOffset);           // [0, 16): sums; 16: TMEM; 17: abort; 18, 19: last piece (+ 1) with NaN codes taken out
+    int* misc = reinterpret_cast<int*>(smem + L::kMiscOffset);           // [0, 16): sums; 16: TMEM; 17: abort; 18..25: NaN tiles
     uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(misc + 16);
     volatile int* abort_flag = misc + 17;
-    volatile int* nan_piece = misc + 18;       // by the parity of the piece
+    volatile int* nan_tile = misc + 18;       // number (+ 1) of the last tile of each 8 whose V lost NaN codes
     int* prefix = reinterpret_cast<int*>(smem + L::kPrefixOffset);
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
 
     if (threadIdx.x == 0) {
-        mbar_init(q_full, 4);
-        mbar_init(q_free, 9);
+        mbar_init(q_full, 8);
+        mbar_init(q_free, 1);
+        for (int i = 0; i < 3; ++i) {
+            mbar_init(&full[i], 4);
+            mbar_init(&free_[i], 1);
+        }
         for (int i = 0; i < 2; ++i) {
-            mbar_init(&k_full[i], 4);
-            mbar_init(&k_free[i], 1);
-            mbar_init(&v_full[i], 4);
-            mbar_init(&v_free[i], 1);
             mbar_init(&s_full[i], 1);
             mbar_init(&p_full[i], 4);
             mbar_init(&pv_done[i], 1);
         }
         for (int i = 0; i < kManyMeta; ++i) mbar_init(&meta_full[i], 1);
         *abort_flag = 0;
-        nan_piece[0] = nan_piece[1] = 0;
+        for (int i = 0; i < 8; ++i) nan_tile[i] = 0;
         fence_mbar_init();
     }
     if (warp == 12) tmem_alloc<1>(tmem_slot, 512);
@@ -208,57 +219,117 @@ cache_attention_many_kernel(const CacheAttentionParams p, const CacheView cache)
             const int pos = s.req.kv - s.req.qlen + i;
             const int see_hi = there ? (p.causal ? min(s.req.kv, pos + 1) : s.req.kv) : 0;
             const int see_lo = p.window > 0 ? max(0, pos - p.window + 1) : 0;
-            ok = mbar_wait(q_full, n_piece & 1, abort_flag, p.status, DEV_TIMEOUT_SMEM_FULL);
-            ok = __all_sync(0xffffffffu, ok);
-            if (!ok) break;
-            const float factor = row_factor[row_in_tile];
-            __syncwarp();
-            if (lane == 0) mbar_arrive(q_free);
+            // ---- this thread's query row, as half (bf16 rows scaled by a power of two, the sign of `scale` taken in)
+            float factor = 1.0f;
+            {
+                constexpr int kLoads = kDim / 8;
+                uint4 w[kLoads];
+                const uint16_t* src = static_cast<const uint16_t*>(p.q) + (long long)(s.req.q0 + i) * p.q_token_stride +
+                                      (long long)head * p.q_head_stride;
+#pragma unroll
+                for (int k = 0; k < kLoads; ++k)
+                    w[k] = there ? *reinterpret_cast<const uint4*>(src + 8 * k) : make_uint4(0, 0, 0, 0);
+                if constexpr (kBf16) {
+                    uint32_t mag = 0;
+#pragma unroll
+                    for (int k = 0; k < kLoads; ++k) {
+                        const uint32_t* e = &w[k].x;
+#pragma unroll
+                        for (int h = 0; h < 4; ++h) {
+                            const uint32_t a = e[h] & 0x7FFFu, b = (e[h] >> 16) & 0x7FFFu;
+                            mag = max(mag, max(a < 0x7F80u ? a : 0u, b < 0x7F80u ? b : 0u));
+                        }
+                    }
+                    const int shift = query_shift(__uint_as_float(mag << 16));
+                    factor = pow2i(-shift);
+                    const float mul = p.scale_log2 < 0.0f ? -pow2i(shift) : pow2i(shift);
+#pragma unroll
+                    for (int k = 0; k < kLoads; ++k) {
+                        uint32_t* e = &w[k].x;
+#pragma unroll
+                        for (int h = 0; h < 4; ++h)
+                            e[h] = pack_f16(__uint_as_float(e[h] << 16) * mul, __uint_as_float(e[h] & 0xFFFF0000u) * mul);
+                    }
+                } else {
+                    const uint32_t flip = p.scale_log2 < 0.0f ? 0x80008000u : 0u;
+#pragma unroll
+                    for (int k = 0; k < kLoads; ++k) {
+                        w[k].x ^= flip; w[k].y ^= flip; w[k].z ^= flip; w[k].w ^= flip;
+                    }
+                }
+                if (n_piece > 0) {
+                    ok = attn_wait(q_free, (n_piece - 1) & 1, abort_flag, p.status, DEV_TIMEOUT_SMEM_EMPTY);
+                    if (!ok) break;
+                }
+                uint8_t* at = smem + L::kQOffset + x * L::kOperandBytes + (row_in_tile & 127) * 128;
+#pragma unroll
+                for (int k = 0; k < kLoads; ++k)
+                    *reinterpret_cast<uint4*>(at + (k >> 3) * 16384 + (((k & 7) ^ (row_in_tile & 7)) << 4)) = w[k];
+                fence_proxy_async();
+                __syncwarp();
+                if (lane == 0) mbar_arrive(q_full);
+            }
 
             float m = -INFINITY, l = 0.0f;
             int done = 0;                                     // tiles of this piece whose P V has been asked for
+            bool nans = false;                                // V of one of them lost NaN codes
+            int before = 0;                                   // number of the last of them
             for (int t = s.tile0; t < s.tile1; ++t, ++n_tile) {
                 if (!sub.active(t)) continue;
-                ok = mbar_wait(&meta_full[n_tile % kManyMeta], (n_tile / kManyMeta) & 1, abort_flag, p.status, DEV_TIMEOUT_SMEM_FULL) &&
-                     mbar_wait(&s_full[x], n_mine & 1, abort_flag, p.status, DEV_TIMEOUT_TMEM_FULL);
-                ok = __all_sync(0xffffffffu, ok);
+                ok = attn_wait(&meta_full[n_tile % kManyMeta], (n_tile / kManyMeta) & 1, abort_flag, p.status, DEV_TIMEOUT_SMEM_FULL) &&
+                     attn_wait(&s_full[x], n_mine & 1, abort_flag, p.status, DEV_TIMEOUT_TMEM_FULL);
                 if (!ok) break;
                 tcgen05_fence_after();
+                if (done > 0) nans |= nan_tile[before & 7] == before + 1;
                 const float4* mt = meta + (n_tile % kManyMeta) * 8;
                 const bool masked = sub.masked(t);
                 const int tok0 = t * kManyTokens;
                 // bits of the tokens [tok0 + 16 g, + 16) that this row sees
                 auto seen = [&](int g) -> uint32_t {
-                    const int a = max(see_lo - (tok0 + 16 * g), 0), b = min(see_hi - (tok0 + 16 * g), 16);
+                    const int at = tok0 + 16 * g;
+                    const int a = max(see_lo - at, 0), b = min(see_hi - at, 16);
                     return b > a ? ((1u << b) - 1u) & ~((1u << a) - 1u) : 0u;
                 };
-                // ---- largest score of the row
+                // ---- the row's largest exponent.  (Blocks that do not exist have codes of zero and an exponent of -inf.)
                 float mx = -INFINITY;
+                if (!masked) {
+#pragma unroll 1
+                    for (int c = 0; c < 4; ++c) {
+                        uint32_t v[32];
+                        tmem_ld_32x32(ts + c * 32, v);
+                        tmem_ld_wait();
 #pragma unroll
-                for (int c = 0; c < 4; ++c) {
-                    uint32_t v[32];
-                    __syncwarp();
-                    tmem_ld_32x32(ts + c * 32, v);
-                    tmem_ld_wait();
+                        for (int h = 0; h < 2; ++h) {
+                            const float4 q = mt[2 * c + h];
+                            float g = __uint_as_float(v[16 * h]), g2 = __uint_as_float(v[16 * h + 1]);
 #pragma unroll
-                    for (int h = 0; h < 2; ++h) {
-                        const float4 q = mt[2 * c + h];
-                        if (q.y == -INFINITY) continue;
-                        float g = -INFINITY;
-                        if (masked) {
-                            const uint32_t bits = seen(2 * c + h);
-                            if (bits == 0) continue;
-#pragma unroll
-                            for (int k = 0; k < 16; ++k)
-                                if (bits >> k & 1) g = fmaxf(g, __uint_as_float(v[16 * h + k]));
-                        } else {
-#pragma unroll
-                            for (int k = 0; k < 16; ++k) g = fmaxf(g, __uint_as_float(v[16 * h + k]));
+                            for (int k = 2; k < 14; k += 4) {
+                                g = max3(g, __uint_as_float(v[16 * h + k]), __uint_as_float(v[16 * h + k + 1]));
+                                g2 = max3(g2, __uint_as_float(v[16 * h + k + 2]), __uint_as_float(v[16 * h + k + 3]));
+                            }
+                            g = max3(g, __uint_as_float(v[16 * h + 14]), __uint_as_float(v[16 * h + 15]));
+                            mx = fmaxf(mx, fmaf(fmaxf(g, g2), factor * q.x, q.y));
                         }
-                        mx = fmaxf(mx, fmaf(g, factor * q.x, q.y));
+                    }
+                } else {
+#pragma unroll 1
+                    for (int c = 0; c < 4; ++c) {
+                        uint32_t v[32];
+                        __syncwarp();
+                        tmem_ld_32x32(ts + c * 32, v);
+                        tmem_ld_wait();
+#pragma unroll
+                        for (int h = 0; h < 2; ++h) {
+                            const float4 q = mt[2 * c + h];
+                            const uint32_t bits = seen(2 * c + h);
+                            float g = -INFINITY;
+#pragma unroll
+                            for (int k = 0; k < 16; ++k) g = fmaxf(g, bits >> k & 1 ? __uint_as_float(v[16 * h + k]) : -INFINITY);
+                            if (bits != 0) mx = fmaxf(mx, fmaf(g, factor * q.x, q.y));
+                        }
                     }
                 }
-                // ---- a new reference, where the row has outgrown the old one
+                // ---- a new reference, only where a score has outgrown the old one by 2^15 (and in a piece's first tile)
                 const bool grow = mx > m + kManyGrow;
                 if (__any_sync(0xffffffffu, grow)) {
                     const float m_new = grow ? mx - kManyShift : m;
@@ -266,13 +337,13 @@ cache_attention_many_kernel(const CacheAttentionParams p, const CacheView cache)
                     m = m_new;
                     l *= al;
                     if (done > 0) {
-                        ok = mbar_wait(&pv_done[x], (n_mine - 1) & 1, abort_flag, p.status, DEV_TIMEOUT_TMEM_FULL);
-                        ok = __all_sync(0xffffffffu, ok);
+                        ok = attn_wait(&pv_done[x], (n_mine - 1) & 1, abort_flag, p.status, DEV_TIMEOUT_TMEM_FULL);
                         if (!ok) break;
                         tcgen05_fence_after();
-#pragma unroll
+#pragma unroll 1
                         for (int c = 0; c < kDim / 32; ++c) {
                             uint32_t v[32];
+                            __syncwarp();
                             tmem_ld_32x32(to + c * 32, v);
                             tmem_ld_wait();
 #pragma unroll
@@ -282,57 +353,57 @@ cache_attention_many_kernel(const CacheAttentionParams p, const CacheView cache)
                     }
                 }
                 const float ms = m == -INFINITY ? 0.0f : m;
-                // ---- probabilities
-#pragma unroll
+                // ---- probabilities, over the scores' own columns (those of 32 tokens fit the columns of 16, read before)
+#pragma unroll 1
                 for (int c = 0; c < 4; ++c) {
                     uint32_t v[32], w[16];
                     __syncwarp();
                     tmem_ld_32x32(ts + c * 32, v);
+                    const float4 q0 = mt[2 * c], q1 = mt[2 * c + 1];
                     tmem_ld_wait();
+                    if (masked) {
+                        // (a score that the row does not see may be anything: taken out before the exponential)
+                        const uint32_t bits = seen(2 * c) | seen(2 * c + 1) << 16;
+#pragma unroll
+                        for (int k = 0; k < 32; ++k) v[k] = bits >> k & 1 ? v[k] : 0xFF800000u;
+                    }
 #pragma unroll
                     for (int h = 0; h < 2; ++h) {
-                        const float4 q = mt[2 * c + h];
-                        const float k1 = factor * q.x, k0 = q.y - ms;
-                        float sum = 0.0f;
-                        if (q.y == -INFINITY) {
+                        const float4 q = h ? q1 : q0;
+                        const float k1 = fmaxf(factor * q.x, masked ? 1e-37f : 0.0f), k0 = q.y - ms;
+                        float part = 0.0f, part2 = 0.0f;
 #pragma unroll
-                            for (int k = 0; k < 8; ++k) w[8 * h + k] = 0;
-                        } else {
-                            const uint32_t bits = masked ? seen(2 * c + h) : 0xFFFFu;
-#pragma unroll
-                            for (int k = 0; k < 16; k += 2) {
-                                float a = ex2(fmaf(__uint_as_float(v[16 * h + k]), k1, k0));
-                                float b = ex2(fmaf(__uint_as_float(v[16 * h + k + 1]), k1, k0));
-                                if (masked) {
-                                    if (!(bits >> k & 1)) a = 0.0f;
-                                    if (!(bits >> k & 2)) b = 0.0f;
-                                }
-                                sum += a + b;
-                                w[8 * h + (k >> 1)] = pack_f16(a, b);
-                            }
-                            l = fmaf(sum, q.z, l);
+                        for (int k = 0; k < 16; k += 4) {
+                            const float a = ex2(fmaf(__uint_as_float(v[16 * h + k]), k1, k0));
+                            const float b = ex2(fmaf(__uint_as_float(v[16 * h + k + 1]), k1, k0));
+                            const float d = ex2(fmaf(__uint_as_float(v[16 * h + k + 2]), k1, k0));
+                            const float e = ex2(fmaf(__uint_as_float(v[16 * h + k + 3]), k1, k0));
+                            part += a + b;
+                            part2 += d + e;
+                            w[8 * h + (k >> 1)] = pack_f16(a, b);
+                            w[8 * h + (k >> 1) + 1] = pack_f16(d, e);
                         }
+                        l = fmaf(part + part2, q.z, l);
                     }
-                    __syncwarp();
                     tmem_st_32x16(ts + c * 16, w);
                 }
                 tmem_st_wait();
                 tcgen05_fence_before();
                 __syncwarp();
                 if (lane == 0) mbar_arrive(&p_full[x]);
+                before = n_tile;
                 ++done;
                 ++n_mine;
             }
             if (!ok) break;
             // ---- epilogue
             if (done > 0) {
-                ok = mbar_wait(&pv_done[x], (n_mine - 1) & 1, abort_flag, p.status, DEV_TIMEOUT_TMEM_FULL);
-                ok = __all_sync(0xffffffffu, ok);
+                ok = attn_wait(&pv_done[x], (n_mine - 1) & 1, abort_flag, p.status, DEV_TIMEOUT_TMEM_FULL);
                 if (!ok) break;
                 tcgen05_fence_after();
+                nans |= nan_tile[before & 7] == before + 1;
             }
             const bool whole = s.item0 >= begin && s.item1 <= end;
-            const bool nans = nan_piece[n_piece & 1] == n_piece + 1;
             const float inv = l != 0.0f ? 1.0f / l : 0.0f;
             const long long slot = (long long)blockIdx.x * 2 + (u == begin ? 0 : 1);
             uint16_t* out = static_cast<uint16_t*>(p.out) + (long long)(s.req.q0 + i) * p.out_token_stride +
@@ -396,245 +467,208 @@ cache_attention_many_kernel(const CacheAttentionParams p, const CacheView cache)
             u = u_next;
         }
     } else if (warp < 12) {
-        // ------------------------------------------------------------------ queries, codes -> half, scales
+        // ------------------------------------------------------------------ codes -> half, scales
         const int tid = threadIdx.x - 256;
         constexpr int kChunks = kDim / 16;                    // 16-code chunks of a row
         constexpr int kPasses = kDim / 16;                    // rows of a tile that a thread has a chunk of
-        constexpr int kPassRows = 128 / kPasses;
+        constexpr int kPassRows = 128 / kPasses;              // (16 or 32: a warp's rows of a pass are of one group of 16)
         const int ch = tid % kChunks, r0 = tid / kChunks;
-        int n_piece = 0, n_tile = 0;
-        for (int u = begin; u < end && ok; ++n_piece) {
+        // where the two halves of a piece go in an operand tile, in an order that keeps the eight lanes of a row on
+        // different banks
+        const int flip = (ch >> 2) & 1;
+        const uint32_t to_a = (ch >> 2) * 16384 + r0 * 128 + ((((ch & 3) * 2 + flip) ^ (r0 & 7)) << 4);
+        const uint32_t to_b = (ch >> 2) * 16384 + r0 * 128 + ((((ch & 3) * 2 + 1 - flip) ^ (r0 & 7)) << 4);
+        uint8_t* raw = smem + L::kRawOffset + tid * 16;
+        int n_tile = 0, ring = 0;                             // tiles so far; place in the ring
+        uint32_t ring_phase = 1;
+        for (int u = begin; u < end && ok;) {
             const AttnPiece s = attn_piece<kManyRows, kManyTokens>(p, prefix, u, end);
             u += max(1, s.tile1 - s.tile0);
+            if (s.tile0 == s.tile1) continue;
             const int* table = p.table + (long long)s.r * p.table_stride;
             const SubTile all = sub_tile(p, s, s.row0, s.row0 + kManyRows);
-            const uint8_t* kc = cache.k + s.head * cache.head_stride + ch * 16;
-            const uint8_t* vc = cache.v + s.head * cache.head_stride + ch * 16;
-            // lanes 0..7 hold the blocks of a tile's groups of 16 tokens
-            auto block_of = [&](int t) -> int {
+            const long long mine = s.head * cache.head_stride + (r0 & 15) * cache.token_stride + ch * 16;
+            // lanes 0..7 hold the blocks of a tile's groups of 16 tokens, -1 for one that has none or that nobody sees
+            // (read two tiles ahead, looked at one tile later: nothing waits for the table)
+            auto wanted = [&](int t) -> bool {
                 const int tok = t * kManyTokens + (lane & 7) * 16;
-                if (t >= s.tile1 || tok >= s.hi || tok + 16 <= s.lo) return -1;
-                const int block = table[tok >> p.block_shift];
-                if (block < 0 || block >= p.num_blocks) {
-                    atomicCAS(p.status, 0, DEV_BAD_CACHE_BLOCK);
-                    return -1;
-                }
-                return block;
+                return t < s.tile1 && tok < s.hi && tok + 16 > s.lo;
+            };
+            auto read_block = [&](int t) -> int {
+                return wanted(t) ? table[(t * kManyTokens + (lane & 7) * 16) >> p.block_shift] : -1;
+            };
+            auto check_block = [&](int t, int block) -> int {
+                if (block >= 0 && block < p.num_blocks) return block;
+                if (wanted(t)) atomicCAS(p.status, 0, DEV_BAD_CACHE_BLOCK);
+                return -1;
             };
             auto scale_of = [&](const float* scales, int block) -> float {
                 return block >= 0 ? scales[(long long)block * p.scale_stride + s.head] : 0.0f;
             };
-            auto load = [&](const uint8_t* base, int t, int blocks, uint4 (&w)[kPasses]) {
+            // copies this thread's pieces of tile t into its staging slots; of blocks that do not exist, zeros
+            auto fetch = [&](int which, int t, int block) {
+                const uint8_t* base = (which ? cache.v : cache.k) + mine;
+                const long long at = block < 0 ? -1
+                    : block * cache.block_stride + ((t * kManyTokens + (lane & 7) * 16) & (cache.block_size - 1)) * cache.token_stride;
+                if (t < s.tile1) {
 #pragma unroll
-                for (int j = 0; j < kPasses; ++j) {
-                    const int row = j * kPassRows + r0, tok = t * kManyTokens + row;
-                    const int block = __shfl_sync(0xffffffffu, blocks, row >> 4);
-                    w[j] = make_uint4(0, 0, 0, 0);
-                    if (block >= 0 && tok >= s.lo && tok < s.hi)
-                        w[j] = *reinterpret_cast<const uint4*>(base + block * cache.block_stride +
-                                                               (long long)(tok & (cache.block_size - 1)) * cache.token_stride);
-                }
-            };
-            auto store = [&](uint8_t* tile, const uint4 (&w)[kPasses]) {
-#pragma unroll
-                for (int j = 0; j < kPasses; ++j) {
-                    const int row = j * kPassRows + r0;
-                    uint8_t* at = tile + (ch >> 2) * 16384 + row * 128;
-                    uint4 a, b;
-                    codes_to_half(w[j], a, b);
-                    // the two 16-byte halves in an order that keeps the eight lanes of a row on different banks
-                    const int c0 = (ch & 3) * 2, flip = (ch >> 2) & 1;
-                    const uint4 first = flip ? b : a, second = flip ? a : b;
-                    *reinterpret_cast<uint4*>(at + (((c0 + flip) ^ (row & 7)) << 4)) = first;
-                    *reinterpret_cast<uint4*>(at + (((c0 + 1 - flip) ^ (row & 7)) << 4)) = second;
-                }
-            };
-            int blk = block_of(s.tile0), blk2 = block_of(s.tile0 + 1);
-            float ks = scale_of(p.k_scale, blk), vs = scale_of(p.v_scale, blk);
-            uint4 kw[kPasses], vw[kPasses];
-            load(kc, s.tile0, blk, kw);
-
-            // ---- queries of the 256 rows: as half, bf16 rows scaled by a power of two
-            if (n_piece > 0) {
-                ok = mbar_wait(q_free, (n_piece - 1) & 1, abort_flag, p.status, DEV_TIMEOUT_SMEM_EMPTY);
-                ok = __all_sync(0xffffffffu, ok);
-                if (!ok) break;
-            }
-            {
-                constexpr int kLanes = kDim / 8;              // lanes of a row, 16 bytes each
-                constexpr int kRowsPer = 32 / kLanes;
-                constexpr int kBatch = 8;
-                const int sub = lane / kLanes, col = (lane % kLanes) * 8;
-                const float sign = p.scale_log2 < 0.0f ? -1.0f : 1.0f;
-                for (int base = (warp - 8) * 64; base < (warp - 8) * 64 + 64; base += kRowsPer * kBatch) {
-                    uint4 w[kBatch];
-#pragma unroll
-                    for (int j = 0; j < kBatch; ++j) {
-                        const int row = s.row0 + base + j * kRowsPer + sub;
-                        w[j] = make_uint4(0, 0, 0, 0);
-                        if (row < s.rows) {
-                            const int i = row / p.group;
-                            const int head = s.head * p.group + row - i * p.group;
-                            w[j] = *reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(p.q) +
-                                                                   (long long)(s.req.q0 + i) * p.q_token_stride +
-                                                                   (long long)head * p.q_head_stride + col);
-                        }
+                    for (int j = 0; j < kPasses; ++j) {
+                        const long long from = __shfl_sync(0xffffffffu, at, (j * kPassRows + r0) >> 4);
+                        cp_async16(raw + which * L::kRawBytes + j * 2048, base + (from < 0 ? 0 : from), from < 0 ? 0 : 16);
                     }
+                }
+                cp_async_commit();
+            };
+            // expands the pieces of tile t
+            auto expand = [&](int which, int t, bool edge) -> bool {
+                uint4 w[kPasses];
 #pragma unroll
-                    for (int j = 0; j < kBatch; ++j) {
-                        const int rit = base + j * kRowsPer + sub;
-                        uint32_t* e = &w[j].x;
-                        int shift = 0;
-                        if constexpr (kBf16) {
-                            uint32_t mag = 0;
+                for (int j = 0; j < kPasses; ++j) w[j] = *reinterpret_cast<const uint4*>(raw + which * L::kRawBytes + j * 2048);
+                bool any = false;
+                if (edge) {
+                    // zeros in place of tokens that no row sees and, of V, of NaN codes
+#pragma unroll
+                    for (int j = 0; j < kPasses; ++j) {
+                        const int tok = t * kManyTokens + j * kPassRows + r0;
+                        if (tok < s.lo || tok >= s.hi) w[j] = make_uint4(0, 0, 0, 0);
+                        if (which == 1) {
+                            uint32_t* e = &w[j].x;
 #pragma unroll
                             for (int h = 0; h < 4; ++h) {
-                                const uint32_t a = e[h] & 0x7FFFu, b = (e[h] >> 16) & 0x7FFFu;
-                                mag = max(mag, max(a < 0x7F80u ? a : 0u, b < 0x7F80u ? b : 0u));
+                                const uint32_t nb = __vcmpeq4(e[h] & 0x7F7F7F7Fu, 0x7F7F7F7Fu);
+                                any |= nb != 0;
+                                e[h] &= ~nb;
                             }
-#pragma unroll
-                            for (int o = 1; o < kLanes; o <<= 1) mag = max(mag, __shfl_xor_sync(0xffffffffu, mag, o));
-                            shift = query_shift(__uint_as_float(mag << 16));
-                            const float mul = pow2i(shift) * sign;
-#pragma unroll
-                            for (int h = 0; h < 4; ++h)
-                                e[h] = pack_f16(__uint_as_float(e[h] << 16) * mul, __uint_as_float(e[h] & 0xFFFF0000u) * mul);
-                        } else if (sign < 0.0f) {
-#pragma unroll
-                            for (int h = 0; h < 4; ++h) e[h] ^= 0x80008000u;
                         }
-                        uint8_t* at = smem + L::kQOffset + (rit >> 7) * L::kOperandBytes + (col >> 6) * 16384 + (rit & 127) * 128;
-                        *reinterpret_cast<uint4*>(at + ((((col & 63) >> 3) ^ (rit & 7)) << 4)) = w[j];
-                        if (lane % kLanes == 0) row_factor[rit] = pow2i(-shift);
                     }
                 }
-            }
-            fence_proxy_async();
-            __syncwarp();
-            if (lane == 0) mbar_arrive(q_full);
-
-            load(vc, s.tile0, blk, vw);
-            for (int t = s.tile0; t < s.tile1; ++t, ++n_tile) {
-                const int st = n_tile & 1;
-                const uint32_t ph = (n_tile >> 1) & 1;
-                const bool partial = all.masked(t);
-                // the scales of this tile (read before: block numbers two tiles ahead, scales and codes one)
-                if (warp == 8 && lane < 8) {
-                    const float lv = fmaxf(lg2(vs), kMinLogScale);
-                    // (the scores' factor is not negative: the sign of `scale` went into the queries)
-                    meta[(n_tile % kManyMeta) * 8 + lane] =
-                        make_float4(ks * fabsf(p.scale_log2), blk >= 0 ? lv : -INFINITY, ex2(-lv), 0.0f);
+                ok = attn_wait(&free_[ring], ring_phase, abort_flag, p.status, DEV_TIMEOUT_SMEM_EMPTY);
+                if (!ok) return false;
+                uint8_t* tile = smem + L::kRingOffset + ring * L::kOperandBytes;
+#pragma unroll
+                for (int j = 0; j < kPasses; ++j) {
+                    uint4 a, b;
+                    codes_to_half(w[j], a, b);
+                    *reinterpret_cast<uint4*>(tile + to_a + j * kPassRows * 128) = flip ? b : a;
+                    *reinterpret_cast<uint4*>(tile + to_b + j * kPassRows * 128) = flip ? a : b;
                 }
+                if (any) nan_tile[n_tile & 7] = n_tile + 1;
+                fence_proxy_async();
+                return true;
+            };
+            int blk = check_block(s.tile0, read_block(s.tile0)), raw_block = read_block(s.tile0 + 1);
+            fetch(0, s.tile0, blk);
+            fetch(1, s.tile0, blk);
+            float ks = scale_of(p.k_scale, blk), vs = scale_of(p.v_scale, blk);
+            for (int t = s.tile0; t < s.tile1; ++t, ++n_tile) {
                 if (warp == 8) {
+                    if (lane < 8) {
+                        const float lv = fmaxf(lg2(vs), kMinLogScale);
+                        // (the scores' factor is not negative: the sign of `scale` went into the queries)
+                        meta[(n_tile % kManyMeta) * 8 + lane] =
+                            make_float4(ks * fabsf(p.scale_log2), blk >= 0 ? lv : -INFINITY, ex2(-lv), 0.0f);
+                    }
                     __syncwarp();
                     if (lane == 0) mbar_arrive(&meta_full[n_tile % kManyMeta]);
                 }
-                blk = blk2;
-                blk2 = block_of(t + 2);
+                blk = check_block(t + 1, raw_block);
+                raw_block = read_block(t + 2);
                 ks = scale_of(p.k_scale, blk);
                 vs = scale_of(p.v_scale, blk);
-                ok = mbar_wait(&k_free[st], ph ^ 1, abort_flag, p.status, DEV_TIMEOUT_SMEM_EMPTY);
-                ok = __all_sync(0xffffffffu, ok);
-                if (!ok) break;
-                store(smem + L::kKOffset + st * L::kOperandBytes, kw);
-                fence_proxy_async();
-                __syncwarp();
-                if (lane == 0) mbar_arrive(&k_full[st]);
-                if (t + 1 < s.tile1) load(kc, t + 1, blk, kw);
-                if (partial) {
-                    bool any = false;
-#pragma unroll
-                    for (int j = 0; j < kPasses; ++j) {
-                        uint32_t* w = &vw[j].x;
-#pragma unroll
-                        for (int h = 0; h < 4; ++h) {
-                            const uint32_t nb = __vcmpeq4(w[h] & 0x7F7F7F7Fu, 0x7F7F7F7Fu);
-                            any |= nb != 0;
-                            w[h] &= ~nb;
-                        }
-                    }
-                    if (any) nan_piece[n_piece & 1] = n_piece + 1;
+                const bool edge = all.masked(t);
+#pragma unroll 1
+                for (int which = 0; which < 2; ++which) {
+                    cp_async_wait<1>();
+                    if (!expand(which, t, edge)) break;
+                    fetch(which, t + 1, blk);
+                    __syncwarp();
+                    if (lane == 0) mbar_arrive(&full[ring]);
+                    if (++ring == 3) { ring = 0; ring_phase ^= 1; }
                 }
-                ok = mbar_wait(&v_free[st], ph ^ 1, abort_flag, p.status, DEV_TIMEOUT_SMEM_EMPTY);
-                ok = __all_sync(0xffffffffu, ok);
                 if (!ok) break;
-                store(smem + L::kVOffset + st * L::kOperandBytes, vw);
-                fence_proxy_async();
-                __syncwarp();
-                if (lane == 0) mbar_arrive(&v_full[st]);
-                if (t + 1 < s.tile1) load(vc, t + 1, blk, vw);
             }
         }
+        cp_async_wait<0>();
     } else {
         // ------------------------------------------------------------------ MMA issue
         constexpr uint32_t idesc_qk = umma_idesc_half(128, false);
         constexpr uint32_t idesc_pv = umma_idesc_half(kDim, true);
-        const uint32_t q_addr = smem_u32(smem + L::kQOffset), k_addr = smem_u32(smem + L::kKOffset), v_addr = smem_u32(smem + L::kVOffset);
-        int n_piece = 0, n_tile = 0, n_mine[2] = {0, 0};
+        const uint32_t q_addr = smem_u32(smem + L::kQOffset), ring_addr = smem_u32(smem + L::kRingOffset);
+        int n_piece = 0;
+        uint32_t n_mine = 0;                                  // bit x: parity of the scores asked for of sub-tile x
+        int ring_k = 0, ring_v = 1;                           // places of the next K and the next V tile, in turn in the ring
+        uint32_t phase_k = 0, phase_v = 0;
+        auto advance = [](int& at, uint32_t& phase) {
+            at += 2;
+            if (at >= 3) { at -= 3; phase ^= 1; }
+        };
         for (int u = begin; u < end && ok; ++n_piece) {
             const AttnPiece s = attn_piece<kManyRows, kManyTokens>(p, prefix, u, end);
             u += max(1, s.tile1 - s.tile0);
-            const SubTile sub[2] = {sub_tile(p, s, s.row0, s.row0 + 128), sub_tile(p, s, s.row0 + 128, s.row0 + 256)};
-            ok = mbar_wait(q_full, n_piece & 1, abort_flag, p.status, DEV_TIMEOUT_SMEM_FULL);
-            ok = __all_sync(0xffffffffu, ok);
+            const SubTile sub0 = sub_tile(p, s, s.row0, s.row0 + 128), sub1 = sub_tile(p, s, s.row0 + 128, s.row0 + 256);
+            ok = attn_wait(q_full, n_piece & 1, abort_flag, p.status, DEV_TIMEOUT_SMEM_FULL);
             if (!ok) break;
-            bool first[2] = {true, true}, pending[2] = {false, false};
+            uint32_t started = 0, pending = 0;                // bit x: sub-tile x has had a P V; its last scores have none yet
             for (int t = s.tile0; t <= s.tile1 && ok; ++t) {
-                const bool more = t < s.tile1;
-                const int st = n_tile & 1, pst = st ^ 1;       // stage of this tile, of the one before
-                if (more) {
-                    ok = mbar_wait(&k_full[st], (n_tile >> 1) & 1, abort_flag, p.status, DEV_TIMEOUT_SMEM_FULL);
-                    ok = __all_sync(0xffffffffu, ok);
+                const bool more = t < s.tile1, behind = t > s.tile0;
+                const uint32_t k_tile = ring_addr + ring_k * L::kOperandBytes, v_tile = ring_addr + ring_v * L::kOperandBytes;
+                const uint32_t active = more ? (sub0.active(t) ? 1u : 0u) | (sub1.active(t) ? 2u : 0u) : 0u;
+                if (behind) {
+                    ok = attn_wait(&full[ring_v], phase_v, abort_flag, p.status, DEV_TIMEOUT_SMEM_FULL);
                     if (!ok) break;
                 }
-                if (t > s.tile0) {
-                    ok = mbar_wait(&v_full[pst], ((n_tile - 1) >> 1) & 1, abort_flag, p.status, DEV_TIMEOUT_SMEM_FULL);
-                    ok = __all_sync(0xffffffffu, ok);
-                    if (!ok) break;
-                }
-#pragma unroll
+#pragma unroll 1
                 for (int x = 0; x < 2; ++x) {
-                    if (pending[x]) {
-                        ok = mbar_wait(&p_full[x], (n_mine[x] - 1) & 1, abort_flag, p.status, DEV_TIMEOUT_TMEM_EMPTY);
-                        ok = __all_sync(0xffffffffu, ok);
+                    const uint32_t ts = tmem + x * 128, to = tmem + 256 + x * kDim;
+                    if (pending >> x & 1) {
+                        ok = attn_wait(&p_full[x], ((n_mine >> x) & 1) ^ 1, abort_flag, p.status, DEV_TIMEOUT_TMEM_EMPTY);
                         if (!ok) break;
                         tcgen05_fence_after();
                         if (elect_one()) {
-                            const uint64_t b = umma_desc_sw128_mn(v_addr + pst * L::kOperandBytes, 16384);
+                            const uint64_t b = umma_desc_sw128_mn(v_tile, 16384);
 #pragma unroll
                             for (int k = 0; k < 8; ++k)        // 16 tokens a step: 2048 bytes of V, 8 columns of P
-                                umma_f16_ts(tmem_o[x], tmem_s[x] + 8 * k, b + 128 * k, idesc_pv, (k > 0 || !first[x]) ? 1u : 0u);
+                                umma_f16_ts(to, ts + 8 * k, b + 128 * k, idesc_pv, k > 0 ? 1u : started >> x & 1);
                             umma_commit(&pv_done[x]);
                         }
                         __syncwarp();
-                        first[x] = false;
-                        pending[x] = false;
+                        started |= 1u << x;
+                        pending &= ~(1u << x);
                     }
-                    if (more && sub[x].active(t)) {
-                        tcgen05_fence_after();
+                    if (x == 0) {
+                        if (more) {
+                            ok = attn_wait(&full[ring_k], phase_k, abort_flag, p.status, DEV_TIMEOUT_SMEM_FULL);
+                            if (!ok) break;
+                            tcgen05_fence_after();
+                        }
+                    } else if (behind) {
+                        if (elect_one()) umma_commit(&free_[ring_v]);
+                        __syncwarp();
+                    }
+                    if (active >> x & 1) {
                         if (elect_one()) {
                             const uint64_t a = umma_desc_sw128(q_addr + x * L::kOperandBytes);
-                            const uint64_t b = umma_desc_sw128(k_addr + st * L::kOperandBytes);
+                            const uint64_t b = umma_desc_sw128(k_tile);
 #pragma unroll
                             for (int k = 0; k < kDim / 16; ++k) {   // 16 dims a step: 32 bytes, 64 dims a half
                                 const uint64_t at = (uint64_t)((k >> 2) * (16384 >> 4) + (k & 3) * 2);
-                                umma_f16_ss(tmem_s[x], a + at, b + at, idesc_qk, k > 0 ? 1u : 0u);
+                                umma_f16_ss(ts, a + at, b + at, idesc_qk, k > 0 ? 1u : 0u);
                             }
                             umma_commit(&s_full[x]);
                         }
                         __syncwarp();
-                        pending[x] = true;
-                        ++n_mine[x];
+                        pending |= 1u << x;
+                        n_mine ^= 1u << x;
                     }
                 }
                 if (!ok) break;
                 if (elect_one()) {
-                    if (more) umma_commit(&k_free[st]);
-                    if (t > s.tile0) umma_commit(&v_free[pst]);
+                    if (more) umma_commit(&free_[ring_k]);
                     if (t == s.tile1 - 1 || s.tile0 == s.tile1) umma_commit(q_free);
                 }
                 __syncwarp();
-                if (more) ++n_tile;
+                if (behind) advance(ring_v, phase_v);
+                if (more) advance(ring_k, phase_k);
             }
         }
     }

@@ -46,6 +46,21 @@ struct CacheAttentionParams {
     int* status;
 };
 
+// A wait whose bounded loop is out of line: the roles of a kernel share the instruction cache, and a wait that has to
+// wait does not mind a call.
+static __device__ __noinline__ bool attn_wait_slow(uint32_t bar, uint32_t parity, volatile int* abort_flag, int* status, int code) {
+    return mbar_wait_addr(bar, parity, abort_flag, status, code);
+}
+__device__ __forceinline__ bool attn_wait(uint64_t* bar, uint32_t parity, volatile int* abort_flag, int* status, int code) {
+    bool ok = mbar_try_wait(bar, parity);
+    if (!__all_sync(0xffffffffu, ok)) {
+        ok = attn_wait_slow(smem_u32(bar), parity, abort_flag, status, code);
+        ok = __all_sync(0xffffffffu, ok);
+        return ok;
+    }
+    return true;
+}
+
 struct AttnRequest {
     int q0, qlen, kv;
 };
@@ -64,7 +79,7 @@ __device__ __forceinline__ AttnRequest attn_request(const CacheAttentionParams& 
 
 // Tokens [lo, hi) that the rows of row tile `qt` see between them.
 template <int kRows>
-__device__ __forceinline__ void attn_span(const CacheAttentionParams& p, const AttnRequest& q, int qt, int& lo, int& hi) {
+__device__ __noinline__ void attn_span(const CacheAttentionParams& p, const AttnRequest& q, int qt, int& lo, int& hi) {
     const int rows = q.qlen * p.group;
     const int i0 = (qt * kRows) / p.group;
     const int i1 = (min(rows, (qt + 1) * kRows) - 1) / p.group;
@@ -84,6 +99,7 @@ template <int kRows, int kTokens>
 __device__ __forceinline__ int attn_units_of_head(const CacheAttentionParams& p, const AttnRequest& q) {
     const int tiles = (q.qlen * p.group + kRows - 1) / kRows;
     int n = 0;
+#pragma unroll 1
     for (int t = 0; t < tiles; ++t) {
         int lo, hi;
         attn_span<kRows>(p, q, t, lo, hi);
@@ -97,6 +113,7 @@ template <int kRows, int kTokens>
 __device__ __forceinline__ void attn_prefix(const CacheAttentionParams& p, int* prefix, int* warp_sums) {
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, warps = blockDim.x >> 5;
     int carry = 0;
+#pragma unroll 1
     for (int base = 0; base < p.requests; base += blockDim.x) {
         const int r = base + threadIdx.x;
         int u = 0;
@@ -113,6 +130,7 @@ __device__ __forceinline__ void attn_prefix(const CacheAttentionParams& p, int* 
         if (lane == 31) warp_sums[warp] = inc;
         __syncthreads();
         int before = carry, total = carry;
+#pragma unroll 1
         for (int w = 0; w < warps; ++w) {
             const int s = warp_sums[w];
             if (w < warp) before += s;
@@ -141,9 +159,10 @@ struct AttnPiece {
 };
 
 template <int kRows, int kTokens>
-__device__ __forceinline__ AttnPiece attn_piece(const CacheAttentionParams& p, const int* prefix, int u, int end) {
+__device__ __noinline__ AttnPiece attn_piece(const CacheAttentionParams& p, const int* prefix, int u, int end) {
     AttnPiece s;
     int a = 0, b = p.requests;
+#pragma unroll 1
     while (b - a > 1) {
         const int mid = (a + b) >> 1;
         if (prefix[mid] <= u) a = mid; else b = mid;
@@ -156,6 +175,7 @@ __device__ __forceinline__ AttnPiece attn_piece(const CacheAttentionParams& p, c
     s.head = local / per_head;
     int rem = local - s.head * per_head;
     int qt = 0, n;
+#pragma unroll 1
     for (;;) {
         attn_span<kRows>(p, s.req, qt, s.lo, s.hi);
         n = attn_units<kTokens>(s.lo, s.hi);

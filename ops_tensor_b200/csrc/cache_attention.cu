@@ -128,7 +128,7 @@ cache_attention_few_kernel(const __grid_constant__ CUtensorMap map_k, const __gr
         uint32_t phase = 0;
         bool ok = true;
         for (int u = begin; u < end && ok;) {
-            const AttnPiece s = attn_piece<kFewRows, kFewTokens>(p, prefix, u, end);
+            const AttnPiece s = attn_piece_at<kFewRows, kFewTokens>(p, prefix, u, end);
             u += max(1, s.tile1 - s.tile0);
             const int* table = p.table + (long long)s.r * p.table_stride;
             // Lane i holds page `base + i` of the request: block number and scales, fetched 32 pages at a time and one
@@ -200,7 +200,7 @@ cache_attention_few_kernel(const __grid_constant__ CUtensorMap map_k, const __gr
         uint32_t phase = 0;
         bool ok = true;
         for (int u = begin; u < end && ok;) {
-            const AttnPiece s = attn_piece<kFewRows, kFewTokens>(p, prefix, u, end);
+            const AttnPiece s = attn_piece_at<kFewRows, kFewTokens>(p, prefix, u, end);
             const int u_next = u + max(1, s.tile1 - s.tile0);
             // ---- queries of this lane's two rows, as half
             uint32_t qf[kSteps][4];
@@ -535,7 +535,7 @@ __global__ void __launch_bounds__(256) cache_attention_join_kernel(const CacheAt
     const int which = blockIdx.x / kGroups, group = blockIdx.x % kGroups;
     const long long border = (long long)(which + 1) * chunk;
     if (border >= total) return;
-    const AttnPiece s = attn_piece<kRows, kTokens>(p, join_prefix, (int)border, total);
+    const AttnPiece s = attn_piece_at<kRows, kTokens>(p, join_prefix, (int)border, total);
     if (s.item0 == (int)border) return;                            // nothing is cut here
     const int first = s.item0 / chunk, last = (s.item1 - 1) / chunk;
     if (first != which) return;                                     // the item's first border belongs to another block

@@ -79,7 +79,7 @@ __device__ __forceinline__ AttnRequest attn_request(const CacheAttentionParams& 
 
 // Tokens [lo, hi) that the rows of row tile `qt` see between them.
 template <int kRows>
-__device__ __noinline__ void attn_span(const CacheAttentionParams& p, const AttnRequest& q, int qt, int& lo, int& hi) {
+__device__ __forceinline__ void attn_span(const CacheAttentionParams& p, const AttnRequest& q, int qt, int& lo, int& hi) {
     const int rows = q.qlen * p.group;
     const int i0 = (qt * kRows) / p.group;
     const int i1 = (min(rows, (qt + 1) * kRows) - 1) / p.group;
@@ -94,18 +94,12 @@ __device__ __forceinline__ int attn_units(int lo, int hi) {
     return hi <= lo ? 1 : (hi + kTokens - 1) / kTokens - lo / kTokens;
 }
 
-// Units of one kv head of request q.
+// Units of row tile t.
 template <int kRows, int kTokens>
-__device__ __forceinline__ int attn_units_of_head(const CacheAttentionParams& p, const AttnRequest& q) {
-    const int tiles = (q.qlen * p.group + kRows - 1) / kRows;
-    int n = 0;
-#pragma unroll 1
-    for (int t = 0; t < tiles; ++t) {
-        int lo, hi;
-        attn_span<kRows>(p, q, t, lo, hi);
-        n += attn_units<kTokens>(lo, hi);
-    }
-    return n;
+__device__ __forceinline__ int attn_units_of_tile(const CacheAttentionParams& p, const AttnRequest& q, int t) {
+    int lo, hi;
+    attn_span<kRows>(p, q, t, lo, hi);
+    return attn_units<kTokens>(lo, hi);
 }
 
 // prefix[r] = units before request r, prefix[requests] = all of them.  Called by the whole block.
@@ -116,11 +110,27 @@ __device__ __forceinline__ void attn_prefix(const CacheAttentionParams& p, int* 
 #pragma unroll 1
     for (int base = 0; base < p.requests; base += blockDim.x) {
         const int r = base + threadIdx.x;
-        int u = 0;
-        if (r < p.requests) {
-            const AttnRequest q = attn_request(p, r);
-            if (q.qlen > 0) u = p.kv_heads * attn_units_of_head<kRows, kTokens>(p, q);
+        AttnRequest q = {0, 0, 0};
+        if (r < p.requests) q = attn_request(p, r);
+        const int tiles = (q.qlen * p.group + kRows - 1) / kRows;
+        int u = tiles > 0 ? attn_units_of_tile<kRows, kTokens>(p, q, 0) : 0;
+        // requests of many row tiles: the warp's lanes share them
+        uint32_t many = __ballot_sync(0xffffffffu, tiles > 1);
+        while (many) {
+            const int src = __ffs(many) - 1;
+            many &= many - 1;
+            AttnRequest o;
+            o.q0 = 0;
+            o.qlen = __shfl_sync(0xffffffffu, q.qlen, src);
+            o.kv = __shfl_sync(0xffffffffu, q.kv, src);
+            const int n = __shfl_sync(0xffffffffu, tiles, src);
+            int sum = 0;
+#pragma unroll 1
+            for (int t = lane; t < n; t += 32) sum += attn_units_of_tile<kRows, kTokens>(p, o, t);
+            sum = __reduce_add_sync(0xffffffffu, sum);
+            if (lane == src) u = sum;
         }
+        u *= p.kv_heads;
         int inc = u;
 #pragma unroll
         for (int o = 1; o < 32; o <<= 1) {
@@ -149,7 +159,7 @@ __device__ __forceinline__ int attn_chunk(const CacheAttentionParams& p, int tot
     return max((total + blocks - 1) / blocks, p.min_chunk);
 }
 
-// The piece of an item that starts at unit u and ends at the item's end or at unit `end`.
+// The piece of an item that starts at unit u and ends at the item's end or at unit `end`; called by whole warps.
 struct AttnPiece {
     AttnRequest req;
     int r, head, row0, rows;          // first packed row of the tile, packed rows of the request
@@ -159,7 +169,7 @@ struct AttnPiece {
 };
 
 template <int kRows, int kTokens>
-__device__ __noinline__ AttnPiece attn_piece(const CacheAttentionParams& p, const int* prefix, int u, int end) {
+__device__ __forceinline__ AttnPiece attn_piece_at(const CacheAttentionParams& p, const int* prefix, int u, int end) {
     AttnPiece s;
     int a = 0, b = p.requests;
 #pragma unroll 1
@@ -174,15 +184,31 @@ __device__ __noinline__ AttnPiece attn_piece(const CacheAttentionParams& p, cons
     const int local = u - prefix[a];
     s.head = local / per_head;
     int rem = local - s.head * per_head;
-    int qt = 0, n;
+    int qt = 0;
+    if (s.rows > kRows) {
+        // the row tile that unit `rem` of the head lies in: the warp's lanes sum the tiles' units 32 at a time
+        const int lane = threadIdx.x & 31, tiles = (s.rows + kRows - 1) / kRows;
 #pragma unroll 1
-    for (;;) {
-        attn_span<kRows>(p, s.req, qt, s.lo, s.hi);
-        n = attn_units<kTokens>(s.lo, s.hi);
-        if (rem < n) break;
-        rem -= n;
-        ++qt;
+        for (;; qt += 32) {
+            const int n = qt + lane < tiles ? attn_units_of_tile<kRows, kTokens>(p, s.req, qt + lane) : 0x3FFFFFFF;
+            int inc = min(n, 0x3FFFFFFF);
+#pragma unroll
+            for (int o = 1; o < 32; o <<= 1) {
+                const int y = __shfl_up_sync(0xffffffffu, inc, o);
+                if (lane >= o) inc = min(inc + y, 0x3FFFFFFF);
+            }
+            const uint32_t beyond = __ballot_sync(0xffffffffu, inc > rem);
+            if (beyond) {
+                const int at = __ffs(beyond) - 1;
+                if (at > 0) rem -= __shfl_sync(0xffffffffu, inc, at - 1);
+                qt += at;
+                break;
+            }
+            rem -= __shfl_sync(0xffffffffu, inc, 31);
+        }
     }
+    attn_span<kRows>(p, s.req, qt, s.lo, s.hi);
+    const int n = attn_units<kTokens>(s.lo, s.hi);
     s.row0 = qt * kRows;
     s.item0 = u - rem;
     s.item1 = s.item0 + n;
@@ -190,6 +216,11 @@ __device__ __noinline__ AttnPiece attn_piece(const CacheAttentionParams& p, cons
     s.tile0 = s.lo / kTokens + rem;
     s.tile1 = s.hi <= s.lo ? s.tile0 : s.tile0 + take;
     return s;
+}
+// The same out of line, for a kernel whose roles share the instruction cache.
+template <int kRows, int kTokens>
+__device__ __noinline__ AttnPiece attn_piece(const CacheAttentionParams& p, const int* prefix, int u, int end) {
+    return attn_piece_at<kRows, kTokens>(p, prefix, u, end);
 }
 
 __device__ __forceinline__ float ex2(float x) {

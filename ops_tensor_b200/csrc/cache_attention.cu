@@ -117,6 +117,7 @@ cache_attention_few_kernel(const __grid_constant__ CUtensorMap map_k, const __gr
     const long long begin64 = (long long)blockIdx.x * chunk;
     const int begin = (int)min(begin64, (long long)total);
     const int end = (int)min(begin64 + chunk, (long long)total);
+    if (threadIdx.x == 0 && begin >= end) p.cuts[blockIdx.x].first = -1;
 
     if (warp == kFewWarps) {
         // ------------------------------------------------------------------ fetching warp
@@ -508,6 +509,7 @@ cache_attention_few_kernel(const __grid_constant__ CUtensorMap map_k, const __gr
                     }
                 }
             }
+            if (threadIdx.x == 0 && u_next >= end) attn_write_cut(p, s, blockIdx.x, chunk, end);
             compute_sync();
             u = u_next;
         }
@@ -520,59 +522,77 @@ cache_attention_few_kernel(const __grid_constant__ CUtensorMap map_k, const __gr
     }
 }
 
-// Joins the pieces of the items that are cut by a chunk's border.  Block b takes the item that holds border (b + 1) *
-// chunk, unless an earlier border is in it too; a row tile is shared by kGroups blocks, whose warps take rows.
-template <int kRows, int kTokens, int kDim, bool kBf16>
-__global__ void __launch_bounds__(256) cache_attention_join_kernel(const CacheAttentionParams p, int blocks) {
+// Joins the pieces of the items that are cut by a chunk's border: out = sum_b w_b O_b / sum_b w_b l_b with w_b = 2^(m_b -
+// max m), in the order of the blocks.  Block `which` takes the item that the end of that block's chunk cuts, unless the
+// item was cut before; a row tile is shared by kRows / 16 blocks, whose warps take rows.  Bound by latency: the
+// statistics of 32 pieces are read at once by a warp's lanes, then four pieces of output are in flight.
+template <int kRows, int kDim, bool kBf16>
+__global__ void __launch_bounds__(256) cache_attention_join_kernel(const CacheAttentionParams p) {
     constexpr int kGroups = kRows / 16;
-    extern __shared__ int join_prefix[];
-    __shared__ int warp_sums[8];
+    constexpr int kPer = kDim / 32;
     grid_launch_dependents();
     grid_dependency_wait();
-    attn_prefix<kRows, kTokens>(p, join_prefix, warp_sums);
-    const int total = join_prefix[p.requests];
-    const int chunk = attn_chunk(p, total, blocks);
     const int which = blockIdx.x / kGroups, group = blockIdx.x % kGroups;
-    const long long border = (long long)(which + 1) * chunk;
-    if (border >= total) return;
-    const AttnPiece s = attn_piece_at<kRows, kTokens>(p, join_prefix, (int)border, total);
-    if (s.item0 == (int)border) return;                            // nothing is cut here
-    const int first = s.item0 / chunk, last = (s.item1 - 1) / chunk;
-    if (first != which) return;                                     // the item's first border belongs to another block
+    const AttnCut s = p.cuts[which];
+    if (s.first != which) return;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    constexpr int kPer = kDim / 32;
     const int rows = min((group + 1) * 16, s.rows - s.row0);
+    const int pieces = s.last - s.first + 1;
+    // slot 0 of a block is the piece at the start of its chunk, slot 1 one that starts inside it
+    auto slot_of = [&](int b) -> long long { return (long long)(s.first + b) * 2 + (b == 0 ? s.inside : 0); };
     for (int row = group * 16 + warp; row < rows; row += 8) {
         float mm = -INFINITY, ll = 0.0f, acc[kPer];
 #pragma unroll
         for (int k = 0; k < kPer; ++k) acc[k] = 0.0f;
-        for (int b = first; b <= last; ++b) {
-            // the piece that starts its block's chunk is in slot 0, one that starts inside it in slot 1
-            const long long slot = (long long)b * 2 + (b == first && s.item0 != b * chunk ? 1 : 0);
-            const float2 v = *reinterpret_cast<const float2*>(p.part_ml + (slot * kRows + row) * 2);
-            if (v.x == -INFINITY) {
-                if (v.y != v.y) ll = v.y;
-                continue;
-            }
-            const float m_new = fmaxf(mm, v.x);
-            const float keep = mm == -INFINITY ? (ll != ll ? 1.0f : 0.0f) : ex2(mm - m_new), add = ex2(v.x - m_new);
-            mm = m_new;
-            ll = ll * keep + v.y * add;
-            const float* src = p.part_out + (slot * kRows + row) * kDim + lane * kPer;
+#pragma unroll 1
+        for (int b0 = 0; b0 < pieces; b0 += 32) {
+            float2 v = make_float2(-INFINITY, 0.0f);
+            if (b0 + lane < pieces) v = *reinterpret_cast<const float2*>(p.part_ml + (slot_of(b0 + lane) * kRows + row) * 2);
+            float m_new = v.x;
 #pragma unroll
-            for (int k = 0; k < kPer; ++k) acc[k] = acc[k] * keep + src[k] * add;
+            for (int o = 1; o < 32; o <<= 1) m_new = fmaxf(m_new, __shfl_xor_sync(0xffffffffu, m_new, o));
+            m_new = fmaxf(m_new, mm);
+            // (a piece that saw nothing has weight 0, but its sum may be the NaN of a score)
+            const float w = v.x == -INFINITY ? 0.0f : ex2(v.x - m_new);
+            const float keep = mm == -INFINITY ? 0.0f : ex2(mm - m_new);
+            mm = m_new;
+            float sum = w * v.y;
+#pragma unroll
+            for (int o = 1; o < 32; o <<= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+            ll = ll * keep + sum;
+#pragma unroll
+            for (int k = 0; k < kPer; ++k) acc[k] *= keep;
+            const int n = min(32, pieces - b0);
+#pragma unroll 1
+            for (int b = 0; b < n; b += 4) {
+                float x[4][kPer];
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                    const float* src = p.part_out + (slot_of(b0 + min(b + j, n - 1)) * kRows + row) * kDim + lane * kPer;
+#pragma unroll
+                    for (int k = 0; k < kPer; ++k) x[j][k] = src[k];
+                }
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                    const float wj = __shfl_sync(0xffffffffu, w, (b + j) & 31);
+                    if (b + j < n && wj != 0.0f) {
+#pragma unroll
+                        for (int k = 0; k < kPer; ++k) acc[k] = fmaf(wj, x[j][k], acc[k]);
+                    }
+                }
+            }
         }
         const int prow = s.row0 + row;
         const int i = prow / p.group;
         const int head = s.head * p.group + (prow - i * p.group);
         const float inv = ll != 0.0f ? 1.0f / ll : 0.0f;
-        uint16_t* dst = static_cast<uint16_t*>(p.out) + (long long)(s.req.q0 + i) * p.out_token_stride +
+        uint16_t* dst = static_cast<uint16_t*>(p.out) + (long long)(s.q0 + i) * p.out_token_stride +
                         (long long)head * p.out_head_stride + lane * kPer;
 #pragma unroll
         for (int k = 0; k < kPer; k += 2)
             *reinterpret_cast<uint32_t*>(dst + k) = pack_out<kBf16>(acc[k] * inv, acc[k + 1] * inv);
         if (p.lse && lane == 0)
-            p.lse[(long long)(s.req.q0 + i) * p.heads + head] =
+            p.lse[(long long)(s.q0 + i) * p.heads + head] =
                 ll != 0.0f ? (mm + lg2(ll)) * 0.6931471805599453f : -INFINITY;
     }
 }
@@ -606,7 +626,7 @@ static int status_of(cudaError_t e) {
 struct AttnPlan {
     bool few, many;
     int few_grid, many_grid;
-    size_t few_ml, many_out, many_ml, total;           // offsets in the workspace (few_out is 0)
+    size_t few_ml, few_cuts, many_out, many_ml, many_cuts, total;      // offsets in the workspace (few_out is 0)
 };
 
 static size_t round256(size_t x) { return (x + 255) & ~size_t(255); }
@@ -635,15 +655,17 @@ static int plan_attention(const blazeKvCache* c, const blazeCacheAttentionArgs* 
     pl->few_grid = 2 * sms;
     pl->many_grid = sms;
     size_t at = 0;
-    auto room = [&](int grid, int tile_rows, size_t* ml) {
+    auto room = [&](int grid, int tile_rows, size_t* ml, size_t* cuts) {
         at += round256((size_t)grid * 2 * tile_rows * c->head_dim * 4);
         *ml = at;
         at += round256((size_t)grid * 2 * tile_rows * 2 * 4);
+        *cuts = at;
+        at += round256((size_t)grid * sizeof(AttnCut));
     };
-    pl->few_ml = pl->many_out = pl->many_ml = 0;
-    if (pl->few) room(pl->few_grid, kFewRows, &pl->few_ml);
+    pl->few_ml = pl->few_cuts = pl->many_out = pl->many_ml = pl->many_cuts = 0;
+    if (pl->few) room(pl->few_grid, kFewRows, &pl->few_ml, &pl->few_cuts);
     pl->many_out = at;
-    if (pl->many) room(pl->many_grid, kManyRows, &pl->many_ml);
+    if (pl->many) room(pl->many_grid, kManyRows, &pl->many_ml, &pl->many_cuts);
     pl->total = at;
     return ACLTENSOR_STATUS_SUCCESS;
 }
@@ -667,7 +689,6 @@ static cudaError_t launch_attention(const CUtensorMap& mk, const CUtensorMap& mv
         if (e != cudaSuccess) return e;
         done[dev & 63] = true;
     }
-    const size_t join_smem = (size_t)(p.requests + 1) * 4;
     cudaError_t e = cudaSuccess;
     p.few_rows = kFewLimit;
     if (pl.few) {
@@ -676,10 +697,10 @@ static cudaError_t launch_attention(const CUtensorMap& mk, const CUtensorMap& mv
         p.min_chunk = kFewMinChunk;
         p.part_out = reinterpret_cast<float*>(ws);
         p.part_ml = reinterpret_cast<float*>(ws + pl.few_ml);
+        p.cuts = reinterpret_cast<AttnCut*>(ws + pl.few_cuts);
         e = launch_after_prepass(few, pl.few_grid, kFewThreads, (size_t)FewSmem<kDim>::bytes(p.requests), stream, mk, mv, p);
         if (e == cudaSuccess && pl.few_grid > 1)
-            e = launch_after_prepass(cache_attention_join_kernel<kFewRows, kFewTokens, kDim, kBf16>, pl.few_grid - 1, 256,
-                                     join_smem, stream, p, pl.few_grid);
+            e = launch_after_prepass(cache_attention_join_kernel<kFewRows, kDim, kBf16>, pl.few_grid - 1, 256, 0, stream, p);
         if (e != cudaSuccess) return e;
     }
     if (pl.many) {
@@ -688,10 +709,11 @@ static cudaError_t launch_attention(const CUtensorMap& mk, const CUtensorMap& mv
         p.min_chunk = kManyMinChunk;
         p.part_out = reinterpret_cast<float*>(ws + pl.many_out);
         p.part_ml = reinterpret_cast<float*>(ws + pl.many_ml);
+        p.cuts = reinterpret_cast<AttnCut*>(ws + pl.many_cuts);
         e = launch_after_prepass(many, pl.many_grid, kManyThreads, (size_t)ManySmem<kDim>::bytes(p.requests), stream, p, cv);
         if (e == cudaSuccess && pl.many_grid > 1)
-            e = launch_after_prepass(cache_attention_join_kernel<kManyRows, kManyTokens, kDim, kBf16>,
-                                     (pl.many_grid - 1) * (kManyRows / 16), 256, join_smem, stream, p, pl.many_grid);
+            e = launch_after_prepass(cache_attention_join_kernel<kManyRows, kDim, kBf16>,
+                                     (pl.many_grid - 1) * (kManyRows / 16), 256, 0, stream, p);
     }
     return e;
 }

@@ -200,6 +200,7 @@ cache_attention_many_kernel(const CacheAttentionParams p, const CacheView cache)
     const int begin = (int)min(begin64, (long long)total);
     const int end = (int)min(begin64 + chunk, (long long)total);
     bool ok = true;
+    if (threadIdx.x == 0 && begin >= end) p.cuts[blockIdx.x].first = -1;
 
     if (warp < 8) {
         // ------------------------------------------------------------------ softmax
@@ -462,6 +463,7 @@ cache_attention_many_kernel(const CacheAttentionParams p, const CacheView cache)
                     *reinterpret_cast<float2*>(p.part_ml + (slot * kManyRows + row_in_tile) * 2) = make_float2(m, l);
                 }
             }
+            if (threadIdx.x == 0 && u_next >= end) attn_write_cut(p, s, blockIdx.x, chunk, end);
             tcgen05_fence_before();                           // O has been read: the next piece may overwrite it
             __syncwarp();
             u = u_next;

@@ -20,6 +20,13 @@ namespace blaze {
 
 constexpr int kAttnMaxRequests = 8192;
 
+// What the joining kernel has to know of an item that lies in more than one chunk.
+struct AttnCut {
+    int first, last;                  // its first and last block; first = -1: nothing is cut here
+    int inside;                       // 1: its first piece starts inside the first block's chunk
+    int q0, head, row0, rows, pad;
+};
+
 struct CacheAttentionParams {
     int requests, tokens, heads, kv_heads, group, head_dim;
     int block_shift, num_blocks, max_blocks;
@@ -43,6 +50,7 @@ struct CacheAttentionParams {
     int min_chunk;                    // units per block, at least
     float* part_out;                  // [block][2][row tile][head_dim]
     float* part_ml;                   // [block][2][row tile][2]
+    struct AttnCut* cuts;             // [block]: the item that the end of the block's chunk cuts
     int* status;
 };
 
@@ -217,7 +225,21 @@ __device__ __forceinline__ AttnPiece attn_piece_at(const CacheAttentionParams& p
     s.tile1 = s.hi <= s.lo ? s.tile0 : s.tile0 + take;
     return s;
 }
-// The same out of line, for a kernel whose roles share the instruction cache.
+// The cut at the end of block `block`'s chunk, s being the chunk's last piece.
+__device__ __forceinline__ void attn_write_cut(const CacheAttentionParams& p, const AttnPiece& s, int block, int chunk, int end) {
+    AttnCut c;
+    c.first = s.item1 > end ? s.item0 / chunk : -1;
+    c.last = (s.item1 - 1) / chunk;
+    c.inside = s.item0 != c.first * chunk ? 1 : 0;
+    c.q0 = s.req.q0;
+    c.head = s.head;
+    c.row0 = s.row0;
+    c.rows = s.rows;
+    c.pad = 0;
+    p.cuts[block] = c;
+}
+
+// attn_piece_at out of line, for a kernel whose roles share the instruction cache.
 template <int kRows, int kTokens>
 __device__ __noinline__ AttnPiece attn_piece(const CacheAttentionParams& p, const int* prefix, int u, int end) {
     return attn_piece_at<kRows, kTokens>(p, prefix, u, end);

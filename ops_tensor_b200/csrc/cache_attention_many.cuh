@@ -21,11 +21,15 @@ namespace blaze {
 
 constexpr int kManyRows = 256;
 constexpr int kManyTokens = 128;
-constexpr int kManyThreads = 32 * 13;
+constexpr int kManyThreads = 32 * 16;      // warps 13-15 only complete the last warpgroup
+// Registers of a thread of the softmax, converting and issuing warpgroups (a softmax thread holds its row's 128 scores);
+// the launch has 128 each, 512 for the four.
+constexpr int kSoftmaxRegs = 184, kConvertRegs = 88, kIssueRegs = 56;
+static_assert(2 * kSoftmaxRegs + kConvertRegs + kIssueRegs <= 4 * 128, "setmaxnreg draws on what the launch has");
 constexpr int kManyMeta = 4;              // tiles whose scales are held
 
-// Largest of the exponents by which p may pass its reference: p <= 2^15.
-constexpr float kManyShift = 7.0f;
+// A row's reference is set 2^3 below its largest score and kept until a score passes it by 2^15 (half ends at 2^16).
+constexpr float kManyShift = 3.0f;
 constexpr float kManyGrow = 15.0f;
 
 template <int kDim>
@@ -91,12 +95,38 @@ __device__ __forceinline__ void tmem_st_32x32(uint32_t taddr, const uint32_t (&r
         "r"(r[28]), "r"(r[29]), "r"(r[30]), "r"(r[31])
         : "memory");
 }
+template <int kRegs>
+__device__ __forceinline__ void regs_inc() { asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kRegs)); }
+template <int kRegs>
+__device__ __forceinline__ void regs_dec() { asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kRegs)); }
+__device__ __forceinline__ void tmem_ld_32x16(uint32_t taddr, uint32_t (&r)[16]) {
+    asm volatile(
+        "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15}, [%16];"
+        : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]), "=r"(r[9]),
+          "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
+        : "r"(taddr)
+        : "memory");
+}
 __device__ __forceinline__ float max3(float a, float b, float c) {
     float d;
     asm("max.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
     return d;
 }
 __device__ __forceinline__ void tmem_st_wait() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
+
+// O of this warp's 32 rows times a factor per row.
+template <int kDim>
+__device__ __forceinline__ void rescale(uint32_t to, float al) {
+#pragma unroll 1
+    for (int c = 0; c < kDim / 16; ++c) {
+        uint32_t v[16];
+        tmem_ld_32x16(to + c * 16, v);
+        tmem_ld_wait();
+#pragma unroll
+        for (int k = 0; k < 16; ++k) v[k] = __float_as_uint(__uint_as_float(v[k]) * al);
+        tmem_st_32x16(to + c * 16, v);
+    }
+}
 
 // Tokens [lo, hi) that any row of the sub-tile of 128 rows at `row0` sees, and [all_lo, all_hi) that every row sees.
 struct SubTile {
@@ -108,7 +138,7 @@ struct SubTile {
         return t * kManyTokens < all_lo || (t + 1) * kManyTokens > all_hi;
     }
 };
-__device__ __noinline__ SubTile sub_tile(const CacheAttentionParams& p, const AttnPiece& s, int row0, int row1) {
+__device__ __forceinline__ SubTile sub_tile(const CacheAttentionParams& p, const AttnPiece& s, int row0, int row1) {
     SubTile x;
     const int end = min(s.rows, row1);
     if (row0 >= end) {
@@ -204,6 +234,7 @@ cache_attention_many_kernel(const CacheAttentionParams p, const CacheView cache)
 
     if (warp < 8) {
         // ------------------------------------------------------------------ softmax
+        regs_inc<kSoftmaxRegs>();
         const int x = warp >> 2;                              // sub-tile
         const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16;
         const uint32_t ts = tmem_s[x] + lanes, to = tmem_o[x] + lanes;
@@ -285,93 +316,30 @@ cache_attention_many_kernel(const CacheAttentionParams p, const CacheView cache)
                 const float4* mt = meta + (n_tile % kManyMeta) * 8;
                 const bool masked = sub.masked(t);
                 const int tok0 = t * kManyTokens;
-                // bits of the tokens [tok0 + 16 g, + 16) that this row sees
-                auto seen = [&](int g) -> uint32_t {
-                    const int at = tok0 + 16 * g;
-                    const int a = max(see_lo - at, 0), b = min(see_hi - at, 16);
-                    return b > a ? ((1u << b) - 1u) & ~((1u << a) - 1u) : 0u;
+                float ms = 0.0f;
+                // A new reference, only where a score has outgrown the old one by 2^15 (and in a piece's first tile).
+                auto refer = [&](float mx) {
+                    const bool grow = mx > m + kManyGrow;
+                    if (__any_sync(0xffffffffu, grow)) {
+                        const float m_new = grow ? mx - kManyShift : m;
+                        const float al = grow ? (m == -INFINITY ? 0.0f : ex2(m - m_new)) : 1.0f;
+                        m = m_new;
+                        l *= al;
+                        if (done > 0) {
+                            ok = attn_wait(&pv_done[x], (n_mine - 1) & 1, abort_flag, p.status, DEV_TIMEOUT_TMEM_FULL);
+                            tcgen05_fence_after();
+                            rescale<kDim>(to, al);
+                        }
+                    }
+                    ms = m == -INFINITY ? 0.0f : m;
                 };
-                // ---- the row's largest exponent.  (Blocks that do not exist have codes of zero and an exponent of -inf.)
-                float mx = -INFINITY;
-                if (!masked) {
-#pragma unroll 1
-                    for (int c = 0; c < 4; ++c) {
-                        uint32_t v[32];
-                        tmem_ld_32x32(ts + c * 32, v);
-                        tmem_ld_wait();
-#pragma unroll
-                        for (int h = 0; h < 2; ++h) {
-                            const float4 q = mt[2 * c + h];
-                            float g = __uint_as_float(v[16 * h]), g2 = __uint_as_float(v[16 * h + 1]);
-#pragma unroll
-                            for (int k = 2; k < 14; k += 4) {
-                                g = max3(g, __uint_as_float(v[16 * h + k]), __uint_as_float(v[16 * h + k + 1]));
-                                g2 = max3(g2, __uint_as_float(v[16 * h + k + 2]), __uint_as_float(v[16 * h + k + 3]));
-                            }
-                            g = max3(g, __uint_as_float(v[16 * h + 14]), __uint_as_float(v[16 * h + 15]));
-                            mx = fmaxf(mx, fmaf(fmaxf(g, g2), factor * q.x, q.y));
-                        }
-                    }
-                } else {
-#pragma unroll 1
-                    for (int c = 0; c < 4; ++c) {
-                        uint32_t v[32];
-                        __syncwarp();
-                        tmem_ld_32x32(ts + c * 32, v);
-                        tmem_ld_wait();
-#pragma unroll
-                        for (int h = 0; h < 2; ++h) {
-                            const float4 q = mt[2 * c + h];
-                            const uint32_t bits = seen(2 * c + h);
-                            float g = -INFINITY;
-#pragma unroll
-                            for (int k = 0; k < 16; ++k) g = fmaxf(g, bits >> k & 1 ? __uint_as_float(v[16 * h + k]) : -INFINITY);
-                            if (bits != 0) mx = fmaxf(mx, fmaf(g, factor * q.x, q.y));
-                        }
-                    }
-                }
-                // ---- a new reference, only where a score has outgrown the old one by 2^15 (and in a piece's first tile)
-                const bool grow = mx > m + kManyGrow;
-                if (__any_sync(0xffffffffu, grow)) {
-                    const float m_new = grow ? mx - kManyShift : m;
-                    const float al = grow ? (m == -INFINITY ? 0.0f : ex2(m - m_new)) : 1.0f;
-                    m = m_new;
-                    l *= al;
-                    if (done > 0) {
-                        ok = attn_wait(&pv_done[x], (n_mine - 1) & 1, abort_flag, p.status, DEV_TIMEOUT_TMEM_FULL);
-                        if (!ok) break;
-                        tcgen05_fence_after();
-#pragma unroll 1
-                        for (int c = 0; c < kDim / 32; ++c) {
-                            uint32_t v[32];
-                            __syncwarp();
-                            tmem_ld_32x32(to + c * 32, v);
-                            tmem_ld_wait();
-#pragma unroll
-                            for (int k = 0; k < 32; ++k) v[k] = __float_as_uint(__uint_as_float(v[k]) * al);
-                            tmem_st_32x32(to + c * 32, v);
-                        }
-                    }
-                }
-                const float ms = m == -INFINITY ? 0.0f : m;
-                // ---- probabilities, over the scores' own columns (those of 32 tokens fit the columns of 16, read before)
-#pragma unroll 1
-                for (int c = 0; c < 4; ++c) {
-                    uint32_t v[32], w[16];
-                    __syncwarp();
-                    tmem_ld_32x32(ts + c * 32, v);
-                    const float4 q0 = mt[2 * c], q1 = mt[2 * c + 1];
-                    tmem_ld_wait();
-                    if (masked) {
-                        // (a score that the row does not see may be anything: taken out before the exponential)
-                        const uint32_t bits = seen(2 * c) | seen(2 * c + 1) << 16;
-#pragma unroll
-                        for (int k = 0; k < 32; ++k) v[k] = bits >> k & 1 ? v[k] : 0xFF800000u;
-                    }
+                // Probabilities of 32 tokens, over the scores' own columns (they fit those of 16 tokens, read before).
+                auto exponentials = [&](int c, const uint32_t (&v)[32], float floor_k1) {
+                    uint32_t w[16];
 #pragma unroll
                     for (int h = 0; h < 2; ++h) {
-                        const float4 q = h ? q1 : q0;
-                        const float k1 = fmaxf(factor * q.x, masked ? 1e-37f : 0.0f), k0 = q.y - ms;
+                        const float4 q = mt[2 * c + h];
+                        const float k1 = fmaxf(factor * q.x, floor_k1), k0 = q.y - ms;
                         float part = 0.0f, part2 = 0.0f;
 #pragma unroll
                         for (int k = 0; k < 16; k += 4) {
@@ -387,6 +355,69 @@ cache_attention_many_kernel(const CacheAttentionParams p, const CacheView cache)
                         l = fmaf(part + part2, q.z, l);
                     }
                     tmem_st_32x16(ts + c * 16, w);
+                };
+                // (blocks that do not exist have codes of zero and an exponent of -inf)
+                float mx = -INFINITY;
+                if (!masked) {
+                    uint32_t sc[4][32];
+#pragma unroll
+                    for (int c = 0; c < 4; ++c) tmem_ld_32x32(ts + c * 32, sc[c]);
+                    tmem_ld_wait();
+#pragma unroll
+                    for (int g = 0; g < 8; ++g) {
+                        const float4 q = mt[g];
+                        const uint32_t* e = &sc[g >> 1][16 * (g & 1)];
+                        float a = __uint_as_float(e[0]), b = __uint_as_float(e[1]);
+#pragma unroll
+                        for (int k = 2; k < 14; k += 4) {
+                            a = max3(a, __uint_as_float(e[k]), __uint_as_float(e[k + 1]));
+                            b = max3(b, __uint_as_float(e[k + 2]), __uint_as_float(e[k + 3]));
+                        }
+                        a = max3(a, __uint_as_float(e[14]), __uint_as_float(e[15]));
+                        mx = fmaxf(mx, fmaf(fmaxf(a, b), factor * q.x, q.y));
+                    }
+                    refer(mx);
+                    if (!ok) break;
+#pragma unroll
+                    for (int c = 0; c < 4; ++c) exponentials(c, sc[c], 0.0f);
+                } else {
+                    // bits of the tokens of 32 columns that this row sees
+                    auto seen = [&](int c) -> uint32_t {
+                        const int a = max(see_lo - (tok0 + 32 * c), 0), b = min(see_hi - (tok0 + 32 * c), 32);
+                        return b > a ? (0xFFFFFFFFu >> (32 - b)) & (0xFFFFFFFFu << a) : 0u;
+                    };
+#pragma unroll 1
+                    for (int c = 0; c < 4; ++c) {
+                        uint32_t v[32];
+                        __syncwarp();
+                        tmem_ld_32x32(ts + c * 32, v);
+                        tmem_ld_wait();
+                        const uint32_t bits = seen(c);
+#pragma unroll
+                        for (int h = 0; h < 2; ++h) {
+                            const float4 q = mt[2 * c + h];
+                            float g = -INFINITY;
+#pragma unroll
+                            for (int k = 16 * h; k < 16 * h + 16; ++k) g = fmaxf(g, bits >> k & 1 ? __uint_as_float(v[k]) : -INFINITY);
+                            if (bits >> (16 * h) & 0xFFFFu) mx = fmaxf(mx, fmaf(g, factor * q.x, q.y));
+                        }
+                    }
+                    __syncwarp();
+                    refer(mx);
+                    if (!ok) break;
+#pragma unroll 1
+                    for (int c = 0; c < 4; ++c) {
+                        uint32_t v[32];
+                        __syncwarp();
+                        tmem_ld_32x32(ts + c * 32, v);
+                        tmem_ld_wait();
+                        // a score that the row does not see may be anything: taken out before the exponential (whose
+                        // factor then must not be zero)
+                        const uint32_t bits = seen(c);
+#pragma unroll
+                        for (int k = 0; k < 32; ++k) v[k] = bits >> k & 1 ? v[k] : 0xFF800000u;
+                        exponentials(c, v, 1e-37f);
+                    }
                 }
                 tmem_st_wait();
                 tcgen05_fence_before();
@@ -470,6 +501,7 @@ cache_attention_many_kernel(const CacheAttentionParams p, const CacheView cache)
         }
     } else if (warp < 12) {
         // ------------------------------------------------------------------ codes -> half, scales
+        regs_dec<kConvertRegs>();
         const int tid = threadIdx.x - 256;
         constexpr int kChunks = kDim / 16;                    // 16-code chunks of a row
         constexpr int kPasses = kDim / 16;                    // rows of a tile that a thread has a chunk of
@@ -592,6 +624,9 @@ cache_attention_many_kernel(const CacheAttentionParams p, const CacheView cache)
         }
         cp_async_wait<0>();
     } else {
+        regs_dec<kIssueRegs>();
+    }
+    if (warp == 12) {
         // ------------------------------------------------------------------ MMA issue
         constexpr uint32_t idesc_qk = umma_idesc_half(128, false);
         constexpr uint32_t idesc_pv = umma_idesc_half(kDim, true);

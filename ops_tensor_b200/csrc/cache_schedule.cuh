@@ -56,7 +56,7 @@ struct CacheAttentionParams {
 
 // A wait whose bounded loop is out of line: the roles of a kernel share the instruction cache, and a wait that has to
 // wait does not mind a call.
-static __device__ __noinline__ bool attn_wait_slow(uint32_t bar, uint32_t parity, volatile int* abort_flag, int* status, int code) {
+static __device__ __forceinline__ bool attn_wait_slow(uint32_t bar, uint32_t parity, volatile int* abort_flag, int* status, int code) {
     return mbar_wait_addr(bar, parity, abort_flag, status, code);
 }
 __device__ __forceinline__ bool attn_wait(uint64_t* bar, uint32_t parity, volatile int* abort_flag, int* status, int code) {
@@ -241,7 +241,7 @@ __device__ __forceinline__ void attn_write_cut(const CacheAttentionParams& p, co
 
 // attn_piece_at out of line, for a kernel whose roles share the instruction cache.
 template <int kRows, int kTokens>
-__device__ __noinline__ AttnPiece attn_piece(const CacheAttentionParams& p, const int* prefix, int u, int end) {
+__device__ __forceinline__ AttnPiece attn_piece(const CacheAttentionParams& p, const int* prefix, int u, int end) {
     return attn_piece_at<kRows, kTokens>(p, prefix, u, end);
 }
 

@@ -22,9 +22,9 @@ namespace blaze {
 constexpr int kManyRows = 256;
 constexpr int kManyTokens = 128;
 constexpr int kManyThreads = 32 * 16;      // warps 13-15 only complete the last warpgroup
-// Registers of a thread of the softmax, converting and issuing warpgroups (a softmax thread holds its row's 128 scores);
+// Registers of a thread of the softmax, converting and issuing warpgroups (a softmax thread holds 64 to 96 scores);
 // the launch has 128 each, 512 for the four.
-constexpr int kSoftmaxRegs = 184, kConvertRegs = 88, kIssueRegs = 56;
+constexpr int kSoftmaxRegs = 176, kConvertRegs = 88, kIssueRegs = 72;
 static_assert(2 * kSoftmaxRegs + kConvertRegs + kIssueRegs <= 4 * 128, "setmaxnreg draws on what the launch has");
 constexpr int kManyMeta = 4;              // tiles whose scales are held
 
@@ -359,27 +359,44 @@ cache_attention_many_kernel(const CacheAttentionParams p, const CacheView cache)
                 // (blocks that do not exist have codes of zero and an exponent of -inf)
                 float mx = -INFINITY;
                 if (!masked) {
-                    uint32_t sc[4][32];
+                    // the largest of the scores of 64..127 first, then of 0..63, which stay for the exponentials; the others
+                    // are read again behind them
+                    uint32_t sc[2][32];
+                    auto largest = [&](int c, const uint32_t (&v)[32]) {
 #pragma unroll
-                    for (int c = 0; c < 4; ++c) tmem_ld_32x32(ts + c * 32, sc[c]);
-                    tmem_ld_wait();
+                        for (int h = 0; h < 2; ++h) {
+                            const float4 q = mt[2 * c + h];
+                            const uint32_t* e = &v[16 * h];
+                            float a = __uint_as_float(e[0]), b = __uint_as_float(e[1]);
 #pragma unroll
-                    for (int g = 0; g < 8; ++g) {
-                        const float4 q = mt[g];
-                        const uint32_t* e = &sc[g >> 1][16 * (g & 1)];
-                        float a = __uint_as_float(e[0]), b = __uint_as_float(e[1]);
-#pragma unroll
-                        for (int k = 2; k < 14; k += 4) {
-                            a = max3(a, __uint_as_float(e[k]), __uint_as_float(e[k + 1]));
-                            b = max3(b, __uint_as_float(e[k + 2]), __uint_as_float(e[k + 3]));
+                            for (int k = 2; k < 14; k += 4) {
+                                a = max3(a, __uint_as_float(e[k]), __uint_as_float(e[k + 1]));
+                                b = max3(b, __uint_as_float(e[k + 2]), __uint_as_float(e[k + 3]));
+                            }
+                            a = max3(a, __uint_as_float(e[14]), __uint_as_float(e[15]));
+                            mx = fmaxf(mx, fmaf(fmaxf(a, b), factor * q.x, q.y));
                         }
-                        a = max3(a, __uint_as_float(e[14]), __uint_as_float(e[15]));
-                        mx = fmaxf(mx, fmaf(fmaxf(a, b), factor * q.x, q.y));
-                    }
+                    };
+                    tmem_ld_32x32(ts + 64, sc[0]);
+                    tmem_ld_32x32(ts + 96, sc[1]);
+                    tmem_ld_wait();
+                    largest(2, sc[0]);
+                    largest(3, sc[1]);
+                    tmem_ld_32x32(ts, sc[0]);
+                    tmem_ld_32x32(ts + 32, sc[1]);
+                    tmem_ld_wait();
+                    largest(0, sc[0]);
+                    largest(1, sc[1]);
                     refer(mx);
                     if (!ok) break;
-#pragma unroll
-                    for (int c = 0; c < 4; ++c) exponentials(c, sc[c], 0.0f);
+                    exponentials(0, sc[0], 0.0f);
+                    tmem_ld_32x32(ts + 64, sc[0]);
+                    exponentials(1, sc[1], 0.0f);
+                    tmem_ld_wait();
+                    tmem_ld_32x32(ts + 96, sc[1]);
+                    exponentials(2, sc[0], 0.0f);
+                    tmem_ld_wait();
+                    exponentials(3, sc[1], 0.0f);
                 } else {
                     // bits of the tokens of 32 columns that this row sees
                     auto seen = [&](int c) -> uint32_t {

@@ -54,19 +54,32 @@ struct CacheAttentionParams {
     int* status;
 };
 
-// A wait whose bounded loop is out of line: the roles of a kernel share the instruction cache, and a wait that has to
-// wait does not mind a call.
-static __device__ __forceinline__ bool attn_wait_slow(uint32_t bar, uint32_t parity, volatile int* abort_flag, int* status, int code) {
-    return mbar_wait_addr(bar, parity, abort_flag, status, code);
-}
+// Bounded wait of a whole warp.  The hardware keeps the warp asleep for up to kAttnNapNs at a time instead of having it
+// spin: the warps of a block share their schedulers with the ones that they wait for.
+constexpr uint32_t kAttnNapNs = 1000000;
 __device__ __forceinline__ bool attn_wait(uint64_t* bar, uint32_t parity, volatile int* abort_flag, int* status, int code) {
-    bool ok = mbar_try_wait(bar, parity);
-    if (!__all_sync(0xffffffffu, ok)) {
-        ok = attn_wait_slow(smem_u32(bar), parity, abort_flag, status, code);
-        ok = __all_sync(0xffffffffu, ok);
-        return ok;
+    const uint32_t at = smem_u32(bar);
+    long long t0 = 0;
+    for (;;) {
+        uint32_t ok;
+        asm volatile(
+            "{\n\t.reg .pred p;\n\t"
+            "mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2, %3;\n\t"
+            "selp.u32 %0, 1, 0, p;\n\t}\n"
+            : "=r"(ok)
+            : "r"(at), "r"(parity), "r"(kAttnNapNs)
+            : "memory");
+        if (__all_sync(0xffffffffu, ok != 0)) return true;
+        const long long now = clock64();
+        if (t0 == 0) t0 = now;
+        int over = *abort_flag;
+        if (now - t0 > BLAZE_WAIT_LIMIT_CYCLES) {
+            over = 1;
+            *abort_flag = 1;
+            atomicCAS(status, 0, code);
+        }
+        if (__any_sync(0xffffffffu, over != 0)) return false;
     }
-    return true;
 }
 
 struct AttnRequest {

@@ -667,40 +667,34 @@ cache_attention_many_kernel(const CacheAttentionParams p, const CacheView cache)
                 const bool more = t < s.tile1, behind = t > s.tile0;
                 const uint32_t k_tile = ring_addr + ring_k * L::kOperandBytes, v_tile = ring_addr + ring_v * L::kOperandBytes;
                 const uint32_t active = more ? (sub0.active(t) ? 1u : 0u) | (sub1.active(t) ? 2u : 0u) : 0u;
+                // (the operands are there long before the probabilities)
                 if (behind) {
                     ok = attn_wait(&full[ring_v], phase_v, abort_flag, p.status, DEV_TIMEOUT_SMEM_FULL);
                     if (!ok) break;
                 }
+                if (more) {
+                    ok = attn_wait(&full[ring_k], phase_k, abort_flag, p.status, DEV_TIMEOUT_SMEM_FULL);
+                    if (!ok) break;
+                }
+                const bool last = t == s.tile1 - 1 || s.tile0 == s.tile1;
 #pragma unroll 1
                 for (int x = 0; x < 2; ++x) {
                     const uint32_t ts = tmem + x * 128, to = tmem + 256 + x * kDim;
-                    if (pending >> x & 1) {
+                    const bool pv = pending >> x & 1, qk = active >> x & 1;
+                    if (pv) {
                         ok = attn_wait(&p_full[x], ((n_mine >> x) & 1) ^ 1, abort_flag, p.status, DEV_TIMEOUT_TMEM_EMPTY);
                         if (!ok) break;
-                        tcgen05_fence_after();
-                        if (elect_one()) {
+                    }
+                    tcgen05_fence_after();
+                    if (elect_one()) {
+                        if (pv) {
                             const uint64_t b = umma_desc_sw128_mn(v_tile, 16384);
 #pragma unroll
                             for (int k = 0; k < 8; ++k)        // 16 tokens a step: 2048 bytes of V, 8 columns of P
                                 umma_f16_ts(to, ts + 8 * k, b + 128 * k, idesc_pv, k > 0 ? 1u : started >> x & 1);
                             umma_commit(&pv_done[x]);
                         }
-                        __syncwarp();
-                        started |= 1u << x;
-                        pending &= ~(1u << x);
-                    }
-                    if (x == 0) {
-                        if (more) {
-                            ok = attn_wait(&full[ring_k], phase_k, abort_flag, p.status, DEV_TIMEOUT_SMEM_FULL);
-                            if (!ok) break;
-                            tcgen05_fence_after();
-                        }
-                    } else if (behind) {
-                        if (elect_one()) umma_commit(&free_[ring_v]);
-                        __syncwarp();
-                    }
-                    if (active >> x & 1) {
-                        if (elect_one()) {
+                        if (qk) {
                             const uint64_t a = umma_desc_sw128(q_addr + x * L::kOperandBytes);
                             const uint64_t b = umma_desc_sw128(k_tile);
 #pragma unroll
@@ -710,17 +704,23 @@ cache_attention_many_kernel(const CacheAttentionParams p, const CacheView cache)
                             }
                             umma_commit(&s_full[x]);
                         }
-                        __syncwarp();
+                        if (x == 1) {
+                            if (behind) umma_commit(&free_[ring_v]);
+                            if (more) umma_commit(&free_[ring_k]);
+                            if (last) umma_commit(q_free);
+                        }
+                    }
+                    __syncwarp();
+                    if (pv) {
+                        started |= 1u << x;
+                        pending &= ~(1u << x);
+                    }
+                    if (qk) {
                         pending |= 1u << x;
                         n_mine ^= 1u << x;
                     }
                 }
                 if (!ok) break;
-                if (elect_one()) {
-                    if (more) umma_commit(&free_[ring_k]);
-                    if (t == s.tile1 - 1 || s.tile0 == s.tile1) umma_commit(q_free);
-                }
-                __syncwarp();
                 if (behind) advance(ring_v, phase_v);
                 if (more) advance(ring_k, phase_k);
             }

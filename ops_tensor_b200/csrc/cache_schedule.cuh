@@ -54,22 +54,13 @@ struct CacheAttentionParams {
     int* status;
 };
 
-// Bounded wait of a whole warp.  The hardware keeps the warp asleep for up to kAttnNapNs at a time instead of having it
-// spin: the warps of a block share their schedulers with the ones that they wait for.
-constexpr uint32_t kAttnNapNs = 1000000;
+// Bounded wait of a whole warp.
 __device__ __forceinline__ bool attn_wait(uint64_t* bar, uint32_t parity, volatile int* abort_flag, int* status, int code) {
-    const uint32_t at = smem_u32(bar);
+    if (__all_sync(0xffffffffu, mbar_try_wait(bar, parity))) return true;
     long long t0 = 0;
     for (;;) {
-        uint32_t ok;
-        asm volatile(
-            "{\n\t.reg .pred p;\n\t"
-            "mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2, %3;\n\t"
-            "selp.u32 %0, 1, 0, p;\n\t}\n"
-            : "=r"(ok)
-            : "r"(at), "r"(parity), "r"(kAttnNapNs)
-            : "memory");
-        if (__all_sync(0xffffffffu, ok != 0)) return true;
+        const bool ok = mbar_try_wait(bar, parity);
+        if (__all_sync(0xffffffffu, ok)) return true;
         const long long now = clock64();
         if (t0 == 0) t0 = now;
         int over = *abort_flag;

@@ -277,26 +277,42 @@ __device__ __forceinline__ uint32_t rescale4(uint32_t w, float ratio) {
     return cvt_e4m3x4_sat(f[0], f[1], f[2], f[3]);
 }
 
-// A run is what neighbouring rows of the call put into one block.  One warp takes a run for one head of K or of V: it
-// reads the rows twice, for the largest magnitude and, out of L1 / L2, for the conversion (16-byte loads, eight in
-// flight per lane), and re-scales the block's older rows when the scale rises.
-// Bound by the bytes: 4 bytes read and 2 written per (token, head, dim) of K and V together.
+// Eight 16-bit inputs -> eight codes under a scale: x * inv where 1 / scale is exact (`inv` not 0), else a division.
+template <bool kBf16>
+__device__ __forceinline__ uint2 encode8(const uint4& v, float inv, float scale) {
+    float f[8];
+    unpack2<kBf16>(v.x, f[0], f[1]);
+    unpack2<kBf16>(v.y, f[2], f[3]);
+    unpack2<kBf16>(v.z, f[4], f[5]);
+    unpack2<kBf16>(v.w, f[6], f[7]);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) f[i] = inv != 0.0f ? f[i] * inv : __fdiv_rn(f[i], scale);
+    return make_uint2(cvt_e4m3x4_sat(f[0], f[1], f[2], f[3]), cvt_e4m3x4_sat(f[4], f[5], f[6], f[7]));
+}
+
+// A run is what neighbouring rows of the call put into one block; it is taken up for one head of K or of V at a time.
+// Runs of more than kStoreShort rows are shared by the block's four warps: every lane holds its 16-byte pieces of up to
+// eight rows from the one read (a block of 64 tokens then needs no second), the largest magnitude goes through shared
+// memory.  Shorter runs (a decode step's single rows) go to one warp each.
+// Bound by the bytes: 4 read and 2 written per (token, head, dim) of K and V together.
+constexpr int kStoreShort = 4;
+
 template <int kDim, bool kBf16>
 __global__ void __launch_bounds__(kStoreWarps * 32) cache_store_kernel(const CacheStoreParams p) {
     constexpr int kLanesPerRow = kDim / 8;               // 16 bytes of input, 8 of codes per lane
     constexpr int kRowsPerLoad = 32 / kLanesPerRow;
     constexpr int kBatch = 8;
+    __shared__ uint32_t warp_max[2][kStoreWarps];
     grid_launch_dependents();
     grid_dependency_wait();
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     const int sub = lane / kLanesPerRow;                 // row of a load that this lane has a part of
     const int col = (lane % kLanesPerRow) * 8;
+    // heads of K and V beside one another, so that what runs together reads whole rows of the input
     const int units = 2 * p.cache.kv_heads;
-    const int windows = (p.tokens + p.window - 1) / p.window;
-    const int win = blockIdx.x % windows;
-    const int unit = blockIdx.x / windows;
-    const int which = unit & 1, head = unit >> 1;
-    (void)units;
+    const int win = blockIdx.x / units;
+    const int unit = blockIdx.x - win * units;
+    const int which = unit >= p.cache.kv_heads ? 1 : 0, head = unit - which * p.cache.kv_heads;
     const int w0 = win * p.window;
     const int w1 = min(p.tokens, w0 + p.window);
     const uint16_t* x = static_cast<const uint16_t*>(p.x[which]) + head * p.head_stride[which] + col;
@@ -309,7 +325,11 @@ __global__ void __launch_bounds__(kStoreWarps * 32) cache_store_kernel(const Cac
         const long long s = p.slots[t];
         return (s < 0 || s >= p.slot_count) ? -1 : (s >> shift);
     };
-    int turn = 0;                                        // runs of the window, dealt to the warps in turn
+    auto load = [&](int row, int end) -> uint4 {
+        return row < end ? *reinterpret_cast<const uint4*>(x + (long long)row * row_stride) : make_uint4(0, 0, 0, 0);
+    };
+    int turn = 0;                                        // short runs of the window, dealt to the warps in turn
+    int shared_runs = 0;
     for (int base = w0; base < w1; base += 32) {
         const int t = base + lane;
         const long long mine = t < w1 ? block_of(t) : -1;
@@ -319,42 +339,53 @@ __global__ void __launch_bounds__(kStoreWarps * 32) cache_store_kernel(const Cac
         while (starts) {
             const int first = __ffs(starts) - 1;
             starts &= starts - 1;
-            if ((turn++ % kStoreWarps) != warp) continue;
             const int a = base + first;
             const long long block = __shfl_sync(0xffffffffu, mine, first);
             // the run's end, and its lowest row within the block
             int b = a, low = p.cache.block_size;
+            bool twice = false;                          // rows out of order: a slot may be named twice
             for (;;) {
                 const int u = b + lane;
                 const long long s = u < p.tokens ? p.slots[u] : -1;
                 const bool in = s >= 0 && s < p.slot_count && (s >> shift) == block;
                 const uint32_t out = ~__ballot_sync(0xffffffffu, in);
                 const int n = out ? __ffs(out) - 1 : 32;
-                low = min(low, (int)__reduce_min_sync(0xffffffffu, lane < n ? (unsigned)(s & (p.cache.block_size - 1))
-                                                                            : 0x7FFFFFFFu));
+                const int at = (int)(s & (p.cache.block_size - 1));
+                low = min(low, (int)__reduce_min_sync(0xffffffffu, lane < n ? (unsigned)at : 0x7FFFFFFFu));
+                const long long s_before = (lane < n && u > a) ? p.slots[u - 1] : s - 1;
+                twice |= __any_sync(0xffffffffu, lane < n && s != s_before + 1);
                 b += n;
                 if (n < 32) break;
             }
-            // largest finite magnitude
+            const bool shared = b - a > kStoreShort && !twice;
+            if (!shared && (turn++ % kStoreWarps) != warp) continue;
+            // this warp's rows: r0, r0 + step, ...; all that a lane loads at once is kept when it is all there is
+            const int span = kRowsPerLoad * kBatch;
+            const int step = shared ? span * kStoreWarps : span;
+            const int r0 = shared ? a + warp * span : a;
+            const bool kept = b - a <= step;
+            uint4 v[kBatch];
             uint32_t m = 0;
-            for (int r = a; r < b; r += kRowsPerLoad * kBatch) {
-                uint4 v[kBatch];
+            for (int r = r0; r < b; r += step) {
 #pragma unroll
-                for (int j = 0; j < kBatch; ++j) {
-                    const int row = r + j * kRowsPerLoad + sub;
-                    v[j] = make_uint4(0, 0, 0, 0);
-                    if (row < b) v[j] = *reinterpret_cast<const uint4*>(x + (long long)row * row_stride);
-                }
+                for (int j = 0; j < kBatch; ++j) v[j] = load(r + j * kRowsPerLoad + sub, b);
 #pragma unroll
                 for (int j = 0; j < kBatch; ++j)
                     m = max_finite<kBf16>(max_finite<kBf16>(max_finite<kBf16>(max_finite<kBf16>(m, v[j].x), v[j].y), v[j].z), v[j].w);
             }
             m = __reduce_max_sync(0xffffffffu, m);
+            float* scale_at = scales + block * p.cache.scale_stride;
+            const float old = low > 0 ? *scale_at : 0.0f;
+            if (shared) {
+                uint32_t* wm = warp_max[shared_runs++ & 1];
+                if (lane == 0) wm[warp] = m;
+                __syncthreads();                         // (and every warp has read the old scale)
+#pragma unroll
+                for (int w = 0; w < kStoreWarps; ++w) m = max(m, wm[w]);
+            }
             float amax, unused;
             unpack2<kBf16>(m, amax, unused);
             const float need = scale_for(amax);
-            float* scale_at = scales + block * p.cache.scale_stride;
-            const float old = low > 0 ? *scale_at : 0.0f;
             const float scale = old >= need ? old : need;
             // 1 / scale is exact for the powers of two that this store writes; another scale is divided by
             const bool pow2 = (__float_as_uint(scale) & 0x7FFFFFu) == 0 && scale >= 0x1p-64f && scale <= 0x1p120f;
@@ -362,55 +393,48 @@ __global__ void __launch_bounds__(kStoreWarps * 32) cache_store_kernel(const Cac
             uint8_t* page = codes + block * p.cache.block_stride;
             if (scale != old && old > 0.0f) {
                 const float ratio = old / scale;
-                for (int r = sub; r < low; r += kRowsPerLoad) {
+                for (int r = sub + (shared ? warp * kRowsPerLoad : 0); r < low; r += kRowsPerLoad * (shared ? kStoreWarps : 1)) {
                     uint2* at = reinterpret_cast<uint2*>(page + (long long)r * p.cache.token_stride);
                     const uint2 w = *at;
                     *at = make_uint2(rescale4(w.x, ratio), rescale4(w.y, ratio));
                 }
             }
-            for (int r = a; r < b; r += kRowsPerLoad * kBatch) {
-                uint4 v[kBatch];
-                long long slot[kBatch];
+            if (shared) {
+                // slots rise one by one: row r goes to slot low + r - a
+                for (int r = r0; r < b; r += step) {
+                    if (!kept) {
 #pragma unroll
-                for (int j = 0; j < kBatch; ++j) {
-                    const int row = r + j * kRowsPerLoad + sub;
-                    v[j] = make_uint4(0, 0, 0, 0);
-                    slot[j] = 0;
-                    if (row < b) {
-                        v[j] = *reinterpret_cast<const uint4*>(x + (long long)row * row_stride);
-                        slot[j] = p.slots[row];
+                        for (int j = 0; j < kBatch; ++j) v[j] = load(r + j * kRowsPerLoad + sub, b);
+                    }
+#pragma unroll
+                    for (int j = 0; j < kBatch; ++j) {
+                        const int row = r + j * kRowsPerLoad + sub;
+                        if (row < b)
+                            *reinterpret_cast<uint2*>(page + (long long)(low + row - a) * p.cache.token_stride) =
+                                encode8<kBf16>(v[j], inv, scale);
                     }
                 }
-#pragma unroll
-                for (int j = 0; j < kBatch; ++j) {
-                    const int row = r + j * kRowsPerLoad + sub;
-                    float f[8];
-                    unpack2<kBf16>(v[j].x, f[0], f[1]);
-                    unpack2<kBf16>(v[j].y, f[2], f[3]);
-                    unpack2<kBf16>(v[j].z, f[4], f[5]);
-                    unpack2<kBf16>(v[j].w, f[6], f[7]);
-#pragma unroll
-                    for (int i = 0; i < 8; ++i) f[i] = pow2 ? f[i] * inv : __fdiv_rn(f[i], scale);
-                    // rows that name a slot twice: the loads of one instruction are the only ones that could meet, and
-                    // the last of them has to win
+                if (threadIdx.x == 0 && scale != old) *scale_at = scale;
+            } else {
+                for (int r = r0; r < b; r += kRowsPerLoad) {
+                    const int row = r + sub;
+                    const uint4 w = load(row, b);
+                    const long long slot = row < b ? p.slots[row] : 0;
+                    // rows that name a slot twice: the rows of one step are the only ones that could meet, and the last
+                    // of them has to win
                     bool last = row < b;
-                    if (kRowsPerLoad > 1) {
 #pragma unroll
-                        for (int o = 1; o < kRowsPerLoad; ++o) {
-                            const long long s = __shfl_down_sync(0xffffffffu, slot[j], o * kLanesPerRow);
-                            if (sub + o < kRowsPerLoad && row + o < b && s == slot[j]) last = false;
-                        }
+                    for (int o = 1; o < kRowsPerLoad; ++o) {
+                        const long long s = __shfl_down_sync(0xffffffffu, slot, o * kLanesPerRow);
+                        if (sub + o < kRowsPerLoad && row + o < b && s == slot) last = false;
                     }
-                    if (last) {
-                        const int at = (int)(slot[j] & (p.cache.block_size - 1));
-                        *reinterpret_cast<uint2*>(page + (long long)at * p.cache.token_stride) =
-                            make_uint2(cvt_e4m3x4_sat(f[0], f[1], f[2], f[3]), cvt_e4m3x4_sat(f[4], f[5], f[6], f[7]));
-                    }
+                    if (last)
+                        *reinterpret_cast<uint2*>(page + (long long)(slot & (p.cache.block_size - 1)) * p.cache.token_stride) =
+                            encode8<kBf16>(w, inv, scale);
                     __syncwarp();                        // the next rows' stores come behind these
                 }
+                if (lane == 0 && scale != old) *scale_at = scale;
             }
-            __syncwarp();
-            if (lane == 0 && scale != old) *scale_at = scale;
         }
     }
 }

@@ -7,6 +7,7 @@ library.
 from __future__ import annotations
 
 import ctypes as C
+import struct
 from pathlib import Path
 
 _LIB_PATH = Path(__file__).resolve().parent / "libops_tensor_b200.so"
@@ -205,11 +206,11 @@ def _declare(l: C.CDLL) -> None:
                                             C.c_void_p, C.c_void_p]
     l.blazeQuantizeFp8Blocks.argtypes = [C.c_void_p, C.c_int64, C.c_int32, C.c_int32, C.c_void_p, C.c_int64,
                                          C.c_void_p, C.c_void_p]
-    l.blazeCacheAssign.argtypes = [C.POINTER(CacheAssignArgs), C.c_void_p]
-    l.blazeCacheStore.argtypes = [C.POINTER(KvCacheDesc), C.POINTER(CacheStoreArgs), C.c_void_p]
-    l.blazeCacheAttentionWorkspaceSize.argtypes = [C.POINTER(KvCacheDesc), C.POINTER(CacheAttentionArgs),
-                                                   C.POINTER(C.c_size_t)]
-    l.blazeCacheAttention.argtypes = [C.POINTER(KvCacheDesc), C.POINTER(CacheAttentionArgs), C.c_void_p]
+    # (void pointers: a byref() of the structure or its bytes)
+    l.blazeCacheAssign.argtypes = [C.c_void_p, C.c_void_p]
+    l.blazeCacheStore.argtypes = [C.c_void_p, C.c_void_p, C.c_void_p]
+    l.blazeCacheAttentionWorkspaceSize.argtypes = [C.c_void_p, C.c_void_p, C.POINTER(C.c_size_t)]
+    l.blazeCacheAttention.argtypes = [C.c_void_p, C.c_void_p, C.c_void_p]
     l.blazeAddF32.argtypes = [C.c_void_p, C.c_void_p, C.c_void_p, C.c_int64, C.c_void_p]
     l.blazeSelfTestWaitTimeout.argtypes = [C.c_int64, C.c_void_p]
     l.blazeSelfTestWaitTimeout.restype = C.c_int
@@ -486,9 +487,23 @@ def peer_signal(local_flags, peer_flags, my_rank: int, peer_ranks, value: int, l
 
 # ------------------------------------------------------------------------------------------------ paged 8-bit cache
 
-def _launch(fn, name, device: int, *args) -> None:
-    """Calls a C entry point on the current stream of the GPU that its tensors live on, with that GPU current."""
+torch = None          # imported when the first of these calls is made
+
+
+def _import_torch():
+    global torch
     import torch
+
+
+# The arguments' layouts, for the calls of every step: packing them costs a fifth of filling the ctypes structures in.
+_ASSIGN = struct.Struct("@Niiii PP Pq Pii PP PP PPP")
+_STORE = struct.Struct("@Nii PP qqqq P")
+_ATTENTION = struct.Struct("@Niiii Pqq Pqq P PP Pq iiii fiii PN")
+
+
+def _launch(name, device: int, *args) -> None:
+    """Calls a C entry point on the current stream of the GPU that its tensors live on, with that GPU current."""
+    fn = getattr(lib(), name)
     if device == torch.cuda.current_device():
         status = fn(*args, torch._C._cuda_getCurrentRawStream(device))
     else:
@@ -518,7 +533,6 @@ def _vector(t, name, dtype, at_least) -> int:
 
 def _table(t):
     """(rows, columns, pitch) of a block table."""
-    import torch
     if t.dtype is not torch.int32 or t.dim() != 2:
         raise ValueError("block_table: an int32 [requests, blocks] tensor is wanted")
     rows, columns = t.shape
@@ -536,7 +550,8 @@ class PagedCache:
     [blocks, kv heads].  Keeps the tensors; `desc` is the C ABI's view of them."""
 
     def __init__(self, k, v, k_scale, v_scale):
-        import torch
+        if torch is None:
+            _import_torch()
         _same_device(k, v, k_scale, v_scale)
         if k.dim() != 4 or k.shape != v.shape or k.dtype != v.dtype or k.dtype not in (torch.uint8, torch.float8_e4m3fn):
             raise ValueError("k and v: two [blocks, heads, block size, head size] tensors of uint8 or float8_e4m3fn")
@@ -560,11 +575,13 @@ class PagedCache:
         c.block_stride, c.head_stride, c.token_stride = k.stride()[:3]
         c.k_scale, c.v_scale = k_scale.data_ptr(), v_scale.data_ptr()
         c.scale_stride = k_scale.stride(0) if n > 1 else h
+        self._desc_at = C.addressof(c)
 
     @classmethod
     def empty(cls, num_blocks, kv_heads, block_size, head_dim, device="cuda"):
         """A new cache: codes of zero, scales of one."""
-        import torch
+        if torch is None:
+            _import_torch()
         shape = (num_blocks, kv_heads, block_size, head_dim)
         k, v = (torch.zeros(shape, dtype=torch.uint8, device=device) for _ in range(2))
         ks, vs = (torch.ones((num_blocks, kv_heads), dtype=torch.float32, device=device) for _ in range(2))
@@ -576,7 +593,8 @@ def cache_assign(cached_len, new_len, block_table, free_blocks, free_count, *, b
     """The bookkeeping of a serving step on the GPU (blazeCacheAssign): blocks for the requests that grow, the blocks of
     the ended ones (`new_len` < 0) back on the stack, and the packed batch's `row_offsets`, `slots` and `positions`.
     `kv_len` may be `cached_len`; `free_count_out` defaults to `free_count` (in place)."""
-    import torch
+    if torch is None:
+        _import_torch()
     if free_count_out is None:
         free_count_out = free_count
     device = _same_device(cached_len, new_len, block_table, free_blocks, free_count, row_offsets, kv_len, slots,
@@ -585,23 +603,22 @@ def cache_assign(cached_len, new_len, block_table, free_blocks, free_count, *, b
     rows, columns, pitch = _table(block_table)
     if rows < n:
         raise ValueError("block_table has fewer rows than there are requests")
-    a = CacheAssignArgs(
-        C.sizeof(CacheAssignArgs), n, block_size, columns, tokens,
+    a = _ASSIGN.pack(
+        _ASSIGN.size, n, block_size, columns, tokens,
         _vector(cached_len, "cached_len", i32, n), _vector(new_len, "new_len", i32, n),
         block_table.data_ptr(), pitch,
         _vector(free_blocks, "free_blocks", i32, 0), free_blocks.numel(), 0,
         _vector(free_count, "free_count", i32, 1), _vector(free_count_out, "free_count_out", i32, 1),
         _vector(row_offsets, "row_offsets", i32, n + 1), _vector(kv_len, "kv_len", i32, n),
         _vector(slots, "slots", torch.int64, 0),
-        None if positions is None else _vector(positions, "positions", i32, tokens),
-        None if denied is None else _vector(denied, "denied", i32, 1))
-    _launch(lib().blazeCacheAssign, "blazeCacheAssign", device, a)
+        0 if positions is None else _vector(positions, "positions", i32, tokens),
+        0 if denied is None else _vector(denied, "denied", i32, 1))
+    _launch("blazeCacheAssign", device, a)
 
 
 def _rows(t, name):
     """(address, token stride, head stride) of bf16 or half rows [tokens, heads, head size]; the stride of a dimension
     of one, which never counts, as 0."""
-    import torch
     if (t.dtype is not torch.bfloat16 and t.dtype is not torch.float16) or t.dim() != 3:
         raise ValueError(f"{name}: a bf16 or half [tokens, heads, head size] tensor is wanted")
     st, sh, sd = t.stride()
@@ -612,7 +629,8 @@ def _rows(t, name):
 
 def cache_store(cache: PagedCache, k, v, slots):
     """Quantises the rows of `k` and `v` [tokens, kv heads, head size] into the cache's slots (blazeCacheStore)."""
-    import torch
+    if torch is None:
+        _import_torch()
     device = _same_device(cache.k, k, v, slots)
     at = _vector(slots, "slots", torch.int64, 0)
     n = slots.numel()
@@ -621,8 +639,8 @@ def cache_store(cache: PagedCache, k, v, slots):
     rows = (cache.kv_heads, cache.head_dim)
     if k.dtype is not v.dtype or k.shape[0] < n or v.shape[0] < n or k.shape[1:] != rows or v.shape[1:] != rows:
         raise ValueError(f"k and v: [at least {n}, {cache.kv_heads}, {cache.head_dim}] is wanted, of one type")
-    a = CacheStoreArgs(C.sizeof(CacheStoreArgs), n, out_type_of(k), pk, pv, k_token, k_head, v_token, v_head, at)
-    _launch(lib().blazeCacheStore, "blazeCacheStore", device, cache.desc, a)
+    a = _STORE.pack(_STORE.size, n, out_type_of(k), pk, pv, k_token, k_head, v_token, v_head, at)
+    _launch("blazeCacheStore", device, cache._desc_at, a)
 
 
 def _attention_bounds(cache, q, requests, max_q, max_kv, sm_limit) -> CacheAttentionArgs:
@@ -634,19 +652,21 @@ def _attention_bounds(cache, q, requests, max_q, max_kv, sm_limit) -> CacheAtten
 
 
 def cache_attention_workspace_bytes(cache: PagedCache, q, *, requests, max_q, max_kv, sm_limit=0) -> int:
-    import torch
+    if torch is None:
+        _import_torch()
     n = C.c_size_t(0)
     _rows(q, "q")
     with torch.cuda.device(cache.device):
         check(lib().blazeCacheAttentionWorkspaceSize(
-            cache.desc, _attention_bounds(cache, q, requests, max_q, max_kv, sm_limit), C.byref(n)),
+            cache._desc_at, C.byref(_attention_bounds(cache, q, requests, max_q, max_kv, sm_limit)), C.byref(n)),
             "blazeCacheAttentionWorkspaceSize")
     return n.value
 
 
 def cache_attention_workspace(cache: PagedCache, q, *, requests, max_q, max_kv, sm_limit=0):
     """A workspace for cache_attention calls of these bounds; needs no initialisation, keeps nothing between calls."""
-    import torch
+    if torch is None:
+        _import_torch()
     need = cache_attention_workspace_bytes(cache, q, requests=requests, max_q=max_q, max_kv=max_kv, sm_limit=sm_limit)
     return torch.empty(max(need, 256), dtype=torch.uint8, device=cache.device)
 
@@ -657,7 +677,8 @@ def cache_attention(cache: PagedCache, q, row_offsets, kv_len, block_table, *, s
     defaults to head size ** -0.5.  `max_q`, `max_kv` bound the requests' rows and lengths, `min_q` is a hint.
     Allocates `out` (zeros: rows outside every request are not written) and `workspace` when not given; fills `lse`
     [tokens, heads] float32 when given."""
-    import torch
+    if torch is None:
+        _import_torch()
     if out is None:
         out = torch.zeros(q.shape, dtype=q.dtype, device=q.device)
     if workspace is None:
@@ -680,12 +701,12 @@ def cache_attention(cache: PagedCache, q, row_offsets, kv_len, block_table, *, s
         raise ValueError("lse: a contiguous float32 [tokens, heads] tensor is wanted")
     if not workspace.is_contiguous():
         raise ValueError("workspace: a contiguous tensor is wanted")
-    a = CacheAttentionArgs(
-        C.sizeof(CacheAttentionArgs), n, tokens, heads, out_type_of(q), pq, q_token, q_head, po, out_token, out_head,
-        None if lse is None else lse.data_ptr(), offsets, lens, block_table.data_ptr(), pitch, columns,
+    a = _ATTENTION.pack(
+        _ATTENTION.size, n, tokens, heads, out_type_of(q), pq, q_token, q_head, po, out_token, out_head,
+        0 if lse is None else lse.data_ptr(), offsets, lens, block_table.data_ptr(), pitch, columns,
         max_q, min_q, max_kv, dim ** -0.5 if scale is None else scale, 1 if causal else 0, window, sm_limit,
         workspace.data_ptr(), workspace.numel() * workspace.element_size())
-    _launch(lib().blazeCacheAttention, "blazeCacheAttention", device, cache.desc, a)
+    _launch("blazeCacheAttention", device, cache._desc_at, a)
     return out
 
 

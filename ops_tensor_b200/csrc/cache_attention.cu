@@ -11,9 +11,11 @@
 // The few-rows kernel (decode steps and short runs of tokens) is bound by the bytes of the cache.  A block has one
 // warp that fetches tiles of 64 tokens into a ring in shared memory by TMA (one box per page and operand, 128-byte
 // swizzle: 64-byte for 64-wide heads) and four warps that each take 16 of a tile's tokens through both products with
-// m16n8k16 instructions, with a running maximum, sum and output of their own, joined once per piece.  The order of the k
-// index of a product is free, so a lane reads 16 consecutive code bytes and converts them in registers; the swizzle
-// makes these reads free of bank conflicts for both operands.
+// m16n8k16 instructions, with a running maximum, sum and output of their own, joined once per piece.  Both products are
+// computed transposed, S^T = K Q^T and O^T = V^T P^T: the 16 rows of the instruction are tokens or dims, of which there
+// are many, its 8 columns the query rows, of which there are few; the probabilities change sides by an 8x8 matrix
+// transposition in registers.  The order of the k index of a product is free, so a lane reads 16 consecutive code bytes
+// and converts them in registers; the swizzle makes these reads free of bank conflicts for both operands.
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 #include <cuda_runtime.h>
@@ -28,7 +30,7 @@
 
 namespace blaze {
 
-constexpr int kFewRows = 16;          // packed rows of a row tile
+constexpr int kFewRows = 16;          // packed rows of a row tile, at most: 8 for each n8 tile of the products
 constexpr int kFewTokens = 64;        // tokens of a tile
 constexpr int kFewWarps = 4;          // computing warps, 16 tokens of a tile each
 constexpr int kFewThreads = 32 * (kFewWarps + 1);
@@ -81,13 +83,22 @@ __device__ __forceinline__ void tma_load_page(uint32_t dst, const CUtensorMap* m
 // A named barrier of the computing warps.
 __device__ __forceinline__ void compute_sync() { asm volatile("bar.sync 1, %0;" ::"n"(32 * kFewWarps) : "memory"); }
 
-template <int kDim, bool kBf16>
+// Transpose of an 8x8 matrix of halves held two to a lane.
+__device__ __forceinline__ uint32_t transpose8x8(uint32_t x) {
+    uint32_t y;
+    asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
+    return y;
+}
+
+template <int kDim, bool kBf16, int kTiles>
 __global__ void __launch_bounds__(kFewThreads, 2)
 cache_attention_few_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v,
                            const CacheAttentionParams p) {
     using L = FewSmem<kDim>;
-    constexpr int kSteps = kDim / 16;          // k16 steps of Q K^T
-    constexpr int kTiles = kDim / 8;           // n8 tiles of P V
+    constexpr int kRows = 8 * kTiles;          // query rows of a row tile, in kTiles n8 tiles
+    constexpr int kSteps = kDim / 16;          // k16 steps of K Q^T
+    constexpr int kBands = kDim / 16;          // m16 tiles of V^T P^T
+    constexpr int kLaneDims = kDim / 8;        // consecutive dims of O of a lane
     extern __shared__ uint8_t few_smem_raw[];
     uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(few_smem_raw) + 1023) & ~uintptr_t(1023));
     float* join = reinterpret_cast<float*>(smem + L::kJoinOffset);
@@ -111,7 +122,7 @@ cache_attention_few_kernel(const __grid_constant__ CUtensorMap map_k, const __gr
         tma_prefetch_desc(&map_v);
     }
     grid_dependency_wait();
-    attn_prefix<kFewRows, kFewTokens>(p, prefix, misc);
+    attn_prefix<kRows, kFewTokens>(p, prefix, misc);
     const int total = prefix[p.requests];
     const int chunk = attn_chunk(p, total, gridDim.x);
     const long long begin64 = (long long)blockIdx.x * chunk;
@@ -129,7 +140,7 @@ cache_attention_few_kernel(const __grid_constant__ CUtensorMap map_k, const __gr
         uint32_t phase = 0;
         bool ok = true;
         for (int u = begin; u < end && ok;) {
-            const AttnPiece s = attn_piece_at<kFewRows, kFewTokens>(p, prefix, u, end);
+            const AttnPiece s = attn_piece_at<kRows, kFewTokens>(p, prefix, u, end);
             u += max(1, s.tile1 - s.tile0);
             const int* table = p.table + (long long)s.r * p.table_stride;
             // Lane i holds page `base + i` of the request: block number and scales, fetched 32 pages at a time and one
@@ -196,27 +207,30 @@ cache_attention_few_kernel(const __grid_constant__ CUtensorMap map_k, const __gr
         grid_launch_dependents();
     } else {
         // ------------------------------------------------------------------ computing warps
-        const int g = lane >> 2, c = lane & 3;         // row g and g + 8 of the tile; column pair of an instruction
+        // g: a token (and the one 8 behind it) or a band of dims, and the query row whose B operand the lane has;
+        // rows 2c, 2c + 1 of each n8 tile are the ones whose scores, statistics and output it has
+        const int g = lane >> 2, c = lane & 3;
         int stage = 0;
         uint32_t phase = 0;
         bool ok = true;
         for (int u = begin; u < end && ok;) {
-            const AttnPiece s = attn_piece_at<kFewRows, kFewTokens>(p, prefix, u, end);
+            const AttnPiece s = attn_piece_at<kRows, kFewTokens>(p, prefix, u, end);
             const int u_next = u + max(1, s.tile1 - s.tile0);
-            // ---- queries of this lane's two rows, as half
-            uint32_t qf[kSteps][4];
-            float c_row[2];
-            int see_lo[2], see_hi[2];                  // tokens that the row sees
             const int off = s.req.kv - s.req.qlen;
+            auto see = [&](int row, int& lo, int& hi) {            // tokens that a row of the tile sees
+                const int i = row / p.group;
+                hi = row < s.rows ? (p.causal ? min(s.req.kv, off + i + 1) : s.req.kv) : 0;
+                lo = p.window > 0 ? max(0, off + i - p.window + 1) : 0;
+            };
+            // ---- queries: the B operand of row g of each tile, as half
+            uint32_t qf[kTiles][kSteps][2];
+            float factor[kTiles][2];                   // of the scores of rows 2c, 2c + 1
 #pragma unroll
-            for (int e = 0; e < 2; ++e) {
-                const int row = s.row0 + g + 8 * e;
+            for (int n = 0; n < kTiles; ++n) {
+                const int row = s.row0 + 8 * n + g;
                 const bool there = row < s.rows;
                 const int i = there ? row / p.group : 0;
                 const int head = s.head * p.group + (there ? row - i * p.group : 0);
-                const int pos = off + i;
-                see_hi[e] = there ? (p.causal ? min(s.req.kv, pos + 1) : s.req.kv) : 0;
-                see_lo[e] = p.window > 0 ? max(0, pos - p.window + 1) : 0;
                 const uint16_t* src = static_cast<const uint16_t*>(p.q) + (long long)(s.req.q0 + i) * p.q_token_stride +
                                       (long long)head * p.q_head_stride;
                 uint4 w[kSteps / 2];                   // 16 dims (two loads) for every four steps
@@ -225,8 +239,7 @@ cache_attention_few_kernel(const __grid_constant__ CUtensorMap map_k, const __gr
                     const int dim = kDim == 128 ? (2 * c + (k >> 1)) * 16 + (k & 1) * 8 : c * 16 + k * 8;
                     w[k] = there ? *reinterpret_cast<const uint4*>(src + dim) : make_uint4(0, 0, 0, 0);
                 }
-                float mul = 1.0f;
-                int shift = 0;
+                float mul = 1.0f, back = 1.0f;
                 if constexpr (kBf16) {
                     float amax = 0.0f;
 #pragma unroll
@@ -241,10 +254,13 @@ cache_attention_few_kernel(const __grid_constant__ CUtensorMap map_k, const __gr
                     }
                     amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, 1));
                     amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, 2));
-                    shift = query_shift(amax);
+                    const int shift = query_shift(amax);
                     mul = pow2i(shift);
+                    back = pow2i(-shift);
                 }
-                c_row[e] = pow2i(-shift);
+                // row r's factor is with the lanes of g = r
+                factor[n][0] = __shfl_sync(0xffffffffu, back, 8 * c);
+                factor[n][1] = __shfl_sync(0xffffffffu, back, 8 * c + 4);
 #pragma unroll
                 for (int k = 0; k < kSteps / 2; ++k) {
                     const uint32_t* x = &w[k].x;
@@ -253,19 +269,27 @@ cache_attention_few_kernel(const __grid_constant__ CUtensorMap map_k, const __gr
                         uint32_t v = x[h];
                         if constexpr (kBf16)
                             v = pack_f16(__uint_as_float(v << 16) * mul, __uint_as_float(v & 0xFFFF0000u) * mul);
-                        qf[2 * k + (h >> 1)][(h & 1) * 2 + e] = v;    // words 0, 1: step 2k; words 2, 3: step 2k + 1
+                        qf[n][2 * k + (h >> 1)][h & 1] = v;        // words 0, 1: step 2k; words 2, 3: step 2k + 1
                     }
                 }
             }
             // every row of the tile sees the tokens [all_lo, all_hi)
-            const int i_first = s.row0 / p.group, i_last = (min(s.rows, s.row0 + kFewRows) - 1) / p.group;
+            const int i_first = s.row0 / p.group, i_last = (min(s.rows, s.row0 + kRows) - 1) / p.group;
             const int all_hi = p.causal ? min(s.req.kv, off + i_first + 1) : s.req.kv;
             const int all_lo = p.window > 0 ? max(0, off + i_last - p.window + 1) : 0;
 
-            float o[kTiles][4];
+            float o[kTiles][kBands][4];
 #pragma unroll
-            for (int j = 0; j < kTiles; ++j) o[j][0] = o[j][1] = o[j][2] = o[j][3] = 0.0f;
-            float m[2] = {-INFINITY, -INFINITY}, l[2] = {0.0f, 0.0f};
+            for (int n = 0; n < kTiles; ++n) {
+#pragma unroll
+                for (int j = 0; j < kBands; ++j) o[n][j][0] = o[n][j][1] = o[n][j][2] = o[n][j][3] = 0.0f;
+            }
+            float m[kTiles][2], l[kTiles][2];
+#pragma unroll
+            for (int n = 0; n < kTiles; ++n) {
+                m[n][0] = m[n][1] = -INFINITY;
+                l[n][0] = l[n][1] = 0.0f;
+            }
 
             for (int t = s.tile0; t < s.tile1; ++t) {
                 ok = mbar_wait(&full[stage], phase, abort_flag, p.status, DEV_TIMEOUT_SMEM_FULL);
@@ -276,27 +300,26 @@ cache_attention_few_kernel(const __grid_constant__ CUtensorMap map_k, const __gr
                 const uint8_t* kt = smem + stage * L::kStageBytes;
                 const uint8_t* vt = kt + L::kTileBytes;
                 if (mt.y != -INFINITY) {               // same for the whole warp
-                    // ---- scores: two n8 tiles of eight tokens
-                    float sc[2][4];
+                    // ---- scores of tokens g, g + 8 and rows 2c, 2c + 1, 16 codes of a token at a time
+                    float sc[kTiles][4];
 #pragma unroll
-                    for (int n = 0; n < 2; ++n) {
-                        sc[n][0] = sc[n][1] = sc[n][2] = sc[n][3] = 0.0f;
-                        const int row = warp * 16 + n * 8 + g;
-                        if constexpr (kDim == 128) {
+                    for (int n = 0; n < kTiles; ++n) sc[n][0] = sc[n][1] = sc[n][2] = sc[n][3] = 0.0f;
 #pragma unroll
-                            for (int i = 0; i < 2; ++i) {
-                                const uint4 w = *reinterpret_cast<const uint4*>(kt + row * 128 + (((2 * c + i) ^ (row & 7)) << 4));
-                                mma_f16(sc[n], qf[4 * i + 0], codes_lo(w.x), codes_hi(w.x));
-                                mma_f16(sc[n], qf[4 * i + 1], codes_lo(w.y), codes_hi(w.y));
-                                mma_f16(sc[n], qf[4 * i + 2], codes_lo(w.z), codes_hi(w.z));
-                                mma_f16(sc[n], qf[4 * i + 3], codes_lo(w.w), codes_hi(w.w));
-                            }
-                        } else {
-                            const uint4 w = *reinterpret_cast<const uint4*>(kt + row * 64 + ((c ^ ((row >> 1) & 3)) << 4));
-                            mma_f16(sc[n], qf[0], codes_lo(w.x), codes_hi(w.x));
-                            mma_f16(sc[n], qf[1], codes_lo(w.y), codes_hi(w.y));
-                            mma_f16(sc[n], qf[2], codes_lo(w.z), codes_hi(w.z));
-                            mma_f16(sc[n], qf[3], codes_lo(w.w), codes_hi(w.w));
+                    for (int i = 0; i < kDim / 64; ++i) {
+                        uint4 w[2];
+#pragma unroll
+                        for (int h = 0; h < 2; ++h) {
+                            const int row = warp * 16 + h * 8 + g;
+                            w[h] = kDim == 128
+                                ? *reinterpret_cast<const uint4*>(kt + row * 128 + (((2 * c + i) ^ (row & 7)) << 4))
+                                : *reinterpret_cast<const uint4*>(kt + row * 64 + ((c ^ ((row >> 1) & 3)) << 4));
+                        }
+#pragma unroll
+                        for (int j = 0; j < 4; ++j) {
+                            const uint32_t w0 = (&w[0].x)[j], w1 = (&w[1].x)[j];
+                            const uint32_t a[4] = {codes_lo(w0), codes_lo(w1), codes_hi(w0), codes_hi(w1)};
+#pragma unroll
+                            for (int n = 0; n < kTiles; ++n) mma_f16(sc[n], a, qf[n][4 * i + j][0], qf[n][4 * i + j][1]);
                         }
                     }
                     // ---- V codes of the tokens 2c, 2c + 1, 2c + 8, 2c + 9, dims [g * kDim / 8, (g + 1) * kDim / 8)
@@ -312,32 +335,36 @@ cache_attention_few_kernel(const __grid_constant__ CUtensorMap map_k, const __gr
                             wv[k][0] = w.x; wv[k][1] = w.y;
                         }
                     }
+                    // band j is dims 2j (instruction rows 0..7) and 2j + 1 (rows 8..15) of every lane's dims
+                    auto band = [&](const uint32_t (&w)[4][kDim / 32], int j, uint32_t (&a)[4]) {
+                        const int i = j >> 1, sel = (j & 1) ? 0x7362 : 0x5140;
+                        const uint32_t x = __byte_perm(w[0][i], w[1][i], sel), y = __byte_perm(w[2][i], w[3][i], sel);
+                        a[0] = codes_lo(x); a[1] = codes_hi(x); a[2] = codes_lo(y); a[3] = codes_hi(y);
+                    };
                     // ---- softmax
-                    const float c0 = c_row[0] * mt.x, c1 = c_row[1] * mt.x;
                     const bool masked = tok0 < all_lo || tok0 + 16 > all_hi;
-                    float tt[2][4];
 #pragma unroll
-                    for (int n = 0; n < 2; ++n) {
-#pragma unroll
-                        for (int e = 0; e < 4; ++e) tt[n][e] = fmaf(sc[n][e], e < 2 ? c0 : c1, mt.y);
+                    for (int n = 0; n < kTiles; ++n) {
+                        const float f0 = factor[n][0] * mt.x, f1 = factor[n][1] * mt.x;
+                        sc[n][0] = fmaf(sc[n][0], f0, mt.y);
+                        sc[n][1] = fmaf(sc[n][1], f1, mt.y);
+                        sc[n][2] = fmaf(sc[n][2], f0, mt.y);
+                        sc[n][3] = fmaf(sc[n][3], f1, mt.y);
                     }
                     if (masked) {
-                        uint32_t pm[4];                // 1 where the row sees the token, in the layout of P
 #pragma unroll
-                        for (int n = 0; n < 2; ++n) {
+                        for (int n = 0; n < kTiles; ++n) {
 #pragma unroll
                             for (int e = 0; e < 2; ++e) {
-                                const int tok = tok0 + n * 8 + 2 * c;
-                                const bool s0 = tok >= see_lo[e] && tok < see_hi[e];
-                                const bool s1 = tok + 1 >= see_lo[e] && tok + 1 < see_hi[e];
-                                if (!s0) tt[n][2 * e] = -INFINITY;
-                                if (!s1) tt[n][2 * e + 1] = -INFINITY;
-                                pm[2 * n + e] = (s0 ? 0x3C00u : 0u) | (s1 ? 0x3C000000u : 0u);
+                                int lo, hi;
+                                see(s.row0 + 8 * n + 2 * c + e, lo, hi);
+                                if (tok0 + g < lo || tok0 + g >= hi) sc[n][e] = -INFINITY;
+                                if (tok0 + g + 8 < lo || tok0 + g + 8 >= hi) sc[n][2 + e] = -INFINITY;
                             }
                         }
                         // codes of tokens outside the item do not count; NaN codes of tokens that some rows see and
                         // others do not are taken out of the product, and the rows that see them are given their NaN
-                        // by a product of ones: seen x is-NaN
+                        // by a product of ones: is-NaN x seen
                         bool any = false;
 #pragma unroll
                         for (int k = 0; k < 4; ++k) {
@@ -360,64 +387,69 @@ cache_attention_few_kernel(const __grid_constant__ CUtensorMap map_k, const __gr
                                 }
                             }
 #pragma unroll
-                            for (int j = 0; j < kTiles; j += 2) {
-                                const int i = j >> 2, sel = (j & 2) ? 0x7362 : 0x5140;
-                                const uint32_t x = __byte_perm(wn[0][i], wn[1][i], sel), y = __byte_perm(wn[2][i], wn[3][i], sel);
-                                float d0[4] = {0.f, 0.f, 0.f, 0.f}, d1[4] = {0.f, 0.f, 0.f, 0.f};
-                                mma_f16(d0, pm, codes_lo(x), codes_lo(y));
-                                mma_f16(d1, pm, codes_hi(x), codes_hi(y));
+                            for (int n = 0; n < kTiles; ++n) {
+                                int lo, hi;
+                                see(s.row0 + 8 * n + g, lo, hi);
+                                uint32_t ones[2];
 #pragma unroll
-                                for (int e = 0; e < 4; ++e) {
-                                    if (d0[e] > 0.0f) o[j][e] = NAN;
-                                    if (d1[e] > 0.0f) o[j + 1][e] = NAN;
+                                for (int k = 0; k < 2; ++k) {
+                                    const int tok = tok0 + 2 * c + 8 * k;
+                                    ones[k] = (tok >= lo && tok < hi ? 0x3C00u : 0u) | (tok + 1 >= lo && tok + 1 < hi ? 0x3C000000u : 0u);
+                                }
+#pragma unroll
+                                for (int j = 0; j < kBands; ++j) {
+                                    uint32_t a[4];
+                                    band(wn, j, a);
+                                    float d[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+                                    mma_f16(d, a, ones[0], ones[1]);
+#pragma unroll
+                                    for (int e = 0; e < 4; ++e)
+                                        if (d[e] > 0.0f) o[n][j][e] = NAN;
                                 }
                             }
                         }
                     }
-                    float mx[2];
+                    uint32_t pf[kTiles][2];
 #pragma unroll
-                    for (int e = 0; e < 2; ++e) {
-                        mx[e] = fmaxf(fmaxf(tt[0][2 * e], tt[0][2 * e + 1]), fmaxf(tt[1][2 * e], tt[1][2 * e + 1]));
-                        mx[e] = fmaxf(mx[e], __shfl_xor_sync(0xffffffffu, mx[e], 1));
-                        mx[e] = fmaxf(mx[e], __shfl_xor_sync(0xffffffffu, mx[e], 2));
-                        mx[e] = fmaxf(m[e], mx[e] - kProbShift);
-                    }
-                    if (__any_sync(0xffffffffu, mx[0] > m[0] || mx[1] > m[1])) {
-                        float al[2];
+                    for (int n = 0; n < kTiles; ++n) {
+                        float mx[2];
 #pragma unroll
                         for (int e = 0; e < 2; ++e) {
-                            al[e] = m[e] == -INFINITY ? 0.0f : ex2(m[e] - mx[e]);
-                            if (m[e] == mx[e]) al[e] = 1.0f;
-                            m[e] = mx[e];
-                            l[e] *= al[e];
+                            mx[e] = fmaxf(sc[n][e], sc[n][2 + e]);
+                            mx[e] = fmaxf(mx[e], __shfl_xor_sync(0xffffffffu, mx[e], 4));
+                            mx[e] = fmaxf(mx[e], __shfl_xor_sync(0xffffffffu, mx[e], 8));
+                            mx[e] = fmaxf(mx[e], __shfl_xor_sync(0xffffffffu, mx[e], 16));
+                            mx[e] = fmaxf(m[n][e], mx[e] - kProbShift);
                         }
+                        if (__any_sync(0xffffffffu, mx[0] > m[n][0] || mx[1] > m[n][1])) {
+                            float al[2];
 #pragma unroll
-                        for (int j = 0; j < kTiles; ++j) {
-                            o[j][0] *= al[0]; o[j][1] *= al[0];
-                            o[j][2] *= al[1]; o[j][3] *= al[1];
+                            for (int e = 0; e < 2; ++e) {
+                                al[e] = m[n][e] == mx[e] ? 1.0f : (m[n][e] == -INFINITY ? 0.0f : ex2(m[n][e] - mx[e]));
+                                m[n][e] = mx[e];
+                                l[n][e] *= al[e];
+                            }
+#pragma unroll
+                            for (int j = 0; j < kBands; ++j) {
+                                o[n][j][0] *= al[0]; o[n][j][1] *= al[1];
+                                o[n][j][2] *= al[0]; o[n][j][3] *= al[1];
+                            }
                         }
+                        const float ms0 = m[n][0] == -INFINITY ? 0.0f : m[n][0], ms1 = m[n][1] == -INFINITY ? 0.0f : m[n][1];
+                        const float p0 = ex2(sc[n][0] - ms0), p1 = ex2(sc[n][1] - ms1);
+                        const float p2 = ex2(sc[n][2] - ms0), p3 = ex2(sc[n][3] - ms1);
+                        l[n][0] = fmaf(p0 + p2, mt.z, l[n][0]);
+                        l[n][1] = fmaf(p1 + p3, mt.z, l[n][1]);
+                        pf[n][0] = transpose8x8(pack_f16(p0, p1));
+                        pf[n][1] = transpose8x8(pack_f16(p2, p3));
                     }
-                    const float ms0 = m[0] == -INFINITY ? 0.0f : m[0], ms1 = m[1] == -INFINITY ? 0.0f : m[1];
-                    uint32_t pf[4];
-                    float sum0 = 0.0f, sum1 = 0.0f;
+                    // ---- V^T P^T
 #pragma unroll
-                    for (int n = 0; n < 2; ++n) {
-                        const float p0 = ex2(tt[n][0] - ms0), p1 = ex2(tt[n][1] - ms0);
-                        const float p2 = ex2(tt[n][2] - ms1), p3 = ex2(tt[n][3] - ms1);
-                        sum0 += p0 + p1;
-                        sum1 += p2 + p3;
-                        pf[2 * n] = pack_f16(p0, p1);
-                        pf[2 * n + 1] = pack_f16(p2, p3);
-                    }
-                    l[0] = fmaf(sum0, mt.z, l[0]);
-                    l[1] = fmaf(sum1, mt.z, l[1]);
-                    // ---- P V: tile j holds dims 16g + j (64-wide heads: 8g + j) in column g
+                    for (int j = 0; j < kBands; ++j) {
+                        uint32_t a[4];
+                        band(wv, j, a);
 #pragma unroll
-                    for (int j = 0; j < kTiles; j += 2) {
-                        const int i = j >> 2, sel = (j & 2) ? 0x7362 : 0x5140;
-                        const uint32_t x = __byte_perm(wv[0][i], wv[1][i], sel), y = __byte_perm(wv[2][i], wv[3][i], sel);
-                        mma_f16(o[j], pf, codes_lo(x), codes_lo(y));
-                        mma_f16(o[j + 1], pf, codes_hi(x), codes_hi(y));
+                        for (int n = 0; n < kTiles; ++n) mma_f16(o[n][j], a, pf[n][0], pf[n][1]);
                     }
                 }
                 __syncwarp();
@@ -425,56 +457,49 @@ cache_attention_few_kernel(const __grid_constant__ CUtensorMap map_k, const __gr
                 if (++stage == kFewStages) { stage = 0; phase ^= 1; }
             }
             if (!ok) break;
-            // ---- join the four warps
+            // ---- join the four warps: this lane has rows 2c, 2c + 1, dims [g * kLaneDims, (g + 1) * kLaneDims)
 #pragma unroll
-            for (int e = 0; e < 2; ++e) {
-                l[e] += __shfl_xor_sync(0xffffffffu, l[e], 1);
-                l[e] += __shfl_xor_sync(0xffffffffu, l[e], 2);
-                const int row = g + 8 * e;
-                if (c == 0) {
-                    ml[(warp * kFewRows + row) * 2] = m[e];
-                    ml[(warp * kFewRows + row) * 2 + 1] = l[e];
-                }
-                // column n of tile j is dim n * kTiles + j: this lane has the kDim / 4 consecutive dims behind 2c * kTiles
-                float* dst = join + (warp * kFewRows + row) * L::kPitch + 2 * c * kTiles;
+            for (int n = 0; n < kTiles; ++n) {
 #pragma unroll
-                for (int k = 0; k < kDim / 16; ++k) {
-                    const int j = 4 * (k % (kTiles / 4)), hi = k / (kTiles / 4);
-                    *reinterpret_cast<float4*>(dst + hi * kTiles + j) =
-                        make_float4(o[j][2 * e + hi], o[j + 1][2 * e + hi], o[j + 2][2 * e + hi], o[j + 3][2 * e + hi]);
+                for (int e = 0; e < 2; ++e) {
+                    float sum = l[n][e];
+                    sum += __shfl_xor_sync(0xffffffffu, sum, 4);
+                    sum += __shfl_xor_sync(0xffffffffu, sum, 8);
+                    sum += __shfl_xor_sync(0xffffffffu, sum, 16);
+                    const int row = 8 * n + 2 * c + e;
+                    if (g == 0) *reinterpret_cast<float2*>(ml + (warp * kFewRows + row) * 2) = make_float2(m[n][e], sum);
+                    // (in an order that keeps lanes of different g on different banks)
+                    float* dst = join + (warp * kFewRows + row) * L::kPitch + g * kLaneDims;
+#pragma unroll
+                    for (int k = 0; k < kLaneDims; k += 4)
+                        *reinterpret_cast<float4*>(dst + k) = make_float4(o[n][k / 2][e], o[n][k / 2][2 + e], o[n][k / 2 + 1][e], o[n][k / 2 + 1][2 + e]);
                 }
             }
             compute_sync();
             {
-                constexpr int kPer = kDim / 8;         // dims of this thread, eight threads a row
+                constexpr int kPer = kDim * kRows / (32 * kFewWarps);       // dims of this thread
+                constexpr int kPerRow = kDim / kPer;                        // threads of a row
                 const int tid = threadIdx.x;           // the computing warps are the block's first
-                const int row = tid >> 3, d0 = (tid & 7) * kPer;
-                float mm = -INFINITY;
+                const int row = tid / kPerRow, d0 = (tid % kPerRow) * kPer;
+                float mm = -INFINITY, ll = 0.0f, acc[kPer];
 #pragma unroll
                 for (int w = 0; w < kFewWarps; ++w) mm = fmaxf(mm, ml[(w * kFewRows + row) * 2]);
-                float acc[kPer];
 #pragma unroll
                 for (int k = 0; k < kPer; ++k) acc[k] = 0.0f;
-                float ll = 0.0f;
 #pragma unroll
                 for (int w = 0; w < kFewWarps; ++w) {
-                    const float mw = ml[(w * kFewRows + row) * 2];
-                    if (mw == -INFINITY) {
-                        // saw nothing: no part in the sum, but a NaN (a score that is one leaves the maximum alone)
-                        const float lw = ml[(w * kFewRows + row) * 2 + 1];
-                        if (lw != lw) ll = lw;
-                        continue;
-                    }
-                    const float wt = ex2(mw - mm);
-                    ll = fmaf(wt, ml[(w * kFewRows + row) * 2 + 1], ll);
+                    const float2 v = *reinterpret_cast<const float2*>(ml + (w * kFewRows + row) * 2);
+                    const float wt = v.x == -INFINITY ? 0.0f : ex2(v.x - mm);
+                    ll += wt * v.y;                    // (0 * NaN for a warp all of whose scores are NaN: so is the row)
+                    if (wt == 0.0f) continue;
                     const float* src = join + (w * kFewRows + row) * L::kPitch + d0;
 #pragma unroll
                     for (int k = 0; k < kPer; k += 4) {
-                        const float4 v = *reinterpret_cast<const float4*>(src + k);
-                        acc[k] = fmaf(wt, v.x, acc[k]);
-                        acc[k + 1] = fmaf(wt, v.y, acc[k + 1]);
-                        acc[k + 2] = fmaf(wt, v.z, acc[k + 2]);
-                        acc[k + 3] = fmaf(wt, v.w, acc[k + 3]);
+                        const float4 x = *reinterpret_cast<const float4*>(src + k);
+                        acc[k] = fmaf(wt, x.x, acc[k]);
+                        acc[k + 1] = fmaf(wt, x.y, acc[k + 1]);
+                        acc[k + 2] = fmaf(wt, x.z, acc[k + 2]);
+                        acc[k + 3] = fmaf(wt, x.w, acc[k + 3]);
                     }
                 }
                 const int prow = s.row0 + row;
@@ -487,25 +512,20 @@ cache_attention_few_kernel(const __grid_constant__ CUtensorMap map_k, const __gr
                         uint16_t* dst = static_cast<uint16_t*>(p.out) + (long long)(s.req.q0 + i) * p.out_token_stride +
                                         (long long)head * p.out_head_stride + d0;
 #pragma unroll
-                        for (int k = 0; k < kPer; k += 8) {
-                            uint4 w;
-                            w.x = pack_out<kBf16>(acc[k] * inv, acc[k + 1] * inv);
-                            w.y = pack_out<kBf16>(acc[k + 2] * inv, acc[k + 3] * inv);
-                            w.z = pack_out<kBf16>(acc[k + 4] * inv, acc[k + 5] * inv);
-                            w.w = pack_out<kBf16>(acc[k + 6] * inv, acc[k + 7] * inv);
-                            *reinterpret_cast<uint4*>(dst + k) = w;
-                        }
-                        if (p.lse && (tid & 7) == 0)
+                        for (int k = 0; k < kPer; k += 4)
+                            *reinterpret_cast<uint2*>(dst + k) = make_uint2(pack_out<kBf16>(acc[k] * inv, acc[k + 1] * inv),
+                                                                            pack_out<kBf16>(acc[k + 2] * inv, acc[k + 3] * inv));
+                        if (p.lse && tid % kPerRow == 0)
                             p.lse[(long long)(s.req.q0 + i) * p.heads + head] =
                                 ll != 0.0f ? (mm + lg2(ll)) * 0.6931471805599453f : -INFINITY;
                     } else {
                         const long long slot = (long long)blockIdx.x * 2 + (u == begin ? 0 : 1);
-                        float* dst = p.part_out + (slot * kFewRows + row) * kDim + d0;
+                        float* dst = p.part_out + (slot * kRows + row) * kDim + d0;
 #pragma unroll
                         for (int k = 0; k < kPer; k += 4)
                             *reinterpret_cast<float4*>(dst + k) = make_float4(acc[k], acc[k + 1], acc[k + 2], acc[k + 3]);
-                        if ((tid & 7) == 0)
-                            *reinterpret_cast<float2*>(p.part_ml + (slot * kFewRows + row) * 2) = make_float2(mm, ll);
+                        if (tid % kPerRow == 0)
+                            *reinterpret_cast<float2*>(p.part_ml + (slot * kRows + row) * 2) = make_float2(mm, ll);
                     }
                 }
             }
@@ -524,11 +544,11 @@ cache_attention_few_kernel(const __grid_constant__ CUtensorMap map_k, const __gr
 
 // Joins the pieces of the items that are cut by a chunk's border: out = sum_b w_b O_b / sum_b w_b l_b with w_b = 2^(m_b -
 // max m), in the order of the blocks.  Block `which` takes the item that the end of that block's chunk cuts, unless the
-// item was cut before; a row tile is shared by kRows / 16 blocks, whose warps take rows.  Bound by latency: the
+// item was cut before; a large row tile is shared by kRows / 16 blocks, whose warps take rows.  Bound by latency: the
 // statistics of 32 pieces are read at once by a warp's lanes, then four pieces of output are in flight.
 template <int kRows, int kDim, bool kBf16>
 __global__ void __launch_bounds__(256) cache_attention_join_kernel(const CacheAttentionParams p) {
-    constexpr int kGroups = kRows / 16;
+    constexpr int kGroups = kRows > 16 ? kRows / 16 : 1;
     constexpr int kPer = kDim / 32;
     grid_launch_dependents();
     grid_dependency_wait();
@@ -536,7 +556,7 @@ __global__ void __launch_bounds__(256) cache_attention_join_kernel(const CacheAt
     const AttnCut s = p.cuts[which];
     if (s.first != which) return;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    const int rows = min((group + 1) * 16, s.rows - s.row0);
+    const int rows = min(min((group + 1) * 16, kRows), s.rows - s.row0);
     const int pieces = s.last - s.first + 1;
     // slot 0 of a block is the piece at the start of its chunk, slot 1 one that starts inside it
     auto slot_of = [&](int b) -> long long { return (long long)(s.first + b) * 2 + (b == 0 ? s.inside : 0); };
@@ -670,22 +690,36 @@ static int plan_attention(const blazeKvCache* c, const blazeCacheAttentionArgs* 
     return ACLTENSOR_STATUS_SUCCESS;
 }
 
+template <int kDim, bool kBf16, int kTiles>
+static cudaError_t launch_few(const CUtensorMap& mk, const CUtensorMap& mv, const CacheAttentionParams& p, int grid,
+                              cudaStream_t stream) {
+    auto few = cache_attention_few_kernel<kDim, kBf16, kTiles>;
+    static bool done[64] = {};
+    int dev = 0;
+    cudaGetDevice(&dev);
+    if (!done[dev & 63]) {
+        static_assert(1024 + FewSmem<kDim>::kPrefixOffset + (kAttnMaxRequests + 1) * 4 <= 227 * 1024, "shared memory");
+        const cudaError_t e = cudaFuncSetAttribute(few, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                                   FewSmem<kDim>::bytes(kAttnMaxRequests));
+        if (e != cudaSuccess) return e;
+        done[dev & 63] = true;
+    }
+    const cudaError_t e = launch_after_prepass(few, grid, kFewThreads, (size_t)FewSmem<kDim>::bytes(p.requests), stream, mk, mv, p);
+    if (e != cudaSuccess || grid < 2) return e;
+    return launch_after_prepass(cache_attention_join_kernel<8 * kTiles, kDim, kBf16>, grid - 1, 256, 0, stream, p);
+}
+
 template <int kDim, bool kBf16>
 static cudaError_t launch_attention(const CUtensorMap& mk, const CUtensorMap& mv, CacheAttentionParams p, const CacheView& cv,
                                     const AttnPlan& pl, uint8_t* ws, cudaStream_t stream) {
-    auto few = cache_attention_few_kernel<kDim, kBf16>;
     auto many = cache_attention_many_kernel<kDim, kBf16>;
     static bool done[64] = {};
     int dev = 0;
     cudaGetDevice(&dev);
     if (!done[dev & 63]) {
-        static_assert(1024 + FewSmem<kDim>::kPrefixOffset + (kAttnMaxRequests + 1) * 4 <= 227 * 1024 &&
-                      1024 + ManySmem<kDim>::kPrefixOffset + (kAttnMaxRequests + 1) * 4 <= 227 * 1024, "shared memory");
-        cudaError_t e = cudaFuncSetAttribute(few, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                             FewSmem<kDim>::bytes(kAttnMaxRequests));
-        if (e == cudaSuccess)
-            e = cudaFuncSetAttribute(many, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                     ManySmem<kDim>::bytes(kAttnMaxRequests));
+        static_assert(1024 + ManySmem<kDim>::kPrefixOffset + (kAttnMaxRequests + 1) * 4 <= 227 * 1024, "shared memory");
+        const cudaError_t e = cudaFuncSetAttribute(many, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                                   ManySmem<kDim>::bytes(kAttnMaxRequests));
         if (e != cudaSuccess) return e;
         done[dev & 63] = true;
     }
@@ -698,9 +732,9 @@ static cudaError_t launch_attention(const CUtensorMap& mk, const CUtensorMap& mv
         p.part_out = reinterpret_cast<float*>(ws);
         p.part_ml = reinterpret_cast<float*>(ws + pl.few_ml);
         p.cuts = reinterpret_cast<AttnCut*>(ws + pl.few_cuts);
-        e = launch_after_prepass(few, pl.few_grid, kFewThreads, (size_t)FewSmem<kDim>::bytes(p.requests), stream, mk, mv, p);
-        if (e == cudaSuccess && pl.few_grid > 1)
-            e = launch_after_prepass(cache_attention_join_kernel<kFewRows, kDim, kBf16>, pl.few_grid - 1, 256, 0, stream, p);
+        // a second n8 tile of query rows only where a request may need it
+        e = (long long)p.max_q * p.group <= 8 ? launch_few<kDim, kBf16, 1>(mk, mv, p, pl.few_grid, stream)
+                                              : launch_few<kDim, kBf16, 2>(mk, mv, p, pl.few_grid, stream);
         if (e != cudaSuccess) return e;
     }
     if (pl.many) {

@@ -42,6 +42,7 @@ constexpr int kFewLimit = kFewRows;
 
 template <int kDim>
 struct FewSmem {
+    static constexpr int kBlocks = kDim == 64 ? 3 : 2;               // resident blocks of an SM
     static constexpr int kTileBytes = kFewTokens * kDim;             // of K, and of V
     static constexpr int kStageBytes = 2 * kTileBytes;
     static constexpr int kPitch = kDim + 4;                          // floats of a row of a warp's output
@@ -91,7 +92,7 @@ __device__ __forceinline__ uint32_t transpose8x8(uint32_t x) {
 }
 
 template <int kDim, bool kBf16, int kTiles>
-__global__ void __launch_bounds__(kFewThreads, 2)
+__global__ void __launch_bounds__(kFewThreads, FewSmem<kDim>::kBlocks)
 cache_attention_few_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v,
                            const CacheAttentionParams p) {
     using L = FewSmem<kDim>;
@@ -672,7 +673,11 @@ static int plan_attention(const blazeKvCache* c, const blazeCacheAttentionArgs* 
         (pl->many && heads * (double)((rows + kManyRows - 1) / kManyRows) * (double)(a->max_kv / kManyTokens + 2) > 2.0e9))
         return ACLTENSOR_STATUS_NOT_SUPPORTED;
     if (a->sm_limit > 0 && a->sm_limit < sms) sms = a->sm_limit;
-    pl->few_grid = 2 * sms;
+    // (a long prefix over many requests may leave no room for the last block of an SM)
+    const int few_bytes = c->head_dim == 128 ? FewSmem<128>::bytes(a->requests) : FewSmem<64>::bytes(a->requests);
+    const int few_blocks = c->head_dim == 128 ? FewSmem<128>::kBlocks : FewSmem<64>::kBlocks;
+    const int fit = (228 * 1024) / (few_bytes + 1024);
+    pl->few_grid = (fit < few_blocks ? fit : few_blocks) * sms;
     pl->many_grid = sms;
     size_t at = 0;
     auto room = [&](int grid, int tile_rows, size_t* ml, size_t* cuts) {

@@ -7,6 +7,7 @@
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 #include <cuda_runtime.h>
+#include <type_traits>
 
 #include "cache.h"
 #include "cann_ops_tensor_types.h"
@@ -277,8 +278,21 @@ __device__ __forceinline__ uint32_t rescale4(uint32_t w, float ratio) {
     return cvt_e4m3x4_sat(f[0], f[1], f[2], f[3]);
 }
 
-// Eight 16-bit inputs -> eight codes under a scale: x * inv where 1 / scale is exact (`inv` not 0), else a division.
+// The magnitudes' maxima of the words' low and high halves, infinities and NaNs among them (they come out on top).
+__device__ __forceinline__ uint32_t max_any(uint32_t m, const uint4& v) {
+    m = __vmaxu2(m, v.x & 0x7FFF7FFFu);
+    m = __vmaxu2(m, v.y & 0x7FFF7FFFu);
+    m = __vmaxu2(m, v.z & 0x7FFF7FFFu);
+    return __vmaxu2(m, v.w & 0x7FFF7FFFu);
+}
 template <bool kBf16>
+__device__ __forceinline__ bool any_not_finite(uint32_t m) {
+    constexpr uint32_t kInf = kBf16 ? 0x7F80u : 0x7C00u;
+    return (m & 0xFFFFu) >= kInf || (m >> 16) >= kInf;
+}
+
+// Eight 16-bit inputs -> eight codes under a scale: x * inv where 1 / scale is exact, else a division.
+template <bool kBf16, bool kExact>
 __device__ __forceinline__ uint2 encode8(const uint4& v, float inv, float scale) {
     float f[8];
     unpack2<kBf16>(v.x, f[0], f[1]);
@@ -286,7 +300,7 @@ __device__ __forceinline__ uint2 encode8(const uint4& v, float inv, float scale)
     unpack2<kBf16>(v.z, f[4], f[5]);
     unpack2<kBf16>(v.w, f[6], f[7]);
 #pragma unroll
-    for (int i = 0; i < 8; ++i) f[i] = inv != 0.0f ? f[i] * inv : __fdiv_rn(f[i], scale);
+    for (int i = 0; i < 8; ++i) f[i] = kExact ? f[i] * inv : __fdiv_rn(f[i], scale);
     return make_uint2(cvt_e4m3x4_sat(f[0], f[1], f[2], f[3]), cvt_e4m3x4_sat(f[4], f[5], f[6], f[7]));
 }
 
@@ -298,7 +312,7 @@ __device__ __forceinline__ uint2 encode8(const uint4& v, float inv, float scale)
 constexpr int kStoreShort = 4;
 
 template <int kDim, bool kBf16>
-__global__ void __launch_bounds__(kStoreWarps * 32) cache_store_kernel(const CacheStoreParams p) {
+__global__ void __launch_bounds__(kStoreWarps * 32, 8) cache_store_kernel(const CacheStoreParams p) {
     constexpr int kLanesPerRow = kDim / 8;               // 16 bytes of input, 8 of codes per lane
     constexpr int kRowsPerLoad = 32 / kLanesPerRow;
     constexpr int kBatch = 8;
@@ -370,8 +384,20 @@ __global__ void __launch_bounds__(kStoreWarps * 32) cache_store_kernel(const Cac
 #pragma unroll
                 for (int j = 0; j < kBatch; ++j) v[j] = load(r + j * kRowsPerLoad + sub, b);
 #pragma unroll
-                for (int j = 0; j < kBatch; ++j)
-                    m = max_finite<kBf16>(max_finite<kBf16>(max_finite<kBf16>(max_finite<kBf16>(m, v[j].x), v[j].y), v[j].z), v[j].w);
+                for (int j = 0; j < kBatch; ++j) m = max_any(m, v[j]);
+            }
+            if (__any_sync(0xffffffffu, any_not_finite<kBf16>(m))) {
+                // rare: infinities and NaNs do not count
+                m = 0;
+                for (int r = r0 + sub; r < b; r += step) {
+#pragma unroll 1
+                    for (int j = 0; j < kBatch; ++j) {
+                        const uint4 w = load(r + j * kRowsPerLoad, b);
+                        m = max_finite<kBf16>(max_finite<kBf16>(max_finite<kBf16>(max_finite<kBf16>(m, w.x), w.y), w.z), w.w);
+                    }
+                }
+            } else {
+                m = max(m & 0xFFFFu, m >> 16);
             }
             m = __reduce_max_sync(0xffffffffu, m);
             float* scale_at = scales + block * p.cache.scale_stride;
@@ -401,19 +427,22 @@ __global__ void __launch_bounds__(kStoreWarps * 32) cache_store_kernel(const Cac
             }
             if (shared) {
                 // slots rise one by one: row r goes to slot low + r - a
-                for (int r = r0; r < b; r += step) {
-                    if (!kept) {
+                auto put = [&](auto exact) {
+                    for (int r = r0; r < b; r += step) {
+                        if (!kept) {
 #pragma unroll
-                        for (int j = 0; j < kBatch; ++j) v[j] = load(r + j * kRowsPerLoad + sub, b);
-                    }
+                            for (int j = 0; j < kBatch; ++j) v[j] = load(r + j * kRowsPerLoad + sub, b);
+                        }
+                        uint8_t* at = page + (long long)(low + r + sub - a) * p.cache.token_stride;
 #pragma unroll
-                    for (int j = 0; j < kBatch; ++j) {
-                        const int row = r + j * kRowsPerLoad + sub;
-                        if (row < b)
-                            *reinterpret_cast<uint2*>(page + (long long)(low + row - a) * p.cache.token_stride) =
-                                encode8<kBf16>(v[j], inv, scale);
+                        for (int j = 0; j < kBatch; ++j) {
+                            if (r + j * kRowsPerLoad + sub < b)
+                                *reinterpret_cast<uint2*>(at + (long long)(j * kRowsPerLoad) * p.cache.token_stride) =
+                                    encode8<kBf16, decltype(exact)::value>(v[j], inv, scale);
+                        }
                     }
-                }
+                };
+                if (pow2) put(std::true_type{}); else put(std::false_type{});
                 if (threadIdx.x == 0 && scale != old) *scale_at = scale;
             } else {
                 for (int r = r0; r < b; r += kRowsPerLoad) {
@@ -430,7 +459,7 @@ __global__ void __launch_bounds__(kStoreWarps * 32) cache_store_kernel(const Cac
                     }
                     if (last)
                         *reinterpret_cast<uint2*>(page + (long long)(slot & (p.cache.block_size - 1)) * p.cache.token_stride) =
-                            encode8<kBf16>(w, inv, scale);
+                            pow2 ? encode8<kBf16, true>(w, inv, scale) : encode8<kBf16, false>(w, inv, scale);
                     __syncwarp();                        // the next rows' stores come behind these
                 }
                 if (lane == 0 && scale != old) *scale_at = scale;

@@ -234,7 +234,7 @@ def test_store_foreign_scales(cuda_device):
 # ------------------------------------------------------------------------------------------------ attention
 
 def attention_case(device, seed, q_lens, kv_lens, heads, kv_heads, dim, bs, kind="bf16", causal=True, window=0, order="hnd",
-                   scale=None, pad=0, table=None, change=None, max_q=None, min_q=0, loud=1.0):
+                   scale=None, pad=0, table=None, change=None, max_q=None, min_q=0, loud=1.0, sm_limit=0):
     """Runs one call and holds it against the reference."""
     import torch
     rng = np.random.default_rng(seed)
@@ -276,10 +276,12 @@ def attention_case(device, seed, q_lens, kv_lens, heads, kv_heads, dim, bs, kind
         t.copy_(torch.from_numpy(c))
     out = torch.full(q_t.shape, 7.0, dtype=q_t.dtype, device=device)
     lse = torch.full(q_t.shape[:2], 7.0, dtype=torch.float32, device=device)
-    workspace = native.cache_attention_workspace(cache, q_t, requests=n, max_q=max_q or max(q_lens), max_kv=max(kv_lens))
+    workspace = native.cache_attention_workspace(cache, q_t, requests=n, max_q=max_q or max(q_lens), max_kv=max(kv_lens),
+                                                 sm_limit=sm_limit)
     workspace.fill_(0xFF)
     args = (cache, q_t, i32(offsets, device), i32(kv_lens, device), i32(tab, device))
-    kw = dict(scale=scale, max_q=max_q or max(q_lens), max_kv=max(kv_lens), min_q=min_q, causal=causal, window=window)
+    kw = dict(scale=scale, max_q=max_q or max(q_lens), max_kv=max(kv_lens), min_q=min_q, causal=causal, window=window,
+              sm_limit=sm_limit)
     native.cache_attention(*args, **kw, out=out, lse=lse, workspace=workspace)
     got, got_lse = out.double().cpu().numpy(), lse.double().cpu().numpy()
     qd = q_t.double().cpu().numpy()
@@ -300,7 +302,8 @@ def attention_case(device, seed, q_lens, kv_lens, heads, kv_heads, dim, bs, kind
     bad = inside[:, None, None] & ~((np.abs(got - want) <= bound) | (np.isnan(got) & np.isnan(want)))
     assert not bad.any(), (np.argwhere(bad)[:5], got[bad][:5], want[bad][:5])
     fin = np.isfinite(want_lse) & inside[:, None]
-    assert (np.abs(got_lse - want_lse)[fin] <= (err + 4 * 2.0 ** -23 * (np.abs(want_lse) + 30))[fin]).all()
+    off = np.abs(np.where(fin, got_lse, 0.0) - np.where(fin, want_lse, 0.0))
+    assert (off[fin] <= (err + 4 * 2.0 ** -23 * (np.abs(want_lse) + 30))[fin]).all()
     rest = inside[:, None] & ~np.isfinite(want_lse)
     assert np.array_equal(got_lse[rest], want_lse[rest], equal_nan=True)
     again = torch.full_like(out, 7.0)
@@ -348,6 +351,75 @@ def test_attention_long(cuda_device):
     attention_case(cuda_device, 8, [1, 1, 2], [9000, 3, 4100], 4, 1, 128, 64)
     attention_case(cuda_device, 9, [1], [20000], 2, 1, 64, 16, "f16")
     attention_case(cuda_device, 10, [40], [5000], 4, 1, 128, 128)
+
+
+@pytest.mark.parametrize("sm_limit", [1, 3, 40])
+def test_attention_on_a_share_of_the_sms(cuda_device, sm_limit):
+    """Other cuts of the work, down to blocks that each take many items and items in many blocks."""
+    attention_case(cuda_device, 51, [1, 1, 30, 2], [700, 3, 400, 64], 6, 2, 64, 16, "f16", sm_limit=sm_limit)
+    attention_case(cuda_device, 52, [70, 300], [900, 310], 4, 1, 128, 64, min_q=70, sm_limit=sm_limit)
+
+
+def test_attention_hints_are_only_hints(cuda_device):
+    """min_q above what the requests have, max_q and max_kv far above it."""
+    attention_case(cuda_device, 53, [1, 40, 3], [90, 60, 200], 8, 2, 64, 32, min_q=40)
+    attention_case(cuda_device, 54, [1, 2], [90, 60], 4, 2, 128, 32, max_q=500)
+
+
+def test_attention_many_requests(cuda_device):
+    """More requests than a block has threads, most of them empty or short."""
+    rng = np.random.default_rng(55)
+    q = rng.integers(0, 2, 1100).tolist()
+    kv = [int(x) for x in rng.integers(0, 40, 1100)]
+    attention_case(cuda_device, 55, q, kv, 1, 1, 64, 16)
+    q[17] = 150
+    attention_case(cuda_device, 56, q, kv, 1, 1, 64, 16, "f16")
+
+
+def test_offsets_beyond_32_bits(cuda_device):
+    """A cache of more than 2^32 bytes for K alone, its last blocks in use: store, decode step and prompt."""
+    import torch
+    bs, heads, dim = 128, 8, 128
+    blocks = (1 << 32) // (bs * heads * dim) + 40
+    k, v = (torch.empty((blocks, heads, bs, dim), dtype=torch.uint8, device=cuda_device) for _ in range(2))
+    ks, vs = (torch.ones((blocks, heads), dtype=torch.float32, device=cuda_device) for _ in range(2))
+    big = native.PagedCache(k, v, ks, vs)
+    small = native.PagedCache.empty(4, heads, bs, dim, cuda_device)
+    ids = [blocks - 1, blocks - 17, 3]
+    g = torch.Generator(device=cuda_device)
+    g.manual_seed(1)
+    rows = 300
+    x, y, q = (torch.randn((rows, heads, dim), generator=g, device=cuda_device).to(torch.bfloat16) for _ in range(3))
+    for cache, table in ((big, ids), (small, [2, 0, 1])):
+        slots = torch.tensor([table[t // bs] * bs + t % bs for t in range(rows)], dtype=torch.int64, device=cuda_device)
+        native.cache_store(cache, x, y, slots)
+    for n in (1, rows):
+        args = (q[:n], i32([0, n], cuda_device), i32([rows], cuda_device))
+        a = native.cache_attention(big, *args, i32([ids], cuda_device), max_q=n, max_kv=rows)
+        b = native.cache_attention(small, *args, i32([[2, 0, 1]], cuda_device), max_q=n, max_kv=rows)
+        assert torch.equal(a, b) and torch.isfinite(a.float()).all() and bool((a != 0).any())
+
+
+def test_other_streams_and_wide_strides(cuda_device):
+    """Inputs made on another stream than the call's, a block table and lengths inside larger tensors."""
+    import torch
+    rng = np.random.default_rng(57)
+    cache, _, _ = random_cache(rng, 20, 2, 16, 64, cuda_device)
+    q = torch.randn((6, 4, 64), device=cuda_device).to(torch.float16)
+    table = i32(rng.permutation(20)[:15].reshape(3, 5), cuda_device)
+    want = native.cache_attention(cache, q, i32([0, 1, 4, 6], cuda_device), i32([80, 50, 33], cuda_device), table, max_q=3, max_kv=80)
+    wide = i32(np.full((3, 9), -1), cuda_device)
+    wide[:, 2:7] = table
+    side = torch.cuda.Stream(cuda_device)
+    side.wait_stream(torch.cuda.current_stream(cuda_device))
+    with torch.cuda.stream(side):
+        qq = torch.zeros((6, 9, 72), dtype=torch.float16, device=cuda_device)
+        qq[:, 3:7, :64] = q
+        out = torch.full((6, 5, 64), 3.0, dtype=torch.float16, device=cuda_device)
+        native.cache_attention(cache, qq[:, 3:7, :64], i32([0, 1, 4, 6], cuda_device), i32([80, 50, 33], cuda_device),
+                               wide[:, 2:7], max_q=3, max_kv=80, out=out[:, 1:])
+    torch.cuda.current_stream(cuda_device).wait_stream(side)
+    assert torch.equal(out[:, 1:], want) and bool((out[:, 0] == 3.0).all())
 
 
 def test_attention_nan_where_it_is_not_seen(cuda_device):

@@ -369,7 +369,8 @@ BLAZE_API int blazeCacheStore(const blazeKvCache* cache, const blazeCacheStoreAr
  * (window == 0 or j > p - window).  Query head h reads kv head h / (heads / kv_heads).
  *   out[row][h] = sum_j softmax_j(scale * q . K_j) V_j,   lse[row][h] = ln sum_j exp(scale * q . K_j)
  * A row that sees nothing gives zeros and lse = -inf.  Nothing that a row does not see reaches its result, NaN codes
- * there and in the blocks' unused rows included.  Rows outside every request are left as they were.
+ * there and in the blocks' unused rows included.  Rows outside every request are left as they were.  out may not overlap
+ * q: a row of q is read by every block that has a part of its work.
  * A token whose block number is outside the cache counts as not seen and the device status word reports code 8.
  * Scores, softmax and sums are float32; probabilities are rounded to half (11 bits) for the product with V.
  * max_q and max_kv bound the requests' rows and kv_len (lengths above are cut to them; max_kv may not pass max_blocks *

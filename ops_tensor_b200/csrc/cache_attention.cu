@@ -723,8 +723,12 @@ static cudaError_t launch_attention(const CUtensorMap& mk, const CUtensorMap& mv
     cudaGetDevice(&dev);
     if (!done[dev & 63]) {
         static_assert(1024 + ManySmem<kDim>::kPrefixOffset + (kAttnMaxRequests + 1) * 4 <= 227 * 1024, "shared memory");
-        const cudaError_t e = cudaFuncSetAttribute(many, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                                   ManySmem<kDim>::bytes(kAttnMaxRequests));
+        // the kernel's warpgroups trade registers: the launch has to have all that they take
+        cudaFuncAttributes attr;
+        cudaError_t e = cudaFuncGetAttributes(&attr, many);
+        if (e == cudaSuccess && attr.numRegs < kManyLaunchRegs) e = cudaErrorInvalidConfiguration;
+        if (e == cudaSuccess)
+            e = cudaFuncSetAttribute(many, cudaFuncAttributeMaxDynamicSharedMemorySize, ManySmem<kDim>::bytes(kAttnMaxRequests));
         if (e != cudaSuccess) return e;
         done[dev & 63] = true;
     }
@@ -809,7 +813,7 @@ extern "C" int blazeCacheAttention(const blazeKvCache* cache, const blazeCacheAt
     p.max_q = a->max_q;
     p.max_kv = a->max_kv;
     p.causal = a->causal;
-    p.window = a->window;
+    p.window = a->window >= a->max_kv ? 0 : a->window;      // (wider than any request: none)
     p.scale_log2 = a->scale * 1.4426950408889634f;
     p.q = a->q;
     p.q_token_stride = a->q_token_stride;

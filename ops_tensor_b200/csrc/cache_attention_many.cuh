@@ -25,7 +25,8 @@ constexpr int kManyThreads = 32 * 16;      // warps 13-15 only complete the last
 // Registers of a thread of the softmax, converting and issuing warpgroups (a softmax thread holds 64 to 96 scores);
 // the launch has 128 each, 512 for the four.
 constexpr int kSoftmaxRegs = 176, kConvertRegs = 88, kIssueRegs = 72;
-static_assert(2 * kSoftmaxRegs + kConvertRegs + kIssueRegs <= 4 * 128, "setmaxnreg draws on what the launch has");
+constexpr int kManyLaunchRegs = 128;
+static_assert(2 * kSoftmaxRegs + kConvertRegs + kIssueRegs <= 4 * kManyLaunchRegs, "setmaxnreg draws on what the launch has");
 constexpr int kManyMeta = 4;              // tiles whose scales are held
 
 // A row's reference is set 2^3 below its largest score and kept until a score passes it by 2^15 (half ends at 2^16).

@@ -364,6 +364,9 @@ def test_attention_hints_are_only_hints(cuda_device):
     """min_q above what the requests have, max_q and max_kv far above it."""
     attention_case(cuda_device, 53, [1, 40, 3], [90, 60, 200], 8, 2, 64, 32, min_q=40)
     attention_case(cuda_device, 54, [1, 2], [90, 60], 4, 2, 128, 32, max_q=500)
+    # windows as wide as an int goes, of more rows than there are keys
+    attention_case(cuda_device, 58, [1, 30], [90, 7], 4, 2, 64, 32, window=(1 << 31) - 1)
+    attention_case(cuda_device, 59, [1, 30], [90, 7], 4, 2, 128, 32, window=89)
 
 
 def test_attention_many_requests(cuda_device):

@@ -16,6 +16,9 @@
 // are many, its 8 columns the query rows, of which there are few; the probabilities change sides by an 8x8 matrix
 // transposition in registers.  The order of the k index of a product is free, so a lane reads 16 consecutive code bytes
 // and converts them in registers; the swizzle makes these reads free of bank conflicts for both operands.
+// Four contexts of 90k to 131k tokens, 64 query and 8 kv heads of 128: 142 us, 6.2 TB/s (141 without the products); 64
+// requests of 200 to 8192 tokens: 117 us, 5.1 TB/s (114 without).  The query rows in the instruction's 16 rows took 174 and
+// 153 us: twice the instructions and registers for the same bytes.
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 #include <cuda_runtime.h>
@@ -37,7 +40,8 @@ constexpr int kFewThreads = 32 * (kFewWarps + 1);
 constexpr int kFewStages = 4;
 constexpr int kFewMinChunk = 2;       // tiles of a block's chunk, at least
 constexpr int kManyMinChunk = 2;
-// Requests of more packed rows go to the many-rows kernel.
+// Requests of more packed rows go to the many-rows kernel: this one reads the cache once per 16 rows, that one once per 256 at
+// the price of 256 rows' products.
 constexpr int kFewLimit = kFewRows;
 
 template <int kDim>

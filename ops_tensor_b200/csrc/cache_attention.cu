@@ -78,13 +78,6 @@ __device__ __forceinline__ uint32_t codes_hi(uint32_t w) {
 // 0xFF in every byte that is an E4M3 NaN.
 __device__ __forceinline__ uint32_t nan_bytes(uint32_t w) { return __vcmpeq4(w & 0x7F7F7F7Fu, 0x7F7F7F7Fu); }
 
-__device__ __forceinline__ void tma_load_page(uint32_t dst, const CUtensorMap* map, uint32_t bar, int row, int head, int block) {
-    asm volatile(
-        "cp.async.bulk.tensor.4d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5, %6}], [%2];" ::"r"(dst),
-        "l"(reinterpret_cast<uint64_t>(map)), "r"(bar), "r"(0), "r"(row), "r"(head), "r"(block)
-        : "memory");
-}
-
 // A named barrier of the computing warps.
 __device__ __forceinline__ void compute_sync() { asm volatile("bar.sync 1, %0;" ::"n"(32 * kFewWarps) : "memory"); }
 
@@ -757,7 +750,8 @@ static cudaError_t launch_attention(const CUtensorMap& mk, const CUtensorMap& mv
         p.part_out = reinterpret_cast<float*>(ws + pl.many_out);
         p.part_ml = reinterpret_cast<float*>(ws + pl.many_ml);
         p.cuts = reinterpret_cast<AttnCut*>(ws + pl.many_cuts);
-        e = launch_after_prepass(many, pl.many_grid, kManyThreads, (size_t)ManySmem<kDim>::bytes(p.requests), stream, p, cv);
+        e = launch_after_prepass(many, pl.many_grid, kManyThreads, (size_t)ManySmem<kDim>::bytes(p.requests), stream, mk, mv,
+                                 p, cv);
         if (e == cudaSuccess && pl.many_grid > 1)
             e = launch_after_prepass(cache_attention_join_kernel<kManyRows, kDim, kBf16>,
                                      (pl.many_grid - 1) * (kManyRows / 16), 256, 0, stream, p);

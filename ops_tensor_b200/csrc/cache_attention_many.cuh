@@ -6,11 +6,12 @@
 //   warps 0-3, 4-7   softmax of sub-tile A / B: scores from TMEM, probabilities back into the same TMEM columns as half
 //                    (the A operand of P V), O re-scaled in TMEM when a row's maximum has grown by more than 2^12
 //                    since it was last taken, the piece's epilogue
-//   warps 8-11       codes -> half: a thread copies its 16-byte pieces of the pages (cp.async, an operand tile and a half
-//                    ahead) into a staging slot of its own and expands them (exactly) into the 128-byte-swizzled operand
-//                    tile, a ring of three that K and V take turns in; block numbers and scales of the tiles
+//   warps 8-11       codes -> half: expand (exactly) the codes of an operand tile out of its staging slot into the
+//                    128-byte-swizzled operand tile, a ring of three that K and V take turns in
 //   warp 12          issues the MMAs: P_A V(t), Q_A K(t+1), P_B V(t), Q_B K(t+1), so each warpgroup's softmax runs while the
 //                    tensor cores work for the other one
+//   warp 13          fetches the pages' codes into the staging slots by TMA, an operand tile and a half ahead; block numbers
+//                    and scales of the tiles
 // The softmax threads also bring their own query row into shared memory at the start of a piece.
 // Q K^T takes K as the K-major operand; P V takes V as it lies, dims contiguous (MN-major), no transposition anywhere.
 // 769 rows of 16 heads of 128 on 15k and 30k tokens: 221 us, 719 TFLOP/s, tensor pipe 36 % busy; 4 prompts of up to 4096
@@ -24,7 +25,7 @@ namespace blaze {
 
 constexpr int kManyRows = 256;
 constexpr int kManyTokens = 128;
-constexpr int kManyThreads = 32 * 16;      // warps 13-15 only complete the last warpgroup
+constexpr int kManyThreads = 32 * 16;      // warps 14, 15 only complete the last warpgroup
 // Registers of a thread of the softmax, converting and issuing warpgroups (a softmax thread holds 64 to 96 scores);
 // the launch has 128 each, 512 for the four.
 constexpr int kSoftmaxRegs = 176, kConvertRegs = 88, kIssueRegs = 72;
@@ -46,7 +47,7 @@ struct ManySmem {
     static constexpr int kRawBytes = 128 * kDim;
     static constexpr int kMetaOffset = kRawOffset + 2 * kRawBytes;   // float4 [kManyMeta][8]
     static constexpr int kBarOffset = kMetaOffset + kManyMeta * 8 * 16;
-    static constexpr int kNumBars = 2 + 6 + kManyMeta + 6;
+    static constexpr int kNumBars = 2 + 6 + kManyMeta + 6 + 4;
     static constexpr int kMiscOffset = kBarOffset + kNumBars * 8;
     static constexpr int kPrefixOffset = kMiscOffset + 128;
     static int bytes(int requests) { return 1024 + kPrefixOffset + (requests + 1) * 4; }
@@ -158,14 +159,6 @@ __device__ __forceinline__ SubTile sub_tile(const CacheAttentionParams& p, const
     return x;
 }
 
-// 16 bytes global -> shared, or zeros where `bytes` is 0 (nothing is read then).
-__device__ __forceinline__ void cp_async16(void* dst, const void* src, int bytes) {
-    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(smem_u32(dst)), "l"(src), "r"(bytes) : "memory");
-}
-__device__ __forceinline__ void cp_async_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
-template <int kPending>
-__device__ __forceinline__ void cp_async_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(kPending) : "memory"); }
-
 // 16 E4M3 codes -> 16 halves.
 __device__ __forceinline__ void codes_to_half(const uint4& w, uint4& a, uint4& b) {
     auto lo = [](uint32_t x) {
@@ -182,7 +175,8 @@ __device__ __forceinline__ void codes_to_half(const uint4& w, uint4& a, uint4& b
 
 template <int kDim, bool kBf16>
 __global__ void __launch_bounds__(kManyThreads, 1)
-cache_attention_many_kernel(const CacheAttentionParams p, const CacheView cache) {
+cache_attention_many_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v,
+                            const CacheAttentionParams p, const CacheView cache) {
     using L = ManySmem<kDim>;
     extern __shared__ uint8_t many_smem_raw[];
     uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(many_smem_raw) + 1023) & ~uintptr_t(1023));
@@ -196,6 +190,8 @@ cache_attention_many_kernel(const CacheAttentionParams p, const CacheView cache)
     uint64_t* s_full = meta_full + kManyMeta; // [2] sub-tiles
     uint64_t* p_full = s_full + 2;            // [2]
     uint64_t* pv_done = s_full + 4;           // [2]
+    uint64_t* raw_full = s_full + 6;          // [2] codes of a K tile, of a V tile are there
+    uint64_t* raw_free = s_full + 8;          // [2] they have been read (the converting warps)
     int* misc = reinterpret_cast<int*>(smem + L::kMiscOffset);           // [0, 16): sums; 16: TMEM; 17: abort; 18..25: NaN tiles
     uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(misc + 16);
     volatile int* abort_flag = misc + 17;
@@ -214,6 +210,8 @@ cache_attention_many_kernel(const CacheAttentionParams p, const CacheView cache)
             mbar_init(&s_full[i], 1);
             mbar_init(&p_full[i], 4);
             mbar_init(&pv_done[i], 1);
+            mbar_init(&raw_full[i], 1);
+            mbar_init(&raw_free[i], 4);
         }
         for (int i = 0; i < kManyMeta; ++i) mbar_init(&meta_full[i], 1);
         *abort_flag = 0;
@@ -521,121 +519,69 @@ cache_attention_many_kernel(const CacheAttentionParams p, const CacheView cache)
             u = u_next;
         }
     } else if (warp < 12) {
-        // ------------------------------------------------------------------ codes -> half, scales
+        // ------------------------------------------------------------------ codes -> half
         regs_dec<kConvertRegs>();
         const int tid = threadIdx.x - 256;
         constexpr int kChunks = kDim / 16;                    // 16-code chunks of a row
         constexpr int kPasses = kDim / 16;                    // rows of a tile that a thread has a chunk of
-        constexpr int kPassRows = 128 / kPasses;              // (16 or 32: a warp's rows of a pass are of one group of 16)
+        constexpr int kPassRows = 128 / kPasses;              // (16 or 32, multiples of the swizzles' eight rows)
         const int ch = tid % kChunks, r0 = tid / kChunks;
-        // where the two halves of a piece go in an operand tile, in an order that keeps the eight lanes of a row on
-        // different banks
+        // where a chunk's codes are in the staging slot, and where the two halves of what they become go, in an order that
+        // keeps the eight lanes of a row on different banks
+        const uint32_t raw_at = r0 * kDim + ((kDim == 128 ? ch ^ (r0 & 7) : ch ^ ((r0 >> 1) & 3)) << 4);
         const int flip = (ch >> 2) & 1;
         const uint32_t to_a = (ch >> 2) * 16384 + r0 * 128 + ((((ch & 3) * 2 + flip) ^ (r0 & 7)) << 4);
         const uint32_t to_b = (ch >> 2) * 16384 + r0 * 128 + ((((ch & 3) * 2 + 1 - flip) ^ (r0 & 7)) << 4);
-        uint8_t* raw = smem + L::kRawOffset + tid * 16;
         int n_tile = 0, ring = 0;                             // tiles so far; place in the ring
         uint32_t ring_phase = 1;
         for (int u = begin; u < end && ok;) {
             const AttnPiece s = attn_piece<kManyRows, kManyTokens>(p, prefix, u, end);
             u += max(1, s.tile1 - s.tile0);
-            if (s.tile0 == s.tile1) continue;
-            const int* table = p.table + (long long)s.r * p.table_stride;
             const SubTile all = sub_tile(p, s, s.row0, s.row0 + kManyRows);
-            const long long mine = s.head * cache.head_stride + (r0 & 15) * cache.token_stride + ch * 16;
-            // lanes 0..7 hold the blocks of a tile's groups of 16 tokens, -1 for one that has none or that nobody sees
-            // (read two tiles ahead, looked at one tile later: nothing waits for the table)
-            auto wanted = [&](int t) -> bool {
-                const int tok = t * kManyTokens + (lane & 7) * 16;
-                return t < s.tile1 && tok < s.hi && tok + 16 > s.lo;
-            };
-            auto read_block = [&](int t) -> int {
-                return wanted(t) ? table[(t * kManyTokens + (lane & 7) * 16) >> p.block_shift] : -1;
-            };
-            auto check_block = [&](int t, int block) -> int {
-                if (block >= 0 && block < p.num_blocks) return block;
-                if (wanted(t)) atomicCAS(p.status, 0, DEV_BAD_CACHE_BLOCK);
-                return -1;
-            };
-            auto scale_of = [&](const float* scales, int block) -> float {
-                return block >= 0 ? scales[(long long)block * p.scale_stride + s.head] : 0.0f;
-            };
-            // copies this thread's pieces of tile t into its staging slots; of blocks that do not exist, zeros
-            auto fetch = [&](int which, int t, int block) {
-                const uint8_t* base = (which ? cache.v : cache.k) + mine;
-                const long long at = block < 0 ? -1
-                    : block * cache.block_stride + ((t * kManyTokens + (lane & 7) * 16) & (cache.block_size - 1)) * cache.token_stride;
-                if (t < s.tile1) {
-#pragma unroll
-                    for (int j = 0; j < kPasses; ++j) {
-                        const long long from = __shfl_sync(0xffffffffu, at, (j * kPassRows + r0) >> 4);
-                        cp_async16(raw + which * L::kRawBytes + j * 2048, base + (from < 0 ? 0 : from), from < 0 ? 0 : 16);
-                    }
-                }
-                cp_async_commit();
-            };
-            // expands the pieces of tile t
-            auto expand = [&](int which, int t, bool edge) -> bool {
-                uint4 w[kPasses];
-#pragma unroll
-                for (int j = 0; j < kPasses; ++j) w[j] = *reinterpret_cast<const uint4*>(raw + which * L::kRawBytes + j * 2048);
-                bool any = false;
-                if (edge) {
-                    // zeros in place of tokens that no row sees and, of V, of NaN codes
-#pragma unroll
-                    for (int j = 0; j < kPasses; ++j) {
-                        const int tok = t * kManyTokens + j * kPassRows + r0;
-                        if (tok < s.lo || tok >= s.hi) w[j] = make_uint4(0, 0, 0, 0);
-                        if (which == 1) {
-                            uint32_t* e = &w[j].x;
-#pragma unroll
-                            for (int h = 0; h < 4; ++h) {
-                                const uint32_t nb = __vcmpeq4(e[h] & 0x7F7F7F7Fu, 0x7F7F7F7Fu);
-                                any |= nb != 0;
-                                e[h] &= ~nb;
-                            }
-                        }
-                    }
-                }
-                ok = attn_wait(&free_[ring], ring_phase, abort_flag, p.status, DEV_TIMEOUT_SMEM_EMPTY);
-                if (!ok) return false;
-                uint8_t* tile = smem + L::kRingOffset + ring * L::kOperandBytes;
-#pragma unroll
-                for (int j = 0; j < kPasses; ++j) {
-                    uint4 a, b;
-                    codes_to_half(w[j], a, b);
-                    *reinterpret_cast<uint4*>(tile + to_a + j * kPassRows * 128) = flip ? b : a;
-                    *reinterpret_cast<uint4*>(tile + to_b + j * kPassRows * 128) = flip ? a : b;
-                }
-                if (any) nan_tile[n_tile & 7] = n_tile + 1;
-                fence_proxy_async();
-                return true;
-            };
-            int blk = check_block(s.tile0, read_block(s.tile0)), raw_block = read_block(s.tile0 + 1);
-            fetch(0, s.tile0, blk);
-            fetch(1, s.tile0, blk);
-            float ks = scale_of(p.k_scale, blk), vs = scale_of(p.v_scale, blk);
-            for (int t = s.tile0; t < s.tile1; ++t, ++n_tile) {
-                if (warp == 8) {
-                    if (lane < 8) {
-                        const float lv = fmaxf(lg2(vs), kMinLogScale);
-                        // (the scores' factor is not negative: the sign of `scale` went into the queries)
-                        meta[(n_tile % kManyMeta) * 8 + lane] =
-                            make_float4(ks * fabsf(p.scale_log2), blk >= 0 ? lv : -INFINITY, ex2(-lv), 0.0f);
-                    }
-                    __syncwarp();
-                    if (lane == 0) mbar_arrive(&meta_full[n_tile % kManyMeta]);
-                }
-                blk = check_block(t + 1, raw_block);
-                raw_block = read_block(t + 2);
-                ks = scale_of(p.k_scale, blk);
-                vs = scale_of(p.v_scale, blk);
-                const bool edge = all.masked(t);
+            for (int t = s.tile0; t < s.tile1 && ok; ++t, ++n_tile) {
+                const bool masked = all.masked(t);
 #pragma unroll 1
                 for (int which = 0; which < 2; ++which) {
-                    cp_async_wait<1>();
-                    if (!expand(which, t, edge)) break;
-                    fetch(which, t + 1, blk);
+                    ok = attn_wait(&raw_full[which], n_tile & 1, abort_flag, p.status, DEV_TIMEOUT_SMEM_FULL);
+                    if (!ok) break;
+                    const uint8_t* raw = smem + L::kRawOffset + which * L::kRawBytes + raw_at;
+                    uint4 w[kPasses];
+#pragma unroll
+                    for (int j = 0; j < kPasses; ++j) w[j] = *reinterpret_cast<const uint4*>(raw + j * kPassRows * kDim);
+                    // groups of 16 tokens that have been fetched
+                    const uint32_t there = __float_as_uint(meta[(n_tile % kManyMeta) * 8].w);
+                    if (masked || there != 0xFFu) {
+                        // zeros in place of tokens that no row sees or that there are not and, of V, of NaN codes
+                        bool any = false;
+#pragma unroll
+                        for (int j = 0; j < kPasses; ++j) {
+                            const int row = j * kPassRows + r0, tok = t * kManyTokens + row;
+                            if (tok < s.lo || tok >= s.hi || !(there >> (row >> 4) & 1)) w[j] = make_uint4(0, 0, 0, 0);
+                            if (which == 1 && masked) {
+                                uint32_t* e = &w[j].x;
+#pragma unroll
+                                for (int h = 0; h < 4; ++h) {
+                                    const uint32_t nb = __vcmpeq4(e[h] & 0x7F7F7F7Fu, 0x7F7F7F7Fu);
+                                    any |= nb != 0;
+                                    e[h] &= ~nb;
+                                }
+                            }
+                        }
+                        if (any) nan_tile[n_tile & 7] = n_tile + 1;
+                    }
+                    __syncwarp();
+                    if (lane == 0) mbar_arrive(&raw_free[which]);
+                    ok = attn_wait(&free_[ring], ring_phase, abort_flag, p.status, DEV_TIMEOUT_SMEM_EMPTY);
+                    if (!ok) break;
+                    uint8_t* tile = smem + L::kRingOffset + ring * L::kOperandBytes;
+#pragma unroll
+                    for (int j = 0; j < kPasses; ++j) {
+                        uint4 a, b;
+                        codes_to_half(w[j], a, b);
+                        *reinterpret_cast<uint4*>(tile + to_a + j * kPassRows * 128) = flip ? b : a;
+                        *reinterpret_cast<uint4*>(tile + to_b + j * kPassRows * 128) = flip ? a : b;
+                    }
+                    fence_proxy_async();
                     __syncwarp();
                     if (lane == 0) mbar_arrive(&full[ring]);
                     if (++ring == 3) { ring = 0; ring_phase ^= 1; }
@@ -643,7 +589,6 @@ cache_attention_many_kernel(const CacheAttentionParams p, const CacheView cache)
                 if (!ok) break;
             }
         }
-        cp_async_wait<0>();
     } else {
         regs_dec<kIssueRegs>();
     }
@@ -727,6 +672,77 @@ cache_attention_many_kernel(const CacheAttentionParams p, const CacheView cache)
                 if (!ok) break;
                 if (behind) advance(ring_v, phase_v);
                 if (more) advance(ring_k, phase_k);
+            }
+        }
+    }
+    if (warp == 13) {
+        // ------------------------------------------------------------------ pages, scales
+        const int bs = cache.block_size;
+        const int box_rows = min(bs, 64);
+        const uint32_t box_bytes = (uint32_t)box_rows * kDim;
+        const int group = lane & 7;                           // of 16 tokens of a tile
+        const bool leads = lane < 8 && group * 16 % box_rows == 0;         // this lane's group starts a box
+        int n_tile = 0;
+        for (int u = begin; u < end && ok;) {
+            const AttnPiece s = attn_piece<kManyRows, kManyTokens>(p, prefix, u, end);
+            u += max(1, s.tile1 - s.tile0);
+            const int* table = p.table + (long long)s.r * p.table_stride;
+            // lanes 0..7 hold the blocks of a tile's groups, -1 for one that has none or that nobody sees (read two tiles
+            // ahead, looked at one tile later: nothing waits for the table)
+            auto wanted = [&](int t) -> bool {
+                const int tok = t * kManyTokens + group * 16;
+                return t < s.tile1 && tok < s.hi && tok + 16 > s.lo;
+            };
+            // (a box is fetched when any of its tokens is seen: its first group then looks its block up too)
+            auto looked_up = [&](int t) -> bool {
+                const int tok = t * kManyTokens + group * 16;
+                return t < s.tile1 && (wanted(t) || (leads && tok < s.hi && tok + box_rows > s.lo));
+            };
+            auto read_block = [&](int t) -> int {
+                return looked_up(t) ? table[(t * kManyTokens + group * 16) >> p.block_shift] : -1;
+            };
+            auto check_block = [&](int t, int block) -> int {
+                if (block >= 0 && block < p.num_blocks) return block;
+                if (wanted(t)) atomicCAS(p.status, 0, DEV_BAD_CACHE_BLOCK);
+                return -1;
+            };
+            auto scale_of = [&](const float* scales, int block) -> float {
+                return block >= 0 ? scales[(long long)block * p.scale_stride + s.head] : 0.0f;
+            };
+            int blk = check_block(s.tile0, read_block(s.tile0)), raw_block = read_block(s.tile0 + 1);
+            float ks = scale_of(p.k_scale, blk), vs = scale_of(p.v_scale, blk);
+            for (int t = s.tile0; t < s.tile1; ++t, ++n_tile) {
+                const bool seen = blk >= 0 && wanted(t);
+                const uint32_t there = __ballot_sync(0xffffffffu, lane < 8 && seen);
+                const bool load = leads && blk >= 0;
+                const uint32_t loads = __ballot_sync(0xffffffffu, load);
+                const int tok = t * kManyTokens + group * 16;
+#pragma unroll 1
+                for (int which = 0; which < 2; ++which) {
+                    ok = attn_wait(&raw_free[which], (n_tile & 1) ^ 1, abort_flag, p.status, DEV_TIMEOUT_SMEM_EMPTY);
+                    if (!ok) break;
+                    if (which == 0) {
+                        if (lane < 8) {
+                            const float lv = fmaxf(lg2(vs), kMinLogScale);
+                            // (the scores' factor is not negative: the sign of `scale` went into the queries)
+                            meta[(n_tile % kManyMeta) * 8 + lane] =
+                                make_float4(ks * fabsf(p.scale_log2), seen ? lv : -INFINITY, ex2(-lv), __uint_as_float(there));
+                        }
+                        __syncwarp();
+                        if (lane == 0) mbar_arrive(&meta_full[n_tile % kManyMeta]);
+                    }
+                    if (lane == 0) mbar_arrive_expect_tx(&raw_full[which], (uint32_t)__popc(loads) * box_bytes);
+                    __syncwarp();
+                    if (load)
+                        tma_load_page(smem_u32(smem + L::kRawOffset + which * L::kRawBytes) + (uint32_t)group * 16u * kDim,
+                                      which ? &map_v : &map_k, smem_u32(&raw_full[which]), tok & (bs - 1), s.head, blk);
+                    __syncwarp();
+                }
+                if (!ok) break;
+                blk = check_block(t + 1, raw_block);
+                raw_block = read_block(t + 2);
+                ks = scale_of(p.k_scale, blk);
+                vs = scale_of(p.v_scale, blk);
             }
         }
     }

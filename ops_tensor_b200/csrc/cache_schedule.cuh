@@ -260,6 +260,14 @@ __device__ __forceinline__ float lg2(float x) {
     return y;
 }
 
+// One box of a page: `row` and on of (head, block).
+__device__ __forceinline__ void tma_load_page(uint32_t dst, const CUtensorMap* map, uint32_t bar, int row, int head, int block) {
+    asm volatile(
+        "cp.async.bulk.tensor.4d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5, %6}], [%2];" ::"r"(dst),
+        "l"(reinterpret_cast<uint64_t>(map)), "r"(bar), "r"(0), "r"(row), "r"(head), "r"(block)
+        : "memory");
+}
+
 // Probabilities are kept up to 2^15 (the running maximum less 15), so that in half the values down to 2^-29 of a row's
 // largest have all their bits and nothing above 2^-40 of it vanishes, however long the row.
 constexpr float kProbShift = 15.0f;

@@ -14,9 +14,11 @@
 //                    and scales of the tiles
 // The softmax threads also bring their own query row into shared memory at the start of a piece.
 // Q K^T takes K as the K-major operand; P V takes V as it lies, dims contiguous (MN-major), no transposition anywhere.
-// 769 rows of 16 heads of 128 on 15k and 30k tokens: 221 us, 719 TFLOP/s, tensor pipe 36 % busy; 4 prompts of up to 4096
-// rows of 32 heads: 612 us, 459 TFLOP/s.  Bound by the chain of a sub-tile's softmax (2700 cycles per 128 tokens), the
-// hand-over to the issuing warp, its MMAs (1170) and the hand-over back, which the other sub-tile's fills only partly.
+// 769 rows of 16 heads of 128 on 15k and 30k tokens: 215 us, 737 TFLOP/s, tensor pipe 36 % busy; 4 prompts of up to 4096
+// rows of 32 heads: 617 us, 456 TFLOP/s.  Bound by the chain of a sub-tile: softmax (2700 cycles per 128 tokens), hand-over to
+// the issuing warp, MMAs (1170), hand-over back, which the other sub-tile's fills only partly: without exponentials and with
+// one MMA of eight the chunk case takes 143 us, with nothing but maxima and hand-overs 113.  An issuing warp for each
+// sub-tile took 243 us (their MMAs take turns in the tensor pipe), hand-overs of 64 tokens 239.
 #pragma once
 
 #include "cache_schedule.cuh"

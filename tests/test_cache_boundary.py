@@ -127,7 +127,8 @@ def test_workspace_follows_the_bounds_and_the_share_of_sms(lib):
         assert lib.blazeCacheAttentionWorkspaceSize(C.byref(cache()), C.byref(attention(**kw)), C.byref(n)) == OK
         return n.value
     assert need() > 0 and need(sm_limit=10) < need()
-    assert need(requests=8192, max_q=1) >= need(max_q=1)
+    # (the lengths of many requests leave room for fewer blocks, and those need less)
+    assert 0 < need(requests=8192, max_q=1) <= need(max_q=1) <= need(max_q=100)
     assert lib.blazeCacheAttentionWorkspaceSize(C.byref(cache()), C.byref(attention()), None) == INVALID
 
 

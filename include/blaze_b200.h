@@ -350,7 +350,8 @@ BLAZE_API int blazeCacheAssign(const blazeCacheAssignArgs* args, void* stream);
  * of two that is exact down to E4M3's subnormals.
  * The rows of one block are neighbours in the call (as blazeCacheAssign lays them out) and, the call's lowest row apart,
  * nothing is assumed about their order; a slot that is named twice among them keeps the last row.  A block that is named
- * again further on in the call, with another block between, would be written by two warps at once: don't. */
+ * again further on in the call, with another block or a skipped row between, would be written by two warps at once:
+ * don't. */
 typedef struct {
     size_t struct_size;        /* sizeof(blazeCacheStoreArgs) */
     int32_t tokens;

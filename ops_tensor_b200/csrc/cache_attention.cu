@@ -54,7 +54,7 @@ struct FewSmem {
     static constexpr int kMlOffset = kJoinOffset + kFewWarps * kFewRows * kPitch * 4;
     static constexpr int kMetaOffset = kMlOffset + kFewWarps * kFewRows * 2 * 4;    // float4 per stage and warp
     static constexpr int kBarOffset = kMetaOffset + kFewStages * kFewWarps * 16;
-    static constexpr int kMiscOffset = kBarOffset + 2 * kFewStages * 8;
+    static constexpr int kMiscOffset = kBarOffset + (2 * kFewStages + 2) * 8;
     static constexpr int kPrefixOffset = kMiscOffset + 64;
     static int bytes(int requests) { return 1024 + kPrefixOffset + (requests + 1) * 4; }
 };
@@ -77,9 +77,6 @@ __device__ __forceinline__ uint32_t codes_hi(uint32_t w) {
 }
 // 0xFF in every byte that is an E4M3 NaN.
 __device__ __forceinline__ uint32_t nan_bytes(uint32_t w) { return __vcmpeq4(w & 0x7F7F7F7Fu, 0x7F7F7F7Fu); }
-
-// A named barrier of the computing warps.
-__device__ __forceinline__ void compute_sync() { asm volatile("bar.sync 1, %0;" ::"n"(32 * kFewWarps) : "memory"); }
 
 // Transpose of an 8x8 matrix of halves held two to a lane.
 __device__ __forceinline__ uint32_t transpose8x8(uint32_t x) {
@@ -104,6 +101,7 @@ cache_attention_few_kernel(const __grid_constant__ CUtensorMap map_k, const __gr
     float4* meta = reinterpret_cast<float4*>(smem + L::kMetaOffset);
     uint64_t* full = reinterpret_cast<uint64_t*>(smem + L::kBarOffset);
     uint64_t* empty = full + kFewStages;
+    uint64_t* joined = empty + kFewStages;         // the computing warps meet here
     int* misc = reinterpret_cast<int*>(smem + L::kMiscOffset);
     volatile int* abort_flag = misc + 8;
     int* prefix = reinterpret_cast<int*>(smem + L::kPrefixOffset);
@@ -114,6 +112,7 @@ cache_attention_few_kernel(const __grid_constant__ CUtensorMap map_k, const __gr
             mbar_init(&full[s], 1);
             mbar_init(&empty[s], kFewWarps);
         }
+        mbar_init(joined, kFewWarps);
         *abort_flag = 0;
         fence_mbar_init();
         tma_prefetch_desc(&map_k);
@@ -126,7 +125,7 @@ cache_attention_few_kernel(const __grid_constant__ CUtensorMap map_k, const __gr
     const long long begin64 = (long long)blockIdx.x * chunk;
     const int begin = (int)min(begin64, (long long)total);
     const int end = (int)min(begin64 + chunk, (long long)total);
-    if (threadIdx.x == 0 && begin >= end) p.cuts[blockIdx.x].first = -1;
+    if (threadIdx.x == 0) p.cuts[blockIdx.x].first = -1;          // until this thread knows better
 
     if (warp == kFewWarps) {
         // ------------------------------------------------------------------ fetching warp
@@ -209,8 +208,16 @@ cache_attention_few_kernel(const __grid_constant__ CUtensorMap map_k, const __gr
         // rows 2c, 2c + 1 of each n8 tile are the ones whose scores, statistics and output it has
         const int g = lane >> 2, c = lane & 3;
         int stage = 0;
-        uint32_t phase = 0;
+        uint32_t phase = 0, meeting = 0;
         bool ok = true;
+        // A meeting of the computing warps, bounded like every wait: a warp that has given up elsewhere does not come.
+        auto meet = [&]() -> bool {
+            __syncwarp();
+            if (lane == 0) mbar_arrive(joined);
+            const bool there = mbar_wait(joined, meeting, abort_flag, p.status, DEV_TIMEOUT_SMEM_EMPTY);
+            meeting ^= 1;
+            return __all_sync(0xffffffffu, there);
+        };
         for (int u = begin; u < end && ok;) {
             const AttnPiece s = attn_piece_at<kRows, kFewTokens>(p, prefix, u, end);
             const int u_next = u + max(1, s.tile1 - s.tile0);
@@ -473,7 +480,8 @@ cache_attention_few_kernel(const __grid_constant__ CUtensorMap map_k, const __gr
                         *reinterpret_cast<float4*>(dst + k) = make_float4(o[n][k / 2][e], o[n][k / 2][2 + e], o[n][k / 2 + 1][e], o[n][k / 2 + 1][2 + e]);
                 }
             }
-            compute_sync();
+            ok = meet();
+            if (!ok) break;
             {
                 constexpr int kPer = kDim * kRows / (32 * kFewWarps);       // dims of this thread
                 constexpr int kPerRow = kDim / kPer;                        // threads of a row
@@ -528,7 +536,7 @@ cache_attention_few_kernel(const __grid_constant__ CUtensorMap map_k, const __gr
                 }
             }
             if (threadIdx.x == 0 && u_next >= end) attn_write_cut(p, s, blockIdx.x, chunk, end);
-            compute_sync();
+            ok = meet();
             u = u_next;
         }
         grid_launch_dependents();

@@ -234,7 +234,7 @@ cache_attention_many_kernel(const __grid_constant__ CUtensorMap map_k, const __g
     const int begin = (int)min(begin64, (long long)total);
     const int end = (int)min(begin64 + chunk, (long long)total);
     bool ok = true;
-    if (threadIdx.x == 0 && begin >= end) p.cuts[blockIdx.x].first = -1;
+    if (threadIdx.x == 0) p.cuts[blockIdx.x].first = -1;          // until this thread knows better
 
     if (warp < 8) {
         // ------------------------------------------------------------------ softmax

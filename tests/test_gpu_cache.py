@@ -362,8 +362,17 @@ def test_attention_on_a_share_of_the_sms(cuda_device, sm_limit):
 
 def test_attention_hints_are_only_hints(cuda_device):
     """min_q above what the requests have, max_q and max_kv far above it."""
+    import torch
     attention_case(cuda_device, 53, [1, 40, 3], [90, 60, 200], 8, 2, 64, 32, min_q=40)
     attention_case(cuda_device, 54, [1, 2], [90, 60], 4, 2, 128, 32, max_q=500)
+    # nothing cached at all, and a table without columns
+    cache = native.PagedCache.empty(2, 2, 16, 64, cuda_device)
+    for n, heads in ((1, 2), (40, 4)):
+        q = torch.ones((n, heads, 64), dtype=torch.bfloat16, device=cuda_device)
+        lse = torch.zeros((n, heads), device=cuda_device)
+        out = native.cache_attention(cache, q, i32([0, n], cuda_device), i32([0], cuda_device),
+                                     torch.zeros((1, 0), dtype=torch.int32, device=cuda_device), max_q=n, max_kv=0, lse=lse)
+        assert bool((out == 0).all()) and bool(torch.isneginf(lse).all())
     # windows as wide as an int goes, of more rows than there are keys
     attention_case(cuda_device, 58, [1, 30], [90, 7], 4, 2, 64, 32, window=(1 << 31) - 1)
     attention_case(cuda_device, 59, [1, 30], [90, 7], 4, 2, 128, 32, window=89)

@@ -378,7 +378,7 @@ BLAZE_API int blazeCacheStore(const blazeKvCache* cache, const blazeCacheStoreAr
  * block_size); min_q is a hint: a bound from below on the rows of every request that has any, 0 if unknown.  The result
  * does not depend on how the work is split over the SMs beyond float32 rounding, and is the same from run to run.
  * The workspace needs no initialisation and keeps nothing between calls; calls that may overlap on the GPU need one
- * each. */
+ * each.  One that suffices for some tokens, requests, max_q and max_kv (with min_q = 0) suffices for any smaller ones. */
 typedef struct {
     size_t struct_size;        /* sizeof(blazeCacheAttentionArgs) */
     int32_t requests;          /* <= 8192 */

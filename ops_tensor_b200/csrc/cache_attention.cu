@@ -43,6 +43,11 @@ constexpr int kManyMinChunk = 2;
 // Requests of more packed rows go to the many-rows kernel: this one reads the cache once per 16 rows, that one once per 256 at
 // the price of 256 rows' products.
 constexpr int kFewLimit = kFewRows;
+// Small calls stay with the few-rows kernel whatever their rows: up to so many tiles of 64 tokens per block, counting 16 rows
+// a row tile and every request as long as the longest.  Measured, few-rows against many-rows kernel: 0.2 tiles (420 rows
+// on 105 tokens) 12.1 / 22.0 us; 3.9 (17 requests of up to 374 rows on up to 291 tokens) 27 / 55; 11.6 (8 of up to 160 rows
+// on up to 340) 41 / 33; 31 (2048 rows on 512) 99 / 40.
+constexpr double kFewSmall = 6.0;
 
 template <int kDim>
 struct FewSmem {
@@ -651,6 +656,7 @@ static int status_of(cudaError_t e) {
 // Which kernels a call needs, by the bounds of its requests' rows, and where their partial results lie.
 struct AttnPlan {
     bool few, many;
+    int few_rows;                                      // packed rows up to which a request is the few-rows kernel's
     int few_grid, many_grid;
     size_t few_ml, few_cuts, many_out, many_ml, many_cuts, total;      // offsets in the workspace (few_out is 0)
 };
@@ -670,12 +676,10 @@ static int plan_attention(const blazeKvCache* c, const blazeCacheAttentionArgs* 
         return ACLTENSOR_STATUS_NOT_SUPPORTED;
     const int64_t group = a->heads / c->kv_heads, rows = (int64_t)a->max_q * group;
     if (a->max_kv > (1 << 30) || rows > (1 << 24)) return ACLTENSOR_STATUS_NOT_SUPPORTED;
-    pl->many = rows > kFewLimit;
-    pl->few = !pl->many || (int64_t)a->min_q * group <= kFewLimit;
     // units are counted in 32 bits
     const double heads = (double)a->requests * c->kv_heads;
     if (heads * (double)(a->max_kv / kFewTokens + 2) > 2.0e9 ||
-        (pl->many && heads * (double)((rows + kManyRows - 1) / kManyRows) * (double)(a->max_kv / kManyTokens + 2) > 2.0e9))
+        (rows > kFewLimit && heads * (double)((rows + kManyRows - 1) / kManyRows) * (double)(a->max_kv / kManyTokens + 2) > 2.0e9))
         return ACLTENSOR_STATUS_NOT_SUPPORTED;
     if (a->sm_limit > 0 && a->sm_limit < sms) sms = a->sm_limit;
     // (a long prefix over many requests may leave no room for the last block of an SM)
@@ -684,6 +688,13 @@ static int plan_attention(const blazeKvCache* c, const blazeCacheAttentionArgs* 
     const int fit = (228 * 1024) / (few_bytes + 1024);
     pl->few_grid = (fit < few_blocks ? fit : few_blocks) * sms;
     pl->many_grid = sms;
+    // tiles of 64 tokens per block if the few-rows kernel took everything, at most
+    const double few_tiles = c->kv_heads * ((double)a->tokens * group / kFewRows + a->requests) *
+                             (a->max_kv / kFewTokens + 1.0) / pl->few_grid;
+    const bool small = few_tiles <= kFewSmall;
+    pl->many = rows > kFewLimit && !small;
+    pl->few = !pl->many || (int64_t)a->min_q * group <= kFewLimit;
+    pl->few_rows = small ? 0x7FFFFFFF : kFewLimit;
     size_t at = 0;
     auto room = [&](int grid, int tile_rows, size_t* ml, size_t* cuts) {
         at += round256((size_t)grid * 2 * tile_rows * c->head_dim * 4);
@@ -693,7 +704,8 @@ static int plan_attention(const blazeKvCache* c, const blazeCacheAttentionArgs* 
         at += round256((size_t)grid * sizeof(AttnCut));
     };
     pl->few_ml = pl->few_cuts = pl->many_out = pl->many_ml = pl->many_cuts = 0;
-    if (pl->few) room(pl->few_grid, kFewRows, &pl->few_ml, &pl->few_cuts);
+    // (room for all the blocks that a call of fewer requests may have: what suffices for larger bounds suffices for smaller)
+    if (pl->few) room(few_blocks * sms, kFewRows, &pl->few_ml, &pl->few_cuts);
     pl->many_out = at;
     if (pl->many) room(pl->many_grid, kManyRows, &pl->many_ml, &pl->many_cuts);
     pl->total = at;
@@ -738,7 +750,7 @@ static cudaError_t launch_attention(const CUtensorMap& mk, const CUtensorMap& mv
         done[dev & 63] = true;
     }
     cudaError_t e = cudaSuccess;
-    p.few_rows = kFewLimit;
+    p.few_rows = pl.few_rows;
     if (pl.few) {
         p.take_few = 1;
         p.take_many = 0;

@@ -664,7 +664,8 @@ def cache_attention_workspace_bytes(cache: PagedCache, q, *, requests, max_q, ma
 
 
 def cache_attention_workspace(cache: PagedCache, q, *, requests, max_q, max_kv, sm_limit=0):
-    """A workspace for cache_attention calls of these bounds; needs no initialisation, keeps nothing between calls."""
+    """A workspace for cache_attention calls of at most these bounds and as many rows as `q` has; needs no initialisation,
+    keeps nothing between calls."""
     if torch is None:
         _import_torch()
     need = cache_attention_workspace_bytes(cache, q, requests=requests, max_q=max_q, max_kv=max_kv, sm_limit=sm_limit)

@@ -127,8 +127,13 @@ def test_workspace_follows_the_bounds_and_the_share_of_sms(lib):
         assert lib.blazeCacheAttentionWorkspaceSize(C.byref(cache()), C.byref(attention(**kw)), C.byref(n)) == OK
         return n.value
     assert need() > 0 and need(sm_limit=10) < need()
-    # (the lengths of many requests leave room for fewer blocks, and those need less)
-    assert 0 < need(requests=8192, max_q=1) <= need(max_q=1) <= need(max_q=100)
+    # larger bounds never need less
+    wide = dict(max_blocks=4096, table_stride=4096)
+    for fixed in (dict(), dict(tokens=400, max_q=300), dict(tokens=30000, max_q=9000, heads=16)):
+        for name, steps in (("tokens", (1, 30, 3000, 100000)), ("requests", (1, 200, 3000, 8192)),
+                            ("max_q", (1, 4, 5, 300, 9000)), ("max_kv", (0, 64, 3000, 65536))):
+            sizes = [need(**{**wide, **fixed, name: v}) for v in steps]
+            assert sizes == sorted(sizes) and sizes[0] > 0, (fixed, name, sizes)
     assert lib.blazeCacheAttentionWorkspaceSize(C.byref(cache()), C.byref(attention()), None) == INVALID
 
 

@@ -137,12 +137,11 @@ cache_attention_few_kernel(const __grid_constant__ CUtensorMap map_k, const __gr
         const int bs = 1 << p.block_shift;
         const int box_rows = min(bs, kFewTokens);
         const uint32_t box_bytes = (uint32_t)box_rows * kDim;
-        const int boxes = kFewTokens / box_rows;
         int stage = 0;
         uint32_t phase = 0;
         bool ok = true;
         for (int u = begin; u < end && ok;) {
-            const AttnPiece s = attn_piece_at<kRows, kFewTokens>(p, prefix, u, end);
+            const AttnPiece s = attn_piece<kRows, kFewTokens>(p, prefix, u, end);
             u += max(1, s.tile1 - s.tile0);
             const int* table = p.table + (long long)s.r * p.table_stride;
             // Lane i holds page `base + i` of the request: block number and scales, fetched 32 pages at a time and one
@@ -205,7 +204,6 @@ cache_attention_few_kernel(const __grid_constant__ CUtensorMap map_k, const __gr
                 if (++stage == kFewStages) { stage = 0; phase ^= 1; }
             }
         }
-        (void)boxes;
         grid_launch_dependents();
     } else {
         // ------------------------------------------------------------------ computing warps
@@ -224,7 +222,7 @@ cache_attention_few_kernel(const __grid_constant__ CUtensorMap map_k, const __gr
             return __all_sync(0xffffffffu, there);
         };
         for (int u = begin; u < end && ok;) {
-            const AttnPiece s = attn_piece_at<kRows, kFewTokens>(p, prefix, u, end);
+            const AttnPiece s = attn_piece<kRows, kFewTokens>(p, prefix, u, end);
             const int u_next = u + max(1, s.tile1 - s.tile0);
             const int off = s.req.kv - s.req.qlen;
             auto see = [&](int row, int& lo, int& hi) {            // tokens that a row of the tile sees
@@ -824,7 +822,6 @@ extern "C" int blazeCacheAttention(const blazeKvCache* cache, const blazeCacheAt
     p.heads = a->heads;
     p.kv_heads = cache->kv_heads;
     p.group = a->heads / cache->kv_heads;
-    p.head_dim = cache->head_dim;
     p.block_shift = cv.block_shift;
     p.num_blocks = cache->num_blocks;
     p.max_blocks = a->max_blocks;

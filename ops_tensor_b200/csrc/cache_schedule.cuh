@@ -28,7 +28,7 @@ struct AttnCut {
 };
 
 struct CacheAttentionParams {
-    int requests, tokens, heads, kv_heads, group, head_dim;
+    int requests, tokens, heads, kv_heads, group;
     int block_shift, num_blocks, max_blocks;
     int max_q, max_kv;
     int causal, window;
@@ -181,7 +181,7 @@ struct AttnPiece {
 };
 
 template <int kRows, int kTokens>
-__device__ __forceinline__ AttnPiece attn_piece_at(const CacheAttentionParams& p, const int* prefix, int u, int end) {
+__device__ __forceinline__ AttnPiece attn_piece(const CacheAttentionParams& p, const int* prefix, int u, int end) {
     AttnPiece s;
     int a = 0, b = p.requests;
 #pragma unroll 1
@@ -241,12 +241,6 @@ __device__ __forceinline__ void attn_write_cut(const CacheAttentionParams& p, co
     c.rows = s.rows;
     c.pad = 0;
     p.cuts[block] = c;
-}
-
-// attn_piece_at out of line, for a kernel whose roles share the instruction cache.
-template <int kRows, int kTokens>
-__device__ __forceinline__ AttnPiece attn_piece(const CacheAttentionParams& p, const int* prefix, int u, int end) {
-    return attn_piece_at<kRows, kTokens>(p, prefix, u, end);
 }
 
 __device__ __forceinline__ float ex2(float x) {

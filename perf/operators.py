@@ -340,7 +340,7 @@ def _plain_assign(s):
     taken = (col >= have[:, None]) & (col < (have + need)[:, None]) & served[:, None]
     nth = ((need_to - need)[:, None] + col - have[:, None])[taken]
     s["block_table"][taken] = stack[top - 1 - nth]
-    popped = torch.where(served & (need > 0), need_to, 0).max()
+    popped = torch.where(served, need_to, 0).max()
     s["free_count_out"][:] = (top - popped).int()
     keep = torch.arange(stack.numel(), device=DEVICE)
     s["free_blocks"][:] = torch.where((keep >= count) & (keep < top - popped), stack, s["free_blocks"])

@@ -373,7 +373,9 @@ BLAZE_API int blazeCacheStore(const blazeKvCache* cache, const blazeCacheStoreAr
  * there and in the blocks' unused rows included.  Rows outside every request are left as they were.  out may not overlap
  * q: a row of q is read by every block that has a part of its work.
  * A token whose block number is outside the cache counts as not seen and the device status word reports code 8.
- * Scores, softmax and sums are float32; probabilities are rounded to half (11 bits) for the product with V.
+ * Scores, softmax and sums are float32; for the product with V probabilities are rounded to half: p_j v_scale_j to 11 bits
+ * down to 2^-26 of the row's largest one, and by at most 2^-37 of that largest one below (2^-29 and 2^-40 where the requests'
+ * rows are few).
  * max_q and max_kv bound the requests' rows and kv_len (lengths above are cut to them; max_kv may not pass max_blocks *
  * block_size); min_q is a hint: a bound from below on the rows of every request that has any, 0 if unknown.  The result
  * does not depend on how the work is split over the SMs beyond float32 rounding, and is the same from run to run.

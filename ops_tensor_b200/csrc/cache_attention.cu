@@ -49,6 +49,10 @@ constexpr int kFewLimit = kFewRows;
 // on up to 340) 41 / 33; 31 (2048 rows on 512) 99 / 40.
 constexpr double kFewSmall = 6.0;
 
+// Probabilities are kept up to 2^15 (the running maximum less 15), so that in half the values down to 2^-29 of a row's
+// largest have all their 11 bits and nothing above 2^-40 of it vanishes, however long the row.
+constexpr float kProbShift = 15.0f;
+
 template <int kDim>
 struct FewSmem {
     static constexpr int kBlocks = kDim == 64 ? 3 : 2;               // resident blocks of an SM

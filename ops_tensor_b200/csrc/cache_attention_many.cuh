@@ -4,7 +4,7 @@
 // A row tile is 256 packed query rows, two sub-tiles A and B of 128, one accumulator row per thread of a warpgroup each;
 // a tile of the cache is 128 tokens.  Roles:
 //   warps 0-3, 4-7   softmax of sub-tile A / B: scores from TMEM, probabilities back into the same TMEM columns as half
-//                    (the A operand of P V), O re-scaled in TMEM when a row's maximum has grown by more than 2^12
+//                    (the A operand of P V), O re-scaled in TMEM when a row's maximum has grown by more than 2^3
 //                    since it was last taken, the piece's epilogue
 //   warps 8-11       codes -> half: expand (exactly) the codes of an operand tile out of its staging slot into the
 //                    128-byte-swizzled operand tile, a ring of three that K and V take turns in
@@ -14,8 +14,8 @@
 //                    and scales of the tiles
 // The softmax threads also bring their own query row into shared memory at the start of a piece.
 // Q K^T takes K as the K-major operand; P V takes V as it lies, dims contiguous (MN-major), no transposition anywhere.
-// 769 rows of 16 heads of 128 on 15k and 30k tokens: 215 us, 737 TFLOP/s, tensor pipe 36 % busy; 4 prompts of up to 4096
-// rows of 32 heads: 617 us, 456 TFLOP/s.  Bound by the chain of a sub-tile: softmax (2700 cycles per 128 tokens), hand-over to
+// 769 rows of 16 heads of 128 on 15k and 30k tokens: 221 us, 720 TFLOP/s, tensor pipe 36 % busy; 4 prompts of up to 4096
+// rows of 32 heads: 624 us, 450 TFLOP/s.  Bound by the chain of a sub-tile: softmax (2700 cycles per 128 tokens), hand-over to
 // the issuing warp, MMAs (1170), hand-over back, which the other sub-tile's fills only partly: without exponentials and with
 // one MMA of eight the chunk case takes 143 us, with nothing but maxima and hand-overs 113.  An issuing warp for each
 // sub-tile took 243 us (their MMAs take turns in the tensor pipe), hand-overs of 64 tokens 239.
@@ -35,8 +35,12 @@ constexpr int kManyLaunchRegs = 128;
 static_assert(2 * kSoftmaxRegs + kConvertRegs + kIssueRegs <= 4 * kManyLaunchRegs, "setmaxnreg draws on what the launch has");
 constexpr int kManyMeta = 4;              // tiles whose scales are held
 
-// A row's reference is set 2^3 below its largest score and kept until a score passes it by 2^15 (half ends at 2^16).
-constexpr float kManyShift = 3.0f;
+// A row's reference is set 2^12 below its largest score (with the V scale in it) and kept until a score passes it by 2^15
+// (half ends at 2^16).  So the largest probability of a row is held as 2^12 to 2^15: in half the values down to 2^-26 of it
+// have all their 11 bits, smaller ones are off by at most 2^-37 of it and vanish below that, while the sum l counts them in
+// full.  A row's output may rest on such values, where the heaviest token has no value (an attention sink).  A reference 2^3
+// below the largest leaves 2^-17 and 2^-28 (2.4 % off at weights of 2^-24.5).
+constexpr float kManyShift = 12.0f;
 constexpr float kManyGrow = 15.0f;
 
 template <int kDim>

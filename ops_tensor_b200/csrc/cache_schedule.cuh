@@ -262,9 +262,6 @@ __device__ __forceinline__ void tma_load_page(uint32_t dst, const CUtensorMap* m
         : "memory");
 }
 
-// Probabilities are kept up to 2^15 (the running maximum less 15), so that in half the values down to 2^-29 of a row's
-// largest have all their bits and nothing above 2^-40 of it vanishes, however long the row.
-constexpr float kProbShift = 15.0f;
 // A V scale enters the exponent; below 2^-64 (which the store never writes) it counts as that.
 constexpr float kMinLogScale = -64.0f;
 

@@ -284,7 +284,10 @@ BLAZE_API int blazeQuantizeFp8Blocks(const void* w, int64_t ldw, int32_t N, int3
  *
  * A cache holds `num_blocks` blocks of `block_size` tokens; a request owns the blocks that its row of the block table
  * names, token p of the request being row p % block_size of block table[p / block_size].  Codes are E4M3, with one
- * float32 scale per (block, kv head) for K and one for V: value = code * scale.
+ * float32 scale per (block, kv head) for K and one for V: value = code * scale.  blazeCacheStore writes powers of two from
+ * 2^-64 to 2^120; blazeCacheAttention reads any positive, finite scale, a V scale below 2^-64 counting as 2^-64.  V scales
+ * of the tokens that one row sees should lie within 2^96 of one another: beyond that the weights of tokens with the
+ * smallest scales may be lost.
  * Constraints: block_size 16, 32, 64 or 128; head_dim 64 or 128; base pointers 16-byte aligned and strides multiples
  * of 16 bytes, so both [block][head][token][dim] and [block][token][head][dim] orders work (in the first one a (block,
  * head) page is one contiguous run).

@@ -192,7 +192,7 @@ cache_attention_few_kernel(const __grid_constant__ CUtensorMap map_k, const __gr
                     const bool seen = block >= 0 && tok < s.hi && tok + 16 > s.lo;
                     const float lv = fmaxf(lg2(v_s), kMinLogScale);
                     meta[stage * kFewWarps + lane] =
-                        make_float4(k_s * p.scale_log2, seen ? lv : -INFINITY, ex2(-lv), 0.0f);
+                        make_float4(k_s * p.scale_log2, seen ? lv : -INFINITY, ex2_subnormal(-lv), 0.0f);
                 }
                 __syncwarp();
                 if (lane == 0) mbar_arrive_expect_tx(&full[stage], (uint32_t)__popc(loads) * 2u * box_bytes);

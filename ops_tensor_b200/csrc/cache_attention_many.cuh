@@ -732,7 +732,7 @@ cache_attention_many_kernel(const __grid_constant__ CUtensorMap map_k, const __g
                             const float lv = fmaxf(lg2(vs), kMinLogScale);
                             // (the scores' factor is not negative: the sign of `scale` went into the queries)
                             meta[(n_tile % kManyMeta) * 8 + lane] =
-                                make_float4(ks * fabsf(p.scale_log2), seen ? lv : -INFINITY, ex2(-lv), __uint_as_float(there));
+                                make_float4(ks * fabsf(p.scale_log2), seen ? lv : -INFINITY, ex2_subnormal(-lv), __uint_as_float(there));
                         }
                         __syncwarp();
                         if (lane == 0) mbar_arrive(&meta_full[n_tile % kManyMeta]);

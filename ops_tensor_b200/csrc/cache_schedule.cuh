@@ -248,6 +248,12 @@ __device__ __forceinline__ float ex2(float x) {
     asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
     return y;
 }
+// Without flushing: 1 / v_scale is subnormal for a scale above 2^126.
+__device__ __forceinline__ float ex2_subnormal(float x) {
+    float y;
+    asm("ex2.approx.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
 __device__ __forceinline__ float lg2(float x) {
     float y;
     asm("lg2.approx.f32 %0, %1;" : "=f"(y) : "f"(x));
@@ -262,7 +268,9 @@ __device__ __forceinline__ void tma_load_page(uint32_t dst, const CUtensorMap* m
         : "memory");
 }
 
-// A V scale enters the exponent; below 2^-64 (which the store never writes) it counts as that.
+// A V scale enters the exponent; below 2^-64 (which the store never writes) it counts as that, so that a sum of p / v_scale
+// stays far below float32's end.  A token's p vanishes from the sum when its score (in powers of two, with its V scale) is
+// 2^138 below the row's largest: with V scales at most 2^96 apart, a weight of 2^-42 of the largest one's.
 constexpr float kMinLogScale = -64.0f;
 
 // Power of two that brings the largest magnitude of a row of bf16 queries to [2^14, 2^15), so that the row fits half

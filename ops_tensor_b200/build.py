@@ -8,6 +8,7 @@ cached under build/ and rebuilt when a source or any header is newer.
 from __future__ import annotations
 
 import os
+import re
 import shutil
 import subprocess
 import sys
@@ -21,8 +22,27 @@ BUILD_DIR = ROOT / "build"
 LIB_PATH = PKG_DIR / "libops_tensor_b200.so"
 
 ARCH_FLAGS = ["-gencode", "arch=compute_100a,code=sm_100a"]
-COMMON = ["-O3", "-std=c++17", "-lineinfo", "-Xcompiler", "-fPIC,-fvisibility=hidden", f"-I{ROOT / 'include'}",
+COMMON = ["-O3", "-Xptxas=-v", "-std=c++17", "-lineinfo", "-Xcompiler", "-fPIC,-fvisibility=hidden", f"-I{ROOT / 'include'}",
           f"-I{CSRC}", f"-I{CSRC / 'host'}"]
+
+
+# Registers per thread that a kernel's launch has to have: its warpgroups trade them (setmaxnreg), and a launch with fewer
+# would wait for registers that are not there.  __launch_bounds__ only caps the number.
+LAUNCH_REGISTERS = {"cache_attention_many_kernel": 128}
+
+
+def check_registers(report: str) -> None:
+    """Holds what ptxas reports (-v) of the kernels in LAUNCH_REGISTERS against what they need."""
+    entry = None
+    for line in report.splitlines():
+        m = re.search(r"Compiling entry function '(\w+)'", line)
+        if m:
+            entry = m.group(1)
+        m = re.search(r"Used (\d+) registers", line)
+        if m and entry:
+            for name, wanted in LAUNCH_REGISTERS.items():
+                if name in entry and int(m.group(1)) != wanted:
+                    raise RuntimeError(f"{entry} was given {m.group(1)} registers, its register trade needs {wanted}")
 
 
 def _nvcc() -> str:
@@ -62,11 +82,15 @@ def build(force: bool = False, verbose: bool = False) -> Path:
             return obj
         cmd = [nvcc, *ARCH_FLAGS, *COMMON, "-x", "cu" if src.suffix == ".cu" else "c++", "-c", str(src), "-o", str(obj)]
         if verbose:
-            cmd.insert(1, "-Xptxas=-v")
             print(" ".join(cmd), flush=True)
         r = subprocess.run(cmd, capture_output=True, text=True)
         if r.returncode != 0:
             raise RuntimeError(f"nvcc failed for {src.name}:\n{r.stdout}\n{r.stderr}")
+        try:
+            check_registers(r.stderr)
+        except RuntimeError:
+            obj.unlink()
+            raise
         if verbose and r.stderr:
             print(r.stderr)
         return obj

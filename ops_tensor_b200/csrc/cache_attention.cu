@@ -714,20 +714,43 @@ static int plan_attention(const blazeKvCache* c, const blazeCacheAttentionArgs* 
     return ACLTENSOR_STATUS_SUCCESS;
 }
 
+// What the kernels of a head size and type need before their first launch on a device.  The ones that the call at hand does
+// not launch are loaded too, so that a capture may follow any first call; only a call that needs the many-rows kernel
+// fails where that one cannot run.
+template <int kDim, bool kBf16>
+static cudaError_t prepare_attention(bool with_many) {
+    enum { kUnknown, kAll, kWithoutMany };
+    static int state[64] = {};
+    int dev = 0;
+    cudaGetDevice(&dev);
+    int& known = state[dev & 63];
+    if (known == kUnknown) {
+        static_assert(1024 + FewSmem<kDim>::kPrefixOffset + (kAttnMaxRequests + 1) * 4 <= 227 * 1024, "shared memory");
+        static_assert(1024 + ManySmem<kDim>::kPrefixOffset + (kAttnMaxRequests + 1) * 4 <= 227 * 1024, "shared memory");
+        const cudaFuncAttribute smem = cudaFuncAttributeMaxDynamicSharedMemorySize;
+        const int few_bytes = FewSmem<kDim>::bytes(kAttnMaxRequests);
+        cudaFuncAttributes attr;
+        cudaError_t e = cudaFuncSetAttribute(cache_attention_few_kernel<kDim, kBf16, 1>, smem, few_bytes);
+        if (e == cudaSuccess) e = cudaFuncSetAttribute(cache_attention_few_kernel<kDim, kBf16, 2>, smem, few_bytes);
+        if (e == cudaSuccess) e = cudaFuncGetAttributes(&attr, cache_attention_join_kernel<8, kDim, kBf16>);
+        if (e == cudaSuccess) e = cudaFuncGetAttributes(&attr, cache_attention_join_kernel<16, kDim, kBf16>);
+        if (e == cudaSuccess) e = cudaFuncGetAttributes(&attr, cache_attention_join_kernel<kManyRows, kDim, kBf16>);
+        if (e == cudaSuccess) e = cudaFuncGetAttributes(&attr, cache_attention_many_kernel<kDim, kBf16>);
+        if (e != cudaSuccess) return e;
+        // its warpgroups trade registers: the launch has to have all that they take (the build checks it too)
+        const bool many = attr.numRegs >= kManyLaunchRegs;
+        if (many)
+            e = cudaFuncSetAttribute(cache_attention_many_kernel<kDim, kBf16>, smem, ManySmem<kDim>::bytes(kAttnMaxRequests));
+        if (e != cudaSuccess) return e;
+        known = many ? kAll : kWithoutMany;
+    }
+    return with_many && known != kAll ? cudaErrorInvalidConfiguration : cudaSuccess;
+}
+
 template <int kDim, bool kBf16, int kTiles>
 static cudaError_t launch_few(const CUtensorMap& mk, const CUtensorMap& mv, const CacheAttentionParams& p, int grid,
                               cudaStream_t stream) {
     auto few = cache_attention_few_kernel<kDim, kBf16, kTiles>;
-    static bool done[64] = {};
-    int dev = 0;
-    cudaGetDevice(&dev);
-    if (!done[dev & 63]) {
-        static_assert(1024 + FewSmem<kDim>::kPrefixOffset + (kAttnMaxRequests + 1) * 4 <= 227 * 1024, "shared memory");
-        const cudaError_t e = cudaFuncSetAttribute(few, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                                   FewSmem<kDim>::bytes(kAttnMaxRequests));
-        if (e != cudaSuccess) return e;
-        done[dev & 63] = true;
-    }
     const cudaError_t e = launch_after_prepass(few, grid, kFewThreads, (size_t)FewSmem<kDim>::bytes(p.requests), stream, mk, mv, p);
     if (e != cudaSuccess || grid < 2) return e;
     return launch_after_prepass(cache_attention_join_kernel<8 * kTiles, kDim, kBf16>, grid - 1, 256, 0, stream, p);
@@ -736,22 +759,8 @@ static cudaError_t launch_few(const CUtensorMap& mk, const CUtensorMap& mv, cons
 template <int kDim, bool kBf16>
 static cudaError_t launch_attention(const CUtensorMap& mk, const CUtensorMap& mv, CacheAttentionParams p, const CacheView& cv,
                                     const AttnPlan& pl, uint8_t* ws, cudaStream_t stream) {
-    auto many = cache_attention_many_kernel<kDim, kBf16>;
-    static bool done[64] = {};
-    int dev = 0;
-    cudaGetDevice(&dev);
-    if (!done[dev & 63]) {
-        static_assert(1024 + ManySmem<kDim>::kPrefixOffset + (kAttnMaxRequests + 1) * 4 <= 227 * 1024, "shared memory");
-        // the kernel's warpgroups trade registers: the launch has to have all that they take
-        cudaFuncAttributes attr;
-        cudaError_t e = cudaFuncGetAttributes(&attr, many);
-        if (e == cudaSuccess && attr.numRegs < kManyLaunchRegs) e = cudaErrorInvalidConfiguration;
-        if (e == cudaSuccess)
-            e = cudaFuncSetAttribute(many, cudaFuncAttributeMaxDynamicSharedMemorySize, ManySmem<kDim>::bytes(kAttnMaxRequests));
-        if (e != cudaSuccess) return e;
-        done[dev & 63] = true;
-    }
-    cudaError_t e = cudaSuccess;
+    cudaError_t e = prepare_attention<kDim, kBf16>(pl.many);
+    if (e != cudaSuccess) return e;
     p.few_rows = pl.few_rows;
     if (pl.few) {
         p.take_few = 1;
@@ -772,8 +781,8 @@ static cudaError_t launch_attention(const CUtensorMap& mk, const CUtensorMap& mv
         p.part_out = reinterpret_cast<float*>(ws + pl.many_out);
         p.part_ml = reinterpret_cast<float*>(ws + pl.many_ml);
         p.cuts = reinterpret_cast<AttnCut*>(ws + pl.many_cuts);
-        e = launch_after_prepass(many, pl.many_grid, kManyThreads, (size_t)ManySmem<kDim>::bytes(p.requests), stream, mk, mv,
-                                 p, cv);
+        e = launch_after_prepass(cache_attention_many_kernel<kDim, kBf16>, pl.many_grid, kManyThreads,
+                                 (size_t)ManySmem<kDim>::bytes(p.requests), stream, mk, mv, p, cv);
         if (e == cudaSuccess && pl.many_grid > 1)
             e = launch_after_prepass(cache_attention_join_kernel<kManyRows, kDim, kBf16>,
                                      (pl.many_grid - 1) * (kManyRows / 16), 256, 0, stream, p);

@@ -1,0 +1,127 @@
+"""GPU: the paged-cache operators at the edges of their buffers (every kind of slot outside the cache, guards around all that
+is written, lengths and offsets that make no sense)."""
+import numpy as np
+import pytest
+
+import cache_reference as ref
+from ops_tensor_b200 import native
+from test_gpu_cache import check_store, i32, random_cache
+
+pytestmark = pytest.mark.gpu
+INT_MIN, INT_MAX = -(1 << 31), (1 << 31) - 1
+
+
+@pytest.mark.parametrize("kind,heads,bs,dim", [("bf16", 2, 16, 128), ("f16", 3, 64, 64)])
+def test_store_skips_every_slot_outside_the_cache(cuda_device, kind, heads, bs, dim):
+    """Slots below, just behind and far outside the cache, up to the ends of 64 bits and at values whose low 32 bits would
+    be inside, before, between and behind runs of several lengths."""
+    import torch
+    rng = np.random.default_rng(bs)
+    blocks = 21
+    cache, codes, scales = random_cache(rng, blocks, heads, bs, dim, cuda_device)
+    outside = [-1, blocks * bs, -(1 << 40), 1 << 40, -(1 << 63), (1 << 63) - 1, (1 << 32) + 3, -(1 << 32) + 5, INT_MIN,
+               1 << 31, -blocks * bs, blocks * bs + 1]
+    slots, ids = [outside[0]], rng.permutation(blocks)
+    for i, b in enumerate(ids[:18]):
+        first, count = [(0, bs), (3, 2), (bs - 1, 1), (5, bs - 5), (1, 7)][i % 5]
+        slots += [int(b) * bs + first + j for j in range(count)]
+        slots += [outside[(i + j) % len(outside)] for j in range(1 + i % 4)]
+    slots += outside
+    assert all(slots.count(x) >= 2 for x in outside)
+    k, v = (torch.from_numpy(rng.standard_normal((len(slots), heads, dim))).to(cuda_device)
+            .to({"bf16": torch.bfloat16, "f16": torch.float16}[kind]) for _ in range(2))
+    native.cache_store(cache, k, v, torch.tensor(slots, dtype=torch.int64, device=cuda_device))
+    check_store(cache, codes, scales, k, v, slots)
+
+
+class Guarded:
+    """A tensor inside a larger one whose borders have to stay as they are."""
+
+    def __init__(self, shape, dtype, device, value, guard=64):
+        import torch
+        self.n, self.guard, self.value = int(np.prod(shape)), guard, value
+        self.all = torch.full((self.n + 2 * guard,), value, dtype=dtype, device=device)
+        self.inside = self.all[guard:guard + self.n].view(shape)
+
+    def intact(self):
+        return bool((self.all[:self.guard] == self.value).all()) and bool((self.all[self.guard + self.n:] == self.value).all())
+
+
+@pytest.mark.parametrize("sm_limit", [0, 1])
+@pytest.mark.parametrize("q_off,kv,rows,lens", [
+    ([-5, 3, 400], [30, 20], [(0, 3), (3, 33)], [30, 20]),            # behind the last row, before the first
+    ([0, 50, 4], [64, 1 << 30], [(0, 30), (50, 50)], [40, 40]),       # falling
+    ([0, 4, 60], [-7, 64], [(0, 4), (4, 34)], [0, 40]),               # more rows than max_q, longer than max_kv
+    ([INT_MIN, 2, INT_MAX], [INT_MAX, INT_MIN], [(0, 2), (2, 32)], [40, 0]),
+    ([INT_MAX, INT_MIN, INT_MIN], [5, 5], [(60, 60), (0, 0)], [5, 5]),
+    ([60, 60, 60], [40, 40], [(60, 60), (60, 60)], [40, 40])])
+def test_attention_cuts_offsets_and_lengths(cuda_device, q_off, kv, rows, lens, sm_limit):
+    """60 rows, max_q 30, max_kv 40: `rows` and `lens` are what is left of the offsets and lengths.  The rows that a request
+    has are the reference's, all others, and what lies around out, lse and the workspace, stay as they were (up to 60
+    packed rows a request: on one SM the many-rows kernel, else the few-rows kernel)."""
+    import torch
+    rng = np.random.default_rng(6)
+    heads, kv_heads, dim, tokens = 4, 2, 64, 60
+    cache, codes, scales = random_cache(rng, 8, kv_heads, 16, dim, cuda_device)
+    q = torch.from_numpy(rng.standard_normal((tokens, heads, dim))).to(cuda_device).to(torch.bfloat16)
+    tab = np.arange(8).reshape(2, 4)
+    out = Guarded((tokens, heads, dim), torch.bfloat16, cuda_device, 7.0)
+    lse = Guarded((tokens, heads), torch.float32, cuda_device, 7.0)
+    need = native.cache_attention_workspace_bytes(cache, q, requests=2, max_q=30, max_kv=40, sm_limit=sm_limit)
+    space = Guarded((need,), torch.uint8, cuda_device, 0xA5, guard=4096)
+    native.cache_attention(cache, q, i32(q_off, cuda_device), i32(kv, cuda_device), i32(tab, cuda_device), max_q=30, max_kv=40,
+                           out=out.inside, lse=lse.inside, workspace=space.inside, sm_limit=sm_limit)
+    assert out.intact() and lse.intact() and space.intact() and native.device_status() == 0
+    got, got_lse = out.inside.double().cpu().numpy(), lse.inside.double().cpu().numpy()
+    qd = q.double().cpu().numpy()
+    written = np.zeros(tokens, dtype=bool)
+    for r, ((a, b), n) in enumerate(zip(rows, lens)):
+        written[a:b] = True
+        args = ([0, b - a], [n], tab[r:r + 1], dim ** -0.5, True, 0)
+        want, want_lse = ref.attention(qd[a:b], codes[0], codes[1], scales[0], scales[1], *args)
+        mass, _ = ref.attention(qd[a:b], codes[0], codes[1] & 127, scales[0], scales[1], *args)
+        # output 2^-8, probabilities 2^-11, scores dim * 2^-23 * scale |q| |k| with |q| |k| below 12 * 64^0.5 * 448 * 2^-7
+        err = dim * 2.0 ** -23 * dim ** -0.5 * 12 * 8 * 448 * 2.0 ** -7 + 2.0 ** -21
+        assert (np.abs(got[a:b] - want) <= 2.0 ** -8 * np.abs(want) + (2.0 ** -11 + 2 * np.expm1(err)) * mass + 1e-7).all()
+        empty = np.isneginf(want_lse)
+        assert np.array_equal(np.isneginf(got_lse[a:b]), empty)
+        assert (np.abs(got_lse[a:b][~empty] - want_lse[~empty]) <= err + 4 * 2.0 ** -23 * (np.abs(want_lse[~empty]) + 30)).all()
+    assert (got[~written] == 7.0).all() and (got_lse[~written] == 7.0).all()
+
+
+@pytest.mark.parametrize("in_place", [False, True])
+@pytest.mark.parametrize("seed", range(6))
+def test_assign_stays_in_its_buffers(cuda_device, seed, in_place):
+    """Lengths of any value, a count of free blocks below zero and above the stack, on one block and many: what lies around
+    every output stays as it was, and the lists agree with the loop on the cut values."""
+    import torch
+    rng = np.random.default_rng(seed)
+    n, block, columns, capacity = [1, 5, 40, 300, 37, 2][seed], [16, 128, 32, 64, 16, 64][seed], 7, [30, 90, 60, 700, 0, 5][seed]
+    max_tokens = [9, 40, 3000, 20000, 60, 0][seed]
+    odd = np.array([INT_MIN, -1, 0, 1, 2, block, columns * block, columns * block + 1, INT_MAX], dtype=np.int64)
+    cached = np.where(rng.random(n) < 0.3, rng.choice(odd, n), rng.integers(0, columns * block + 1, n))
+    new = np.where(rng.random(n) < 0.3, rng.choice(odd, n), rng.integers(-1, 2 * block, n))
+    count = [INT_MAX, -9, 60, 350, 3, INT_MIN][seed]
+    guarded = {"table": Guarded((n, columns), torch.int32, cuda_device, -5), "free": Guarded((capacity,), torch.int32, cuda_device, -5),
+               "count": Guarded((1,), torch.int32, cuda_device, -5), "cached": Guarded((n,), torch.int32, cuda_device, -5),
+               "offsets": Guarded((n + 1,), torch.int32, cuda_device, -5), "slots": Guarded((max_tokens,), torch.int64, cuda_device, -5),
+               "positions": Guarded((max_tokens,), torch.int32, cuda_device, -5), "denied": Guarded((1,), torch.int32, cuda_device, -5),
+               "kv": Guarded((n,), torch.int32, cuda_device, -5), "left": Guarded((1,), torch.int32, cuda_device, -5)}
+    t = {k: g.inside for k, g in guarded.items()}
+    table, free = rng.permutation(n * columns).reshape(n, columns), rng.permutation(capacity) + 5000
+    for key, x in (("table", table), ("free", free), ("count", [count]), ("cached", cached)):
+        t[key].copy_(i32(x, cuda_device).reshape(t[key].shape))
+    kv, left = (t["cached"], t["count"]) if in_place else (t["kv"], t["left"])
+    native.cache_assign(t["cached"], i32(new, cuda_device), t["table"], t["free"], t["count"], block_size=block,
+                        row_offsets=t["offsets"], kv_len=kv, slots=t["slots"], positions=t["positions"], free_count_out=left,
+                        denied=t["denied"])
+    assert all(g.intact() for g in guarded.values())
+    cut = np.clip(cached, 0, columns * block)
+    # (the loop walks a request's rows one by one: as many as pass every limit stand for 2^31)
+    some = np.minimum(new, columns * block + max_tokens + 1)
+    want = ref.assign(cut.tolist(), some.tolist(), table, free, min(max(count, 0), capacity), block, max_tokens)
+    got = {"block_table": t["table"], "free_blocks": t["free"], "row_offsets": t["offsets"], "kv_len": kv, "slots": t["slots"],
+           "positions": t["positions"]}
+    for key, x in got.items():
+        assert np.array_equal(x.cpu().numpy(), want[key]), key
+    assert int(left.item()) == min(want["free_count"], capacity) and int(t["denied"].item()) == want["denied"]

@@ -1,5 +1,5 @@
 """GPU: the paged-cache operators at the edges of their buffers (every kind of slot outside the cache, guards around all that
-is written, lengths and offsets that make no sense)."""
+is written, lengths and offsets that make no sense) and a whole step captured once and replayed."""
 import numpy as np
 import pytest
 
@@ -125,3 +125,68 @@ def test_assign_stays_in_its_buffers(cuda_device, seed, in_place):
     for key, x in got.items():
         assert np.array_equal(x.cpu().numpy(), want[key]), key
     assert int(left.item()) == min(want["free_count"], capacity) and int(t["denied"].item()) == want["denied"]
+
+
+@pytest.mark.parametrize("dim,bs,heads,kv_heads,rows", [(64, 16, 6, 3, 60), (128, 32, 8, 2, 1100)])
+def test_captured_step(cuda_device, dim, bs, heads, kv_heads, rows):
+    """Assign, store and attention of a padded batch captured once, lengths updated in place, and replayed on other lengths:
+    prompts, decode steps, drafted tokens, requests that wait, end and start again.  1100 rows take assign's second launch.
+    Codes, scales, tables and lists have to be the loop's; the attention's bound is 2^-8 of the output, 2^-11 for its
+    probabilities and less than 2^-11 for the scores: |q| |k| <= dim (1 + 2^-4), twice dim^0.5 * 2^-23 times that."""
+    import torch
+    rng = np.random.default_rng(dim)
+    n, blocks, columns = 4, 30, 9
+    torch_rows = lambda h: torch.zeros((rows, h, dim), dtype=torch.bfloat16, device=cuda_device)
+
+    def state():
+        return dict(cache=native.PagedCache.empty(blocks, kv_heads, bs, dim, cuda_device), kv=i32([0] * n, cuda_device),
+                    table=torch.full((n, columns), -1, dtype=torch.int32, device=cuda_device),
+                    free=torch.arange(blocks, dtype=torch.int32, device=cuda_device), count=i32([blocks], cuda_device),
+                    denied=i32([0], cuda_device), new=i32([0] * n, cuda_device), offsets=i32([0] * (n + 1), cuda_device),
+                    slots=torch.zeros(rows, dtype=torch.int64, device=cuda_device), k=torch_rows(kv_heads), v=torch_rows(kv_heads),
+                    q=torch_rows(heads), out=torch_rows(heads), lse=torch.zeros((rows, heads), device=cuda_device))
+
+    def step(s, space):
+        native.cache_assign(s["kv"], s["new"], s["table"], s["free"], s["count"], block_size=bs, row_offsets=s["offsets"],
+                            kv_len=s["kv"], slots=s["slots"], denied=s["denied"])
+        native.cache_store(s["cache"], s["k"], s["v"], s["slots"])
+        native.cache_attention(s["cache"], s["q"], s["offsets"], s["kv"], s["table"], max_q=50, max_kv=columns * bs, out=s["out"],
+                               lse=s["lse"], workspace=space)
+
+    s = state()
+    space = native.cache_attention_workspace(s["cache"], s["q"], requests=n, max_q=50, max_kv=columns * bs)
+    step(state(), space)                                              # first calls outside the capture, on other tensors
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        step(s, space)
+    codes = [np.zeros((blocks, kv_heads, bs, dim), np.uint8) for _ in range(2)]
+    scales = [np.ones((blocks, kv_heads)) for _ in range(2)]
+    table, free, count, kv = s["table"].cpu().numpy(), np.arange(blocks), blocks, [0] * n
+    for new in ([20, 0, 7, 1], [1, 33, 1, 1], [4, 1, -1, 1], [1, 1, 9, 0], [-1, 2, 1, 30], [5, 1, 1, -1], [1, 1, 1, 1]):
+        data = {"k": kv_heads, "v": kv_heads, "q": heads}
+        for key, h in data.items():
+            s[key].copy_(torch.from_numpy(rng.standard_normal((rows, h, dim))).to(cuda_device).clamp(-1, 1))
+        s["new"].copy_(i32(new, cuda_device))
+        s["out"].fill_(7.0)
+        graph.replay()
+        torch.cuda.synchronize()
+        a = ref.assign(kv, new, table, free, count, bs, rows)
+        for key, x in (("block_table", s["table"]), ("free_blocks", s["free"]), ("row_offsets", s["offsets"]), ("kv_len", s["kv"]),
+                       ("slots", s["slots"])):
+            assert np.array_equal(x.cpu().numpy(), a[key]), key
+        assert int(s["count"].item()) == a["free_count"] and int(s["denied"].item()) == a["denied"] == 0
+        table, free, count, kv = a["block_table"], a["free_blocks"], a["free_count"], a["kv_len"].tolist()
+        for i, (x, c, w) in enumerate(((s["k"], s["cache"].k, s["cache"].k_scale), (s["v"], s["cache"].v, s["cache"].v_scale))):
+            codes[i], scales[i] = ref.store(codes[i], scales[i], x.double().cpu().numpy(), a["slots"].tolist())
+            assert np.array_equal(c.cpu().numpy(), codes[i]) and np.array_equal(w.cpu().numpy().astype(np.float64), scales[i])
+        used = a["row_offsets"][-1]
+        args = (scales[0], scales[1], a["row_offsets"], kv, table, dim ** -0.5, True, 0)
+        q = s["q"].double().cpu().numpy()[:used]
+        want, want_lse = ref.attention(q, codes[0], codes[1], *args)
+        mass, _ = ref.attention(q, codes[0], codes[1] & 127, *args)
+        got = s["out"].double().cpu().numpy()
+        assert (np.abs(got[:used] - want) <= 2.0 ** -8 * np.abs(want) + 2.0 ** -10 * mass + 1e-7).all()
+        assert (np.abs(s["lse"].double().cpu().numpy()[:used] - want_lse) <= 2.0 ** -11).all()
+        assert (got[used:] == 7.0).all()
+    assert native.device_status() == 0

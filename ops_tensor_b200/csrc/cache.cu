@@ -521,12 +521,6 @@ CacheView cache_view(const blazeKvCache* c) {
     return v;
 }
 
-static int status_of(cudaError_t e) {
-    if (e == cudaSuccess) return ACLTENSOR_STATUS_SUCCESS;
-    cudaGetLastError();
-    return ACLTENSOR_STATUS_EXECUTION_FAILED;
-}
-
 template <class K>
 static cudaError_t allow_smem(K kernel, int bytes, bool (&done)[64]) {
     int dev = 0;

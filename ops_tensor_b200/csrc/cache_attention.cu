@@ -75,15 +75,6 @@ __device__ __forceinline__ void mma_f16(float (&d)[4], const uint32_t (&a)[4], u
         : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
 
-// Two E4M3 codes (the low or the high half of w) as two halves.
-__device__ __forceinline__ uint32_t codes_lo(uint32_t w) {
-    const __half2_raw r = __nv_cvt_fp8x2_to_halfraw2((__nv_fp8x2_storage_t)(w & 0xFFFFu), __NV_E4M3);
-    return *reinterpret_cast<const uint32_t*>(&r);
-}
-__device__ __forceinline__ uint32_t codes_hi(uint32_t w) {
-    const __half2_raw r = __nv_cvt_fp8x2_to_halfraw2((__nv_fp8x2_storage_t)(w >> 16), __NV_E4M3);
-    return *reinterpret_cast<const uint32_t*>(&r);
-}
 // 0xFF in every byte that is an E4M3 NaN.
 __device__ __forceinline__ uint32_t nan_bytes(uint32_t w) { return __vcmpeq4(w & 0x7F7F7F7Fu, 0x7F7F7F7Fu); }
 
@@ -649,12 +640,6 @@ static bool make_tmap_pages(CUtensorMap* map, const void* base, const blazeKvCac
               CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
-static int status_of(cudaError_t e) {
-    if (e == cudaSuccess) return ACLTENSOR_STATUS_SUCCESS;
-    cudaGetLastError();
-    return ACLTENSOR_STATUS_EXECUTION_FAILED;
-}
-
 // Which kernels a call needs, by the bounds of its requests' rows, and where their partial results lie.
 struct AttnPlan {
     bool few, many;
@@ -662,8 +647,6 @@ struct AttnPlan {
     int few_grid, many_grid;
     size_t few_ml, few_cuts, many_out, many_ml, many_cuts, total;      // offsets in the workspace (few_out is 0)
 };
-
-static size_t round256(size_t x) { return (x + 255) & ~size_t(255); }
 
 static int plan_attention(const blazeKvCache* c, const blazeCacheAttentionArgs* a, int sms, AttnPlan* pl) {
     const int st = check_kv_cache(c);

@@ -157,16 +157,8 @@ __device__ __forceinline__ SubTile sub_tile(const CacheAttentionParams& p, const
 
 // 16 E4M3 codes -> 16 halves.
 __device__ __forceinline__ void codes_to_half(const uint4& w, uint4& a, uint4& b) {
-    auto lo = [](uint32_t x) {
-        const __half2_raw r = __nv_cvt_fp8x2_to_halfraw2((__nv_fp8x2_storage_t)(x & 0xFFFFu), __NV_E4M3);
-        return *reinterpret_cast<const uint32_t*>(&r);
-    };
-    auto hi = [](uint32_t x) {
-        const __half2_raw r = __nv_cvt_fp8x2_to_halfraw2((__nv_fp8x2_storage_t)(x >> 16), __NV_E4M3);
-        return *reinterpret_cast<const uint32_t*>(&r);
-    };
-    a = make_uint4(lo(w.x), hi(w.x), lo(w.y), hi(w.y));
-    b = make_uint4(lo(w.z), hi(w.z), lo(w.w), hi(w.w));
+    a = make_uint4(codes_lo(w.x), codes_hi(w.x), codes_lo(w.y), codes_hi(w.y));
+    b = make_uint4(codes_lo(w.z), codes_hi(w.z), codes_lo(w.w), codes_hi(w.w));
 }
 
 template <int kDim, bool kBf16>

@@ -260,6 +260,16 @@ __device__ __forceinline__ float lg2(float x) {
     return y;
 }
 
+// Two E4M3 codes (the low or the high half of w) as two halves.
+__device__ __forceinline__ uint32_t codes_lo(uint32_t w) {
+    const __half2_raw r = __nv_cvt_fp8x2_to_halfraw2((__nv_fp8x2_storage_t)(w & 0xFFFFu), __NV_E4M3);
+    return *reinterpret_cast<const uint32_t*>(&r);
+}
+__device__ __forceinline__ uint32_t codes_hi(uint32_t w) {
+    const __half2_raw r = __nv_cvt_fp8x2_to_halfraw2((__nv_fp8x2_storage_t)(w >> 16), __NV_E4M3);
+    return *reinterpret_cast<const uint32_t*>(&r);
+}
+
 // One box of a page: `row` and on of (head, block).
 __device__ __forceinline__ void tma_load_page(uint32_t dst, const CUtensorMap* map, uint32_t bar, int row, int head, int block) {
     asm volatile(

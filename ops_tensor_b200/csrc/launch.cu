@@ -134,13 +134,6 @@ static bool make_tmap_store(CUtensorMap* map, void* base, uint64_t cols, uint64_
 }
 
 static inline bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
-static inline size_t round256(size_t x) { return (x + 255) & ~size_t(255); }
-
-static int status_of(cudaError_t e) {
-    if (e == cudaSuccess) return ACLTENSOR_STATUS_SUCCESS;
-    cudaGetLastError();
-    return ACLTENSOR_STATUS_EXECUTION_FAILED;
-}
 
 // ------------------------------------------------------------------------------------------------ MX GEMM
 

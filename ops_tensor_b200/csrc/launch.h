@@ -6,6 +6,8 @@
 #include <cstddef>
 #include <cstdint>
 
+#include "cann_ops_tensor_types.h"
+
 namespace blaze {
 
 struct DeviceContext {
@@ -17,6 +19,15 @@ struct DeviceContext {
 
 // Per-device context of the current device (created on first use; thread-safe).  nullptr if no usable device.
 DeviceContext* current_context();
+
+// A launch's outcome as an acltensorStatus_t; clears the error.
+inline int status_of(cudaError_t e) {
+    if (e == cudaSuccess) return ACLTENSOR_STATUS_SUCCESS;
+    cudaGetLastError();
+    return ACLTENSOR_STATUS_EXECUTION_FAILED;
+}
+
+inline size_t round256(size_t x) { return (x + 255) & ~size_t(255); }
 
 // cuTensorMapEncodeTiled, looked up through the runtime (the library does not link the driver); nullptr if missing.
 using EncodeTiledFn = CUresult (*)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*,

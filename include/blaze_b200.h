@@ -380,8 +380,10 @@ BLAZE_API int blazeCacheStore(const blazeKvCache* cache, const blazeCacheStoreAr
  * down to 2^-26 of the row's largest one, and by at most 2^-37 of that largest one below (2^-29 and 2^-40 where the requests'
  * rows are few).
  * max_q and max_kv bound the requests' rows and kv_len (lengths above are cut to them; max_kv may not pass max_blocks *
- * block_size); min_q is a hint: a bound from below on the rows of every request that has any, 0 if unknown.  The result
- * does not depend on how the work is split over the SMs beyond float32 rounding, and is the same from run to run.
+ * block_size); min_q is a hint: a bound from below on the rows of every request that has any, 0 if unknown.  The same
+ * call gives the same result, bit for bit.  Another split of the work (another number of SMs, other bounds, other requests
+ * in the batch) may move a result by the rounding of its probabilities, since each piece of a request rounds them against a
+ * largest one of its own.
  * The workspace needs no initialisation and keeps nothing between calls; calls that may overlap on the GPU need one
  * each.  One that suffices for some tokens, requests, max_q and max_kv (with min_q = 0) suffices for any smaller ones. */
 typedef struct {

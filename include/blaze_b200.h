@@ -403,7 +403,7 @@ typedef struct {
     int64_t table_stride;      /* elements, >= max_blocks */
     int32_t max_blocks;
     int32_t max_q, min_q, max_kv;
-    float scale;               /* finite */
+    float scale;               /* scale * log2(e) finite */
     int32_t causal;            /* 0 or 1 */
     int32_t window;            /* 0 = none */
     int32_t sm_limit;          /* 0 = all SMs */

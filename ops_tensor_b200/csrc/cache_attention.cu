@@ -33,6 +33,7 @@
 
 namespace blaze {
 
+constexpr float kLog2E = 1.4426950408889634f;
 constexpr int kFewRows = 16;          // packed rows of a row tile, at most: 8 for each n8 tile of the products
 constexpr int kFewTokens = 64;        // tokens of a tile
 constexpr int kFewWarps = 4;          // computing warps, 16 tokens of a tile each
@@ -655,7 +656,7 @@ static int plan_attention(const blazeKvCache* c, const blazeCacheAttentionArgs* 
     if (a->requests < 0 || a->tokens < 0 || a->heads < 1 || (a->heads % c->kv_heads) || a->max_q < 0 || a->min_q < 0 ||
         a->max_kv < 0 || a->max_blocks < 0 || a->window < 0 || a->sm_limit < 0 || (a->causal != 0 && a->causal != 1) ||
         a->table_stride < a->max_blocks || (int64_t)a->max_kv > (int64_t)a->max_blocks * c->block_size ||
-        !std::isfinite(a->scale))
+        !std::isfinite(a->scale * kLog2E))            // (scores are taken as powers of two)
         return ACLTENSOR_STATUS_INVALID_VALUE;
     if (a->requests > kAttnMaxRequests || (a->q_type != BLAZE_OUT_BF16 && a->q_type != BLAZE_OUT_F16))
         return ACLTENSOR_STATUS_NOT_SUPPORTED;
@@ -825,7 +826,7 @@ extern "C" int blazeCacheAttention(const blazeKvCache* cache, const blazeCacheAt
     p.max_kv = a->max_kv;
     p.causal = a->causal;
     p.window = a->window >= a->max_kv ? 0 : a->window;      // (wider than any request: none)
-    p.scale_log2 = a->scale * 1.4426950408889634f;
+    p.scale_log2 = a->scale * kLog2E;
     p.q = a->q;
     p.q_token_stride = a->q_token_stride;
     p.q_head_stride = a->q_head_stride;

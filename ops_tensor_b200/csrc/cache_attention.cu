@@ -802,7 +802,7 @@ extern "C" int blazeCacheAttention(const blazeKvCache* cache, const blazeCacheAt
         (a->out_token_stride % 8) || (a->out_head_stride % 8))
         return ACLTENSOR_STATUS_NOT_SUPPORTED;
     if (!a->workspace || a->workspace_bytes < pl.total) return ACLTENSOR_STATUS_INSUFFICIENT_WORKSPACE;
-    if (!aligned(a->workspace, 256)) return ACLTENSOR_STATUS_INVALID_VALUE;
+    if (!aligned(a->workspace, 256) || a->out == a->q) return ACLTENSOR_STATUS_INVALID_VALUE;
     if (!ctx) return ACLTENSOR_STATUS_NOT_INITIALIZED;
     if (ctx->cc_major != 10) return ACLTENSOR_STATUS_ARCH_MISMATCH;
     cudaStream_t stream = static_cast<cudaStream_t>(stream_v);

@@ -17,3 +17,8 @@ def test_scales_that_powers_of_two_cannot_hold(lib, scale, status):
     # (a call that is right otherwise ends at its workspace)
     got = lib.blazeCacheAttention(C.byref(cache()), C.byref(attention(scale=scale, out=2 * P, workspace=None)), None)
     assert got == (NO_SPACE if status == OK else status)
+
+
+def test_output_over_the_queries(lib):
+    """A query row is read by every block that has a part of its work, so the output cannot take its place."""
+    assert lib.blazeCacheAttention(C.byref(cache()), C.byref(attention(q=P, out=P)), None) == INVALID

@@ -34,6 +34,24 @@ def test_store_skips_every_slot_outside_the_cache(cuda_device, kind, heads, bs, 
     check_store(cache, codes, scales, k, v, slots)
 
 
+@pytest.mark.parametrize("kind,bs,dim", [("bf16", 16, 128), ("f16", 128, 64), ("bf16", 128, 128)])
+def test_store_runs_in_any_order(cuda_device, kind, bs, dim):
+    """Rows of one block in reverse, shuffled, with holes, and slots named again near by and far off, in runs of up to twice a
+    block: the last row of a slot stays, all of them count for the scale."""
+    import torch
+    rng = np.random.default_rng(bs + dim)
+    blocks, heads = 9, 2
+    cache, codes, scales = random_cache(rng, blocks, heads, bs, dim, cuda_device)
+    rows = [np.arange(bs)[::-1], rng.permutation(bs), rng.permutation(bs)[:bs // 2 + 1], rng.integers(0, bs, 2 * bs),
+            rng.integers(bs // 2, bs, bs), np.r_[np.arange(3, bs), np.arange(bs - 4)], np.repeat(np.arange(1, bs), 2),
+            np.array([7, 5, 7]), np.full(9, bs - 1)]
+    slots = [int(b) * bs + int(x) for b, r in zip(rng.permutation(blocks), rows) for x in r]
+    k, v = (torch.from_numpy(rng.standard_normal((len(slots), heads, dim)) * np.exp2(rng.integers(-6, 7, (len(slots), heads, 1))))
+            .to(cuda_device).to({"bf16": torch.bfloat16, "f16": torch.float16}[kind]) for _ in range(2))
+    native.cache_store(cache, k, v, torch.tensor(slots, dtype=torch.int64, device=cuda_device))
+    check_store(cache, codes, scales, k, v, slots)
+
+
 class Guarded:
     """A tensor inside a larger one whose borders have to stay as they are."""
 

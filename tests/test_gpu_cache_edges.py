@@ -208,3 +208,54 @@ def test_captured_step(cuda_device, dim, bs, heads, kv_heads, rows):
         assert (np.abs(s["lse"].double().cpu().numpy()[:used] - want_lse) <= 2.0 ** -11).all()
         assert (got[used:] == 7.0).all()
     assert native.device_status() == 0
+
+
+def test_layers_without_waiting(cuda_device):
+    """Steps of a layer (QKV product, assign, store, attention, quantiser, output product) issued without waiting for anything,
+    with buffers used again at once, against the same steps with a wait behind every call: equal bit for bit.  The kernels
+    start before the one in front of them has ended (programmatic stream serialisation) and may touch nothing until it
+    has."""
+    import torch
+    heads, kv_heads, dim, bs, width, steps = 8, 2, 128, 64, 512, 12
+    g = torch.Generator(device=cuda_device)
+    g.manual_seed(9)
+    w = (torch.randn(((heads + 2 * kv_heads) * dim, width), generator=g, device=cuda_device) * width ** -0.5).to(torch.bfloat16)
+    wo, so = native.quantize_fp8_blocks(torch.randn((width, heads * dim), generator=g, device=cuda_device) * 0.03)
+    news = [[200, 3, 70]] + [[1, 1, 1], [4, 0, 90], [1, 30, 1], [-1, 1, 1], [130, 1, 2]] * 3
+    inputs = [(torch.randn((240, width), generator=g, device=cuda_device).to(torch.bfloat16), i32(n, cuda_device))
+              for n in news[:steps]]
+
+    def run(wait):
+        cache = native.PagedCache.empty(40, kv_heads, bs, dim, cuda_device)
+        table = torch.full((3, 16), -1, dtype=torch.int32, device=cuda_device)
+        free, count = torch.arange(40, dtype=torch.int32, device=cuda_device), i32([40], cuda_device)
+        kv, offsets = i32([0] * 3, cuda_device), i32([0] * 4, cuda_device)
+        slots = torch.zeros(280, dtype=torch.int64, device=cuda_device)[:240]
+        out = torch.zeros((240, heads, dim), dtype=torch.bfloat16, device=cuda_device)
+        results, space = [], None
+        pause = torch.cuda.synchronize if wait else (lambda: None)
+        for x, new in inputs:
+            qkv = native.dense_gemm(x, w).view(240, heads + 2 * kv_heads, dim)
+            pause()
+            q, k, v = qkv[:, :heads], qkv[:, heads:heads + kv_heads], qkv[:, heads + kv_heads:]
+            native.cache_assign(kv, new, table, free, count, block_size=bs, row_offsets=offsets, kv_len=kv, slots=slots)
+            pause()
+            native.cache_store(cache, k, v, slots)
+            pause()
+            if space is None:
+                space = native.cache_attention_workspace(cache, q, requests=3, max_q=200, max_kv=1024)
+            out.zero_()
+            native.cache_attention(cache, q, offsets, kv, table, max_q=200, max_kv=1024, out=out, workspace=space)
+            pause()
+            codes, scale = native.quantize_fp8_row_groups(out.view(240, heads * dim).float())
+            pause()
+            results += [out.clone(), native.fp8_gemm(codes, scale, wo, so)]
+            pause()
+        torch.cuda.synchronize()
+        return results + [cache.k, cache.v, cache.k_scale, cache.v_scale, table, kv, count, slots]
+
+    want = run(True)
+    for _ in range(4):
+        for a, b in zip(run(False), want):
+            assert torch.equal(a, b)
+    assert all(bool((x != 0).any()) for x in want) and native.device_status() == 0

@@ -74,15 +74,14 @@ __device__ __forceinline__ int last_at_or_below(const int* start, int n, int x) 
     return lo;
 }
 
-// Integer work, a few bytes per token: bound by latency (256 requests of one token, one block: 5.8 us) and, for prompts, by
-// the binary search and the table load of each row (1000 requests, 640k rows, 148 blocks: 14.6 us, 0.6 TB/s; four rows
-// a thread with one search made both slower, 7.8 and 16.7 us, their loads being one behind the other).  Every block makes the sums over all requests for itself in
-// shared memory (8 bytes read per request, out of L2 after the first), so blocks need nothing from one another: blocks
-// popped from the stack are found by their number from the top, a popped block that an ended request gives back in the
-// same call through the sum over the given-back blocks.  Reads and writes do not meet: the stack is read below
-// free_count and written at or above it, table rows are read of one set of requests (old entries) and written for
-// another (new entries).  The lengths, which may be updated in place, are written by a block that has read them all:
-// the only one, or a second launch (`write_lists` = 0).
+// Integer work, a few bytes per token: bound by latency (256 requests of one token, one block: 5.8 us) and, for
+// prompts, by the binary search and the table load of each row (1000 requests, 640k rows, 148 blocks: 14.6 us, 0.6
+// TB/s).  Every block makes the sums over all requests for itself in shared memory (8 bytes read per request, out of L2
+// after the first), so blocks need nothing from one another: blocks popped from the stack are found by their number
+// from the top, a popped block that an ended request gives back in the same call through the sum over the given-back
+// blocks.  Reads and writes do not meet: the stack is read below free_count and written at or above it, table rows are
+// read of one set of requests (old entries) and written for another (new entries).  The lengths, which may be updated
+// in place, are written by a block that has read them all: the only one, or a second launch (`write_lists` = 0).
 __global__ void __launch_bounds__(kAssignThreads) cache_assign_kernel(const CacheAssignParams p) {
     extern __shared__ int assign_smem[];
     __shared__ long long warp_sums[32];
@@ -310,8 +309,10 @@ __device__ __forceinline__ uint2 encode8(const uint4& v, float inv, float scale)
 // eight rows from the one read (a block of 64 tokens then needs no second), the largest magnitude goes through shared
 // memory.  Shorter runs (a decode step's single rows) go to one warp each.
 // Bytes: 4 read and 2 written per (token, head, dim) of K and V together.  26k rows of 8 heads of 128: 46 us, 3.4 TB/s, bound
-// by the dependent loads of a run (slots, rows, old scale) at the 32 warps of an SM that 64 registers allow; with one warp
-// for a run and its rows read twice 91 us, with magnitudes compared one by one 59.  128 single rows: 6.1 us, latency.
+// by the dependent loads of a run (slots, rows, old scale) at the 32 warps of an SM that 64 registers allow (64 bytes spilled).
+// 128 single rows: 6.1 us, latency.  Runs by one warp each / shared: of 2 rows (200 in all) 4.8 / 5.7 us, of 4 (400) 6.3 / 7.1,
+// of 8 (800) 6.7 / 8.2, of 12 (480) the same; but with a limit of 16 the short runs at the ends of prompts hold the others
+// up (4800 rows of four 11.9 us against 9.7).
 constexpr int kStoreShort = 4;
 
 template <int kDim, bool kBf16>
@@ -620,6 +621,9 @@ extern "C" int blazeCacheStore(const blazeKvCache* cache, const blazeCacheStoreA
     p.slots = static_cast<const long long*>(a->slots);
     p.tokens = a->tokens;
     p.slot_count = (long long)cache->num_blocks * cache->block_size;
+    // Rows per block: few where the call has too few for all SMs, many where each block would repeat the search for its runs.
+    // 4 / 16 / 64 rows: 400 single rows 9.1 / 14.8 / 41 us; 1500 rows of a prompt 10.0 / 6.4 / 6.7; 4800 of four 23.7 / 12.0 / 9.7;
+    // 26k of sixteen 128 / 58 / 47; but 4500 single rows 73 / 68 / 79.
     p.window = a->tokens >= 4096 ? 64 : (a->tokens >= 512 ? 16 : 4);
     const long long blocks = (long long)((a->tokens + p.window - 1) / p.window) * 2 * cache->kv_heads;
     if (blocks > 0x7FFFFFFFll) return ACLTENSOR_STATUS_NOT_SUPPORTED;

@@ -6,7 +6,9 @@
 //
 // for the codes k8, v8 of block b's tokens: with the V scale in the exponent neither K nor V is ever multiplied by its
 // scale, the codes enter the matrix products as they are (E4M3 is a subset of half), and what is rounded to half is
-// p_j relative to the largest p_j * v_scale of its row.
+// p_j relative to the largest p_j * v_scale of its row.  Rounding it is a choice: the codes' own type is the one that the
+// products take, and holding p in two halves would double the products with V.  Against 64 bits it costs nothing that bf16
+// outputs show (1.4e-3 with p in half as with p in float32), half outputs go from 1.9e-4 to 2.0e-4.
 //
 // The few-rows kernel (decode steps and short runs of tokens) is bound by the bytes of the cache.  A block has one
 // warp that fetches tiles of 64 tokens into a ring in shared memory by TMA (one box per page and operand, 128-byte
@@ -16,9 +18,9 @@
 // are many, its 8 columns the query rows, of which there are few; the probabilities change sides by an 8x8 matrix
 // transposition in registers.  The order of the k index of a product is free, so a lane reads 16 consecutive code bytes
 // and converts them in registers; the swizzle makes these reads free of bank conflicts for both operands.
-// Four contexts of 90k to 131k tokens, 64 query and 8 kv heads of 128: 142 us, 6.2 TB/s (141 without the products); 64
-// requests of 200 to 8192 tokens: 117 us, 5.1 TB/s (114 without).  The query rows in the instruction's 16 rows took 174 and
-// 153 us: twice the instructions and registers for the same bytes.
+// Four contexts of 90k to 131k tokens, 64 query and 8 kv heads of 128: 143 us, 6.2 TB/s (141 without the products); 64
+// requests of 200 to 8192 tokens: 118 us, 5.1 TB/s (114 without).  The instance for 9 to 16 rows of 128 spills 96 to 104 bytes at
+// its 168 registers.
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 #include <cuda_runtime.h>
@@ -39,15 +41,21 @@ constexpr int kFewTokens = 64;        // tokens of a tile
 constexpr int kFewWarps = 4;          // computing warps, 16 tokens of a tile each
 constexpr int kFewThreads = 32 * (kFewWarps + 1);
 constexpr int kFewStages = 4;
-constexpr int kFewMinChunk = 2;       // tiles of a block's chunk, at least
+// Tiles of a block's chunk, at least.  1, 2 and 4 of them: one token on 1000 tokens 11.0, 9.2 and 9.0 us, on 300 tokens 7.9,
+// 10.2 and 10.7; a prompt of 512 tokens (many rows) 39.5, 39.6 and 50.
+constexpr int kFewMinChunk = 2;
 constexpr int kManyMinChunk = 2;
 // Requests of more packed rows go to the many-rows kernel: this one reads the cache once per 16 rows, that one once per 256 at
-// the price of 256 rows' products.
+// the price of 256 rows' products.  Measured, few-rows / many-rows kernel in us, 2 kv heads, 16 requests of 2k tokens, 4 of 30k
+// and 32 of 8k: heads of 128, 24 rows 30 / 26, 48 / 57, 84 / 92; 32 rows 32 / 26, 49 / 58, 87 / 94; 40 rows 34 / 27, 61 / 59,
+// 113 / 94; 72 rows 42 / 28, 84 / 64, 166 / 97.  Heads of 64, 32 rows 22 / 22, 35 / 46, 55 / 72; 48 rows 25 / 22, 41 / 47, 71 / 74;
+// 64 rows 27 / 22, 47 / 48, 87 / 75.  So up to 32 rows of 128 each is ahead by 10 to 20 % somewhere, and for heads of 64 this
+// one would be ahead up to 48 rows on long contexts.
 constexpr int kFewLimit = kFewRows;
 // Small calls stay with the few-rows kernel whatever their rows: up to so many tiles of 64 tokens per block, counting 16 rows
-// a row tile and every request as long as the longest.  Measured, few-rows against many-rows kernel: 0.2 tiles (420 rows
-// on 105 tokens) 12.1 / 22.0 us; 3.9 (17 requests of up to 374 rows on up to 291 tokens) 27 / 55; 11.6 (8 of up to 160 rows
-// on up to 340) 41 / 33; 31 (2048 rows on 512) 99 / 40.
+// a row tile and every request as long as the longest.  Measured, few-rows / many-rows kernel: 0.2 tiles (420 rows on 105
+// tokens) 12 / 21 us; 3.9 (17 requests of up to 374 rows on up to 291 tokens) 27 / 53; 11.6 (8 of up to 160 rows on up to 340)
+// 41 / 33; 31 (2048 rows on 512) 96 / 40.
 constexpr double kFewSmall = 6.0;
 
 // Probabilities are kept up to 2^15 (the running maximum less 15), so that in half the values down to 2^-29 of a row's

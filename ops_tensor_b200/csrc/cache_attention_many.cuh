@@ -14,11 +14,12 @@
 //                    and scales of the tiles
 // The softmax threads also bring their own query row into shared memory at the start of a piece.
 // Q K^T takes K as the K-major operand; P V takes V as it lies, dims contiguous (MN-major), no transposition anywhere.
-// 769 rows of 16 heads of 128 on 15k and 30k tokens: 221 us, 720 TFLOP/s, tensor pipe 36 % busy; 4 prompts of up to 4096
-// rows of 32 heads: 624 us, 450 TFLOP/s.  Bound by the chain of a sub-tile: softmax (2700 cycles per 128 tokens), hand-over to
-// the issuing warp, MMAs (1170), hand-over back, which the other sub-tile's fills only partly: without exponentials and with
-// one MMA of eight the chunk case takes 143 us, with nothing but maxima and hand-overs 113.  An issuing warp for each
-// sub-tile took 243 us (their MMAs take turns in the tensor pipe), hand-overs of 64 tokens 239.
+// 769 rows of 16 heads of 128 on 15k and 30k tokens: 221 us, 720 TFLOP/s, tensor pipe and exponentials 37 % busy each; 4 prompts
+// of up to 4096 rows of 32 heads: 625 us, 450 TFLOP/s.  Bound, within a piece, by the chain of a sub-tile: softmax, hand-over to the
+// issuing warp, MMAs, hand-over back, which the other sub-tile's fills only partly (2.9 us per 128 tokens); between pieces
+// by the epilogue and the next queries, one behind the other (10 us a piece in the prompts, whose blocks have equal tiles but
+// up to 25 pieces: they end after 335 to 619 us).  Spills at the 128 registers that ptxas allocates for: 44 to 52 bytes stored
+// for heads of 128, 16 for heads of 64.
 #pragma once
 
 #include "cache_schedule.cuh"

@@ -1,6 +1,7 @@
 """GPU: what the first calls of a process prepare, in processes of their own."""
 import subprocess
 import sys
+from pathlib import Path
 
 import pytest
 
@@ -8,9 +9,8 @@ pytestmark = pytest.mark.gpu
 
 PROGRAM = """
 import sys
-import numpy as np
 import torch
-sys.path[:0] = ["tests", "."]
+sys.path.insert(0, ".")
 from ops_tensor_b200 import native
 
 dim, kind = int(sys.argv[1]), getattr(torch, sys.argv[2])
@@ -48,5 +48,6 @@ print("captured")
 @pytest.mark.parametrize("dim,kind", [(64, "float16"), (128, "bfloat16")])
 def test_one_decode_step_prepares_every_capture(cuda_device, dim, kind):
     """After one call with a head size and type, calls that take its other kernels may be captured at once."""
-    r = subprocess.run([sys.executable, "-c", PROGRAM, str(dim), kind], capture_output=True, text=True, timeout=300)
+    r = subprocess.run([sys.executable, "-c", PROGRAM, str(dim), kind], capture_output=True, text=True, timeout=300,
+                       cwd=Path(__file__).resolve().parent.parent)
     assert r.returncode == 0 and "captured" in r.stdout, r.stdout + r.stderr
